@@ -20,7 +20,9 @@ SOURCES = ["fit_kernels.hip", "fit_kernels_wide.hip", "warp_tile.hip", "warp_til
 HEADERS = ["device.hpp", "kernels.hpp", "pool.hpp", "warp_tile_kernel.hpp", "warp_tile_ahead.hpp", "warp_tile_narrow.hpp", "feat_kernel.hpp", os.path.join("..", "..", "include", "lfm_hip.h")]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
-         "-munsafe-fp-atomics", "-Wall", "-Wno-unused-function"]
+         "-munsafe-fp-atomics", "-Wall", "-Wno-unused-function",
+         # no packed float32 instructions: some of their forms have given wrong results on MI355X
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 if os.environ.get("LFM_BUILD_DEBUG"):  # line tables + symbols for rocgdb (same code generation)
     FLAGS.append("-g")
 # A/B builds: LFM_BUILD_DEFINES="-DX -DY" LFM_BUILD_DIR=<dir under lightfm_amd/> python -m lightfm_amd.build
