@@ -1,4 +1,4 @@
-"""Builds lightfm_amd/_lib/liblfm_hip.so with hipcc for gfx950 (in-tree).
+"""Builds lightfm_amd/_lib/liblfm_hip.so and liblfm_ops.so with hipcc for gfx950 (in-tree).
 
     python -m lightfm_amd.build [--force]
 
@@ -15,9 +15,13 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "_lib")
 LIB = os.path.join(OUT_DIR, "liblfm_hip.so")
+OPS_LIB = os.path.join(OUT_DIR, "liblfm_ops.so")
 SOURCES = ["fit_kernels.hip", "fit_kernels_wide.hip", "warp_tile.hip", "warp_tile_lpr16.hip", "warp_tile_lpr32.hip",
            "warp_tile_lpr64.hip", "warp_tile_ahead.hip", "warp_tile_bpr.hip", "logistic_tile.hip", "feat_kernels.hip", "feat_kernels_wide.hip", "feat_kernels_hot.hip", "feat_kernels_ada.hip", "hot_slices.hip", "predict_kernels.hip", "csr_build.hip", "session.hip"]
-HEADERS = ["device.hpp", "kernels.hpp", "pool.hpp", "warp_tile_kernel.hpp", "warp_tile_ahead.hpp", "warp_tile_narrow.hpp", "feat_kernel.hpp", os.path.join("..", "..", "include", "lfm_hip.h")]
+# the device-memory operators: in liblfm_ops.so with their C ABI
+OPS_SOURCES = ["softmax_loss.hip", "embedding_ops.hip", "clip_norm.hip"]
+OPS_API = ["lfm_ops.hip"]
+HEADERS = ["ops_common.hpp", os.path.join("..", "..", "include", "lfm_ops.h"), "device.hpp", "kernels.hpp", "pool.hpp", "warp_tile_kernel.hpp", "warp_tile_ahead.hpp", "warp_tile_narrow.hpp", "feat_kernel.hpp", os.path.join("..", "..", "include", "lfm_hip.h")]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
          "-munsafe-fp-atomics", "-Wall", "-Wno-unused-function",
@@ -30,6 +34,7 @@ FLAGS += os.environ.get("LFM_BUILD_DEFINES", "").split()
 if os.environ.get("LFM_BUILD_DIR"):
     OUT_DIR = os.path.join(HERE, os.environ["LFM_BUILD_DIR"])
     LIB = os.path.join(OUT_DIR, "liblfm_hip.so")
+    OPS_LIB = os.path.join(OUT_DIR, "liblfm_ops.so")
 
 
 def _stale(target, deps):
@@ -42,21 +47,33 @@ def _stale(target, deps):
 def build(force=False, verbose=False):
     os.makedirs(OUT_DIR, exist_ok=True)
     hdrs = [os.path.join(CSRC, h) for h in HEADERS]
-    objs, jobs = [], []
-    for src in SOURCES:
+    objs, jobs = {}, []
+    for src in SOURCES + OPS_SOURCES + OPS_API:
         s = os.path.join(CSRC, src)
         o = os.path.join(OUT_DIR, src.replace(".hip", ".o"))
-        objs.append(o)
+        objs[src] = o
         if force or _stale(o, [s] + hdrs):
             jobs.append([HIPCC] + FLAGS + ["-c", s, "-o", o])
     def run(cmd):
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.check_call(cmd)
-    with ThreadPoolExecutor(max_workers=len(SOURCES)) as ex:
+    with ThreadPoolExecutor(max_workers=len(objs)) as ex:
         list(ex.map(run, jobs))
-    if jobs or force or _stale(LIB, objs):
-        run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs + ["-ldl"])
+    mine = [objs[s] for s in SOURCES]
+    if force or _stale(LIB, mine):
+        run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + mine + ["-ldl"])
+    mine = [objs[s] for s in OPS_SOURCES + OPS_API]
+    if force or _stale(OPS_LIB, mine):
+        # liblfm_ops.so works on torch's memory and streams, so it has to bind to the HIP runtime torch has loaded --
+        # which is torch's own copy, known to the loader as "libamdhip64.so" (liblfm_hip.so asks for the system's
+        # versioned name).  An empty stand-in of that name gives the library the right dependency.
+        stand_in = os.path.join(OUT_DIR, "link", "libamdhip64.so")
+        os.makedirs(os.path.dirname(stand_in), exist_ok=True)
+        run(["gcc", "-shared", "-fPIC", "-x", "c", os.devnull, "-Wl,-soname,libamdhip64.so", "-o", stand_in])
+        run([HIPCC, "--offload-arch=gfx950", "-no-hip-rt", "-shared", "-fPIC", "-o", OPS_LIB] + mine
+            + ["-Wl,--no-as-needed", stand_in])
+        os.remove(stand_in)
     return LIB
 
 

@@ -1,0 +1,535 @@
+// embedding_ops.hip -- rows of an embedding table times a scale (single ids or weighted bags of ids) and the gradient
+// by sorted ids.  Both move memory and compute next to nothing: the lookup reads each picked row and writes each
+// output row once; the gradient reads each row of d_out once per id and writes the table's gradient once.
+#include "ops_common.hpp"
+
+namespace lfm {
+namespace ops {
+namespace {
+
+// ------------------------------------------------------------------ lookup ---
+
+// A group of `lanes` (a power of two <= 64) neighbouring lanes owns one output row, VEC elements (16 bytes where the
+// addresses allow it) per lane and step: 16 lanes read a row of 64 floats in one access.  Accumulates in float32 in the
+// order of the bag and rounds once, after the scale.
+template <typename T, typename I, int VEC, bool BAGS>
+__global__ __launch_bounds__(256) void lookup_kernel(lfm_lookup_args a, int lanes_log2)
+{
+    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t row = t >> lanes_log2;
+    if (row >= a.rows) return;
+    const int lanes = 1 << lanes_log2, lane = (int)(t & (lanes - 1));
+    const I *ids = (const I *)a.ids;
+    typedef Vec<T, VEC> V;
+    int64_t lo = row, hi = row + 1;
+    if (BAGS) {  // an indptr that is not monotone inside [0, nnz] never leaves the arrays
+        const int64_t l = (int64_t)((const I *)a.indptr)[row], h = (int64_t)((const I *)a.indptr)[row + 1];
+        lo = l < 0 ? 0 : (l > a.nnz ? a.nnz : l);
+        hi = h > a.nnz ? a.nnz : h;
+    }
+    for (int c = lane * VEC; c < a.d; c += lanes * VEC) {
+        float acc[VEC];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
+        int64_t j = lo;
+        if (BAGS) {
+            for (; j + 4 <= hi; j += 4) {  // four rows in flight
+                V r[4];
+                float w[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int64_t id = (int64_t)ids[j + q];
+                    const bool ok = (uint64_t)id < (uint64_t)a.vocab;
+                    w[q] = a.values ? a.values[j + q] : 1.0f;
+                    if (ok) r[q] = *(const V *)((const T *)a.table + id * a.table_stride + c);
+                    else {
+                        w[q] = 0.0f;
+#pragma unroll
+                        for (int k = 0; k < VEC; ++k) r[q].v[k] = (T)0.0f;
+                    }
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) acc[k] = fmaf(w[q], (float)r[q].v[k], acc[k]);
+            }
+        }
+        for (; j < hi; ++j) {
+            const int64_t id = (int64_t)ids[j];
+            if ((uint64_t)id >= (uint64_t)a.vocab) continue;
+            const float w = BAGS && a.values ? a.values[j] : 1.0f;
+            const V r = *(const V *)((const T *)a.table + id * a.table_stride + c);
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) acc[k] = fmaf(w, (float)r.v[k], acc[k]);
+        }
+        V o;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) o.v[k] = (T)(acc[k] * a.scale);
+        *(V *)((T *)a.out + row * a.d + c) = o;
+    }
+}
+
+int lanes_for(int d, int vec)
+{
+    int l = 0;
+    while ((1 << l) * vec < d && l < 6) ++l;
+    return l;
+}
+
+bool aligned(const void *p, int64_t stride, int d, int item, int vec)
+{
+    return ((uintptr_t)p % (uintptr_t)(item * vec)) == 0 && stride % vec == 0 && d % vec == 0;
+}
+
+template <typename T, typename I, int VEC>
+hipError_t launch_lookup(const lfm_lookup_args &a, hipStream_t st)
+{
+    const int ll = lanes_for(a.d, VEC);
+    const int64_t blocks = ceil_div(a.rows << ll, 256);
+    if (a.indptr) lookup_kernel<T, I, VEC, true><<<dim3((unsigned)blocks), 256, 0, st>>>(a, ll);
+    else lookup_kernel<T, I, VEC, false><<<dim3((unsigned)blocks), 256, 0, st>>>(a, ll);
+    return hipGetLastError();
+}
+
+template <typename T, typename I>
+hipError_t lookup_typed(const lfm_lookup_args &a, hipStream_t st)
+{
+    constexpr int W = 16 / (int)sizeof(T);
+    if (aligned(a.table, a.table_stride, a.d, sizeof(T), W) && aligned(a.out, a.d, a.d, sizeof(T), W))
+        return launch_lookup<T, I, W>(a, st);
+    if (aligned(a.table, a.table_stride, a.d, sizeof(T), W / 2) && aligned(a.out, a.d, a.d, sizeof(T), W / 2))
+        return launch_lookup<T, I, W / 2>(a, st);
+    return launch_lookup<T, I, 1>(a, st);
+}
+
+// ---------------------------------------------------------------- gradient ---
+//
+// 1. the ids are sorted by value with their positions, stable: a least-significant-digit radix sort of one to three
+//    digits of up to 11 bits (200 003 ids: two digits of 9 bits).  A block owns one contiguous piece of the list, its
+//    eight waves one contiguous part of the piece each, so "earlier block, earlier wave, earlier lane" is the order of
+//    the positions.  The scatter kernel sums the blocks' digit counts itself (at most 128 blocks): a digit takes two
+//    launches, and no count depends on the order in which atomics land.
+// 2. the sorted list is cut into chunks of CHUNK ids; a lane group sums a chunk's runs of equal ids in float32, in
+//    order.  A run inside one chunk is written to its row at once, a run that crosses chunks leaves partial sums.
+// 3. the block of the chunk where a crossing run starts adds the run's partial sums, in a fixed order.
+// Rows without ids are zero: the first launch fills the output.
+
+constexpr int SORT_WAVES = 8, SORT_THREADS = 64 * SORT_WAVES, MAX_BINS = 2048, MAX_BLOCKS = 128, CHUNK = 32;
+
+struct SortPlan {
+    int passes, bits, bins;  // digits, bits of a digit, 1 << bits
+    int blocks;
+    int64_t items;           // ids of a block, a multiple of SORT_THREADS
+};
+
+SortPlan sort_plan(int64_t vocab, int64_t nnz)
+{
+    SortPlan p;
+    int all = 1;
+    while (all < 32 && ((uint64_t)vocab >> all) != 0) ++all;  // keys 0 .. vocab (= an id to leave out)
+    p.passes = (all + 10) / 11;
+    p.bits = (all + p.passes - 1) / p.passes;
+    p.bins = 1 << p.bits;
+    int64_t want = ceil_div(nnz, 4096);
+    if (want < 1) want = 1;
+    if (want > MAX_BLOCKS) want = MAX_BLOCKS;
+    p.items = ceil_div(ceil_div(nnz, want), SORT_THREADS) * SORT_THREADS;
+    if (p.items < SORT_THREADS) p.items = SORT_THREADS;  // no ids at all
+    p.blocks = (int)ceil_div(nnz, p.items);
+    if (p.blocks < 1) p.blocks = 1;
+    return p;
+}
+
+template <typename I>
+__device__ inline uint32_t key_of(const I *ids, int64_t j, int64_t vocab)
+{
+    const int64_t id = (int64_t)ids[j];
+    return (uint64_t)id < (uint64_t)vocab ? (uint32_t)id : (uint32_t)vocab;
+}
+
+// Digit counts of every block's piece (blocks [0, sort_blocks)); in the first pass (FIRST) the other blocks fill the
+// output with zeros and write the bag of every position.
+template <typename I, bool FIRST>
+__global__ __launch_bounds__(SORT_THREADS) void count_kernel(const I *ids, const uint32_t *keys, int64_t n, int64_t vocab,
+                                                            int shift, int bins, int64_t items, uint32_t *hist,
+                                                            int sort_blocks, uint4 *fill, int64_t fill_words,
+                                                            char *fill_tail, int fill_tail_bytes, const I *indptr,
+                                                            int64_t rows, int32_t *bag_of)
+{
+    if (FIRST && (int)blockIdx.x >= sort_blocks) {
+        const int64_t t = (int64_t)((int)blockIdx.x - sort_blocks) * SORT_THREADS + threadIdx.x;
+        const int64_t step = (int64_t)((int)gridDim.x - sort_blocks) * SORT_THREADS;
+        for (int64_t i = t; i < fill_words; i += step) fill[i] = make_uint4(0, 0, 0, 0);
+        if (t < fill_tail_bytes) fill_tail[t] = 0;
+        if (indptr) {
+            for (int64_t j = t; j < n; j += step) {  // the last row whose bag starts at or before j
+                int64_t lo = 0, hi = rows - 1;
+                while (lo < hi) {
+                    const int64_t mid = (lo + hi + 1) >> 1;
+                    if ((int64_t)indptr[mid] <= j) lo = mid;
+                    else hi = mid - 1;
+                }
+                bag_of[j] = (int64_t)indptr[lo] <= j && j < (int64_t)indptr[lo + 1] ? (int32_t)lo : -1;
+            }
+        }
+        return;
+    }
+    __shared__ uint32_t count[MAX_BINS];
+    for (int b = threadIdx.x; b < bins; b += SORT_THREADS) count[b] = 0;
+    __syncthreads();
+    const int64_t lo = (int64_t)blockIdx.x * items, hi = lo + items < n ? lo + items : n;
+    for (int64_t j = lo + threadIdx.x; j < hi; j += SORT_THREADS) {
+        const uint32_t k = FIRST ? key_of(ids, j, vocab) : keys[j];
+        atomicAdd(&count[(k >> shift) & (uint32_t)(bins - 1)], 1u);
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < bins; b += SORT_THREADS) hist[(int64_t)blockIdx.x * bins + b] = count[b];
+}
+
+template <typename I, bool FIRST>
+__global__ __launch_bounds__(SORT_THREADS) void scatter_kernel(const I *ids, const uint32_t *keys, const uint32_t *pos,
+                                                              int64_t n, int64_t vocab, int shift, int bits,
+                                                              int64_t items, const uint32_t *hist, int blocks,
+                                                              uint32_t *keys_out, uint32_t *pos_out)
+{
+    __shared__ uint32_t count[SORT_WAVES][MAX_BINS];  // per wave: ids of the digit, then where the next one goes
+    __shared__ uint32_t wave_sum[SORT_WAVES];
+    const int bins = 1 << bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int i = threadIdx.x; i < SORT_WAVES * bins; i += SORT_THREADS) count[i / bins][i % bins] = 0;
+    __syncthreads();
+    const int64_t part = items / SORT_WAVES;
+    const int64_t lo = (int64_t)blockIdx.x * items + wave * part;
+    const int64_t hi = lo + part < n ? lo + part : n;
+    for (int64_t j = lo + lane; j < hi; j += 64) {
+        const uint32_t k = FIRST ? key_of(ids, j, vocab) : keys[j];
+        atomicAdd(&count[wave][(k >> shift) & (uint32_t)(bins - 1)], 1u);
+    }
+    // a thread's bins: `per` neighbouring ones
+    const int per = bins > SORT_THREADS ? bins / SORT_THREADS : 1;
+    uint32_t before[4] = {0, 0, 0, 0}, total[4] = {0, 0, 0, 0}, sum = 0;
+    const int first = threadIdx.x * per;
+    if (first < bins) {
+        for (int b = 0; b < blocks; ++b)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (q < per) {
+                    const uint32_t h = hist[(int64_t)b * bins + first + q];
+                    total[q] += h;
+                    if (b < (int)blockIdx.x) before[q] += h;
+                }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) sum += total[q];
+    }
+    uint32_t scan = sum;  // inclusive scan over the threads
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t up = __shfl_up(scan, o);
+        if (lane >= o) scan += up;
+    }
+    if (lane == 63) wave_sum[wave] = scan;
+    __syncthreads();  // also: the waves' counts are complete
+    uint32_t at = scan - sum;
+    for (int w = 0; w < wave; ++w) at += wave_sum[w];
+    if (first < bins) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (q < per) {
+                uint32_t next = at + before[q];
+                for (int w = 0; w < SORT_WAVES; ++w) {
+                    const uint32_t c = count[w][first + q];
+                    count[w][first + q] = next;
+                    next += c;
+                }
+                at += total[q];
+            }
+    }
+    __syncthreads();
+    for (int64_t j0 = lo; j0 < hi; j0 += 64) {
+        const int64_t j = j0 + lane;
+        const bool ok = j < hi;
+        const uint32_t k = !ok ? 0u : FIRST ? key_of(ids, j, vocab) : keys[j];
+        const uint32_t p = !ok ? 0u : FIRST ? (uint32_t)j : pos[j];
+        const uint32_t digit = (k >> shift) & (uint32_t)(bins - 1);
+        uint64_t same = __ballot(ok);  // the lanes with this lane's digit
+        for (int b = 0; b < bits; ++b) {
+            const uint64_t has = __ballot((digit >> b) & 1u);
+            same &= ((digit >> b) & 1u) ? has : ~has;
+        }
+        const int leader = ok ? __ffsll((unsigned long long)same) - 1 : lane;
+        uint32_t base = 0;
+        if (ok && lane == leader) base = atomicAdd(&count[wave][digit], (uint32_t)__popcll(same));
+        base = __shfl(base, leader);
+        if (ok) {
+            const uint32_t to = base + (uint32_t)__popcll(same & ((1ull << lane) - 1ull));
+            if (to < (uint64_t)n) {
+                keys_out[to] = k;
+                pos_out[to] = p;
+            }
+        }
+    }
+}
+
+struct SumArgs {
+    const uint32_t *keys, *pos;
+    const int32_t *bag_of;  // or NULL: the position is the row
+    const float *values;
+    const void *d_out;
+    void *out;
+    float *head, *tail;     // [chunks, d]: the part of a run that began earlier / that goes on
+    int64_t n, vocab, rows, stride;
+    int d;
+    float scale;
+};
+
+template <typename T, int VEC>
+__device__ inline void store_row(const SumArgs &a, uint32_t key, int c, const float *acc)
+{
+    Vec<T, VEC> o;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) o.v[k] = (T)(acc[k] * a.scale);
+    *(Vec<T, VEC> *)((T *)a.out + (int64_t)key * a.d + c) = o;
+}
+
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void chunk_sum_kernel(SumArgs a, int lanes_log2)
+{
+    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t chunk = t >> lanes_log2, lo = chunk * CHUNK;
+    if (lo >= a.n) return;
+    const int lanes = 1 << lanes_log2, lane = (int)(t & (lanes - 1));
+    const int64_t hi = lo + CHUNK < a.n ? lo + CHUNK : a.n;
+    const uint32_t none = (uint32_t)a.vocab;
+    const uint32_t earlier = lo ? a.keys[lo - 1] : none, later = hi < a.n ? a.keys[hi] : none;
+    typedef Vec<T, VEC> V;
+    for (int c = lane * VEC; c < a.d; c += lanes * VEC) {
+        float acc[VEC];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
+        uint32_t run = a.keys[lo];
+        bool began = lo == 0 || earlier != run;  // the run's first id is in this chunk
+        for (int64_t j0 = lo; j0 < hi; j0 += 8) {
+            V r[8];
+            float w[8];
+            uint32_t key[8];
+            const int m = hi - j0 < 8 ? (int)(hi - j0) : 8;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                key[q] = none;
+                w[q] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) r[q].v[k] = (T)0.0f;
+                if (q < m) {
+                    key[q] = a.keys[j0 + q];
+                    const uint32_t p = a.pos[j0 + q];
+                    const int64_t row = a.bag_of ? (int64_t)a.bag_of[p] : (int64_t)p;
+                    if (key[q] != none && (uint64_t)row < (uint64_t)a.rows) {
+                        w[q] = a.values ? a.values[p] : 1.0f;
+                        r[q] = *(const V *)((const T *)a.d_out + row * a.stride + c);
+                    }
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                if (q >= m) break;
+                if (key[q] != run) {  // the run ends here
+                    if (began) {
+                        if (run != none) store_row<T, VEC>(a, run, c, acc);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < VEC; ++k) a.head[chunk * a.d + c + k] = acc[k];
+                    }
+                    run = key[q];
+                    began = true;
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
+                }
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) acc[k] = fmaf(w[q], (float)r[q].v[k], acc[k]);
+            }
+        }
+        if (run == none) continue;
+        if (began && later != run) store_row<T, VEC>(a, run, c, acc);
+        else {
+            float *to = (began ? a.tail : a.head) + chunk * a.d + c;
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) to[k] = acc[k];
+        }
+    }
+}
+
+// One block per chunk; only those whose last run starts there and goes on have work: the run's chunks are shared by the
+// block's lane groups (contiguous shares), whose sums are added in order.
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void join_kernel(SumArgs a, int lanes_log2)
+{
+    const int64_t chunk = blockIdx.x, end = (chunk + 1) * CHUNK;
+    if (end >= a.n) return;
+    const uint32_t key = a.keys[end - 1];
+    if (key == (uint32_t)a.vocab || a.keys[end] != key) return;
+    if (chunk && a.keys[end - CHUNK] == key && a.keys[end - CHUNK - 1] == key) return;  // began earlier
+    int64_t lo = end, hi = a.n;  // the first position behind the run
+    while (lo < hi) {
+        const int64_t mid = (lo + hi) >> 1;
+        if (a.keys[mid] <= key) lo = mid + 1;
+        else hi = mid;
+    }
+    const int64_t parts = (lo - 1) / CHUNK - chunk;  // the chunks behind this one that the run reaches
+    const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> lanes_log2,
+              groups = 256 >> lanes_log2;
+    __shared__ float sums[256 * VEC];
+    const int64_t share = ceil_div(parts, groups);
+    const int64_t p0 = group * share < parts ? group * share : parts, p1 = p0 + share < parts ? p0 + share : parts;
+    for (int c0 = 0; c0 < a.d; c0 += lanes * VEC) {
+        const int c = c0 + lane * VEC;
+        float acc[VEC];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
+        if (c < a.d) {
+            for (int64_t p = p0; p < p1; ++p)
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) acc[k] += a.head[(chunk + 1 + p) * a.d + c + k];
+        }
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) sums[threadIdx.x * VEC + k] = acc[k];
+        __syncthreads();
+        if (group == 0 && c < a.d) {
+            const int used = share ? (int)ceil_div(parts, share) : 0;
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) acc[k] = a.tail[chunk * a.d + c + k];
+            for (int g = 0; g < used; ++g)
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) acc[k] += sums[(g * lanes + lane) * VEC + k];
+            store_row<T, VEC>(a, key, c, acc);
+        }
+        __syncthreads();
+    }
+}
+
+struct GradSpace {
+    uint32_t *keys[2], *pos[2], *hist;
+    int32_t *bag_of;
+    float *head, *tail;
+    int64_t bytes;
+};
+
+GradSpace grad_space(int64_t vocab, int64_t nnz, int d, bool bags, void *ws)
+{
+    Carver c(ws);
+    GradSpace s;
+    const SortPlan p = sort_plan(vocab, nnz);
+    const int64_t chunks = ceil_div(nnz, CHUNK);
+    for (int i = 0; i < 2; ++i) {
+        s.keys[i] = c.take<uint32_t>(nnz);
+        s.pos[i] = c.take<uint32_t>(nnz);
+    }
+    s.hist = c.take<uint32_t>((int64_t)p.blocks * p.bins);
+    s.bag_of = c.take<int32_t>(bags ? nnz : 0);
+    s.head = c.take<float>(chunks * d);
+    s.tail = c.take<float>(chunks * d);
+    s.bytes = c.used;
+    return s;
+}
+
+template <typename T, int VEC>
+hipError_t launch_sums(const SumArgs &s, hipStream_t st)
+{
+    const int ll = lanes_for(s.d, VEC);
+    const int64_t chunks = ceil_div(s.n, CHUNK);
+    chunk_sum_kernel<T, VEC><<<dim3((unsigned)ceil_div(chunks << ll, 256)), 256, 0, st>>>(s, ll);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || chunks < 2) return e;
+    join_kernel<T, VEC><<<dim3((unsigned)chunks), 256, 0, st>>>(s, ll);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t sums_typed(const SumArgs &s, hipStream_t st)
+{
+    constexpr int W = 16 / (int)sizeof(T);
+    if (aligned(s.d_out, s.stride, s.d, sizeof(T), W) && aligned(s.out, s.d, s.d, sizeof(T), W))
+        return launch_sums<T, W>(s, st);
+    if (aligned(s.d_out, s.stride, s.d, sizeof(T), W / 2) && aligned(s.out, s.d, s.d, sizeof(T), W / 2))
+        return launch_sums<T, W / 2>(s, st);
+    return launch_sums<T, 1>(s, st);
+}
+
+template <typename I>
+hipError_t grad_typed(const lfm_lookup_args &a, void *ws, hipStream_t st)
+{
+    const SortPlan p = sort_plan(a.vocab, a.nnz);
+    const GradSpace s = grad_space(a.vocab, a.nnz, a.d, a.indptr != nullptr, ws);
+    const int64_t out_bytes = a.vocab * a.d * dtype_bytes(a.dtype);
+    const int64_t words = out_bytes / 16;  // the output is 16-byte aligned (checked by the caller)
+    int64_t fill_blocks = ceil_div(words > a.nnz ? words : a.nnz, (int64_t)SORT_THREADS * 4);
+    if (fill_blocks < 1) fill_blocks = 1;
+    if (fill_blocks > 2048) fill_blocks = 2048;
+    const I *ids = (const I *)a.ids;
+    hipError_t e;
+    const uint32_t *keys = nullptr, *pos = nullptr;
+    int at = 0;
+    for (int pass = 0; pass < p.passes; ++pass) {
+        const int shift = pass * p.bits;
+        if (pass == 0)
+            count_kernel<I, true><<<dim3((unsigned)(p.blocks + fill_blocks)), SORT_THREADS, 0, st>>>(
+                ids, nullptr, a.nnz, a.vocab, shift, p.bins, p.items, s.hist, p.blocks, (uint4 *)a.out, words,
+                (char *)a.out + words * 16, (int)(out_bytes - words * 16), (const I *)a.indptr, a.rows, s.bag_of);
+        else
+            count_kernel<I, false><<<dim3((unsigned)p.blocks), SORT_THREADS, 0, st>>>(
+                ids, keys, a.nnz, a.vocab, shift, p.bins, p.items, s.hist, p.blocks, nullptr, 0, nullptr, 0, nullptr, 0,
+                nullptr);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+        if (a.nnz == 0) return hipSuccess;
+        if (pass == 0)
+            scatter_kernel<I, true><<<dim3((unsigned)p.blocks), SORT_THREADS, 0, st>>>(
+                ids, nullptr, nullptr, a.nnz, a.vocab, shift, p.bits, p.items, s.hist, p.blocks, s.keys[at], s.pos[at]);
+        else
+            scatter_kernel<I, false><<<dim3((unsigned)p.blocks), SORT_THREADS, 0, st>>>(
+                ids, keys, pos, a.nnz, a.vocab, shift, p.bits, p.items, s.hist, p.blocks, s.keys[at], s.pos[at]);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+        keys = s.keys[at];
+        pos = s.pos[at];
+        at ^= 1;
+    }
+    SumArgs sum;
+    sum.keys = keys;
+    sum.pos = pos;
+    sum.bag_of = a.indptr ? s.bag_of : nullptr;
+    sum.values = a.values;
+    sum.d_out = a.d_out;
+    sum.out = a.out;
+    sum.head = s.head;
+    sum.tail = s.tail;
+    sum.n = a.nnz;
+    sum.vocab = a.vocab;
+    sum.rows = a.rows;
+    sum.stride = a.d_out_stride;
+    sum.d = a.d;
+    sum.scale = a.scale;
+    return a.dtype == LFM_F32 ? sums_typed<float>(sum, st)
+         : a.dtype == LFM_BF16 ? sums_typed<bf16_t>(sum, st) : sums_typed<f16_t>(sum, st);
+}
+
+}  // namespace
+
+hipError_t embedding_lookup(const lfm_lookup_args &a, hipStream_t st)
+{
+    if (a.rows == 0) return hipSuccess;
+    if (a.id_bytes == 8)
+        return a.dtype == LFM_F32 ? lookup_typed<float, int64_t>(a, st)
+             : a.dtype == LFM_BF16 ? lookup_typed<bf16_t, int64_t>(a, st) : lookup_typed<f16_t, int64_t>(a, st);
+    return a.dtype == LFM_F32 ? lookup_typed<float, int32_t>(a, st)
+         : a.dtype == LFM_BF16 ? lookup_typed<bf16_t, int32_t>(a, st) : lookup_typed<f16_t, int32_t>(a, st);
+}
+
+int64_t embedding_grad_workspace(int64_t rows, int64_t vocab, int64_t nnz, int d, bool bags)
+{
+    (void)rows;
+    return grad_space(vocab, nnz, d, bags, nullptr).bytes;
+}
+
+hipError_t embedding_grad(const lfm_lookup_args &a, void *ws, hipStream_t st)
+{
+    return a.id_bytes == 8 ? grad_typed<int64_t>(a, ws, st) : grad_typed<int32_t>(a, ws, st);
+}
+
+}  // namespace ops
+}  // namespace lfm
