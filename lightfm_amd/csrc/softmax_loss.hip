@@ -26,6 +26,13 @@
 
 #include <math.h>
 
+#ifndef LFM_ROWS_WAVES
+#define LFM_ROWS_WAVES 2
+#endif
+#ifndef LFM_TABLE_WAVES
+#define LFM_TABLE_WAVES 2
+#endif
+
 namespace lfm {
 namespace ops {
 namespace {
@@ -221,11 +228,12 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs p, int dp, int width
 // ------------------------------------------------------------- the sweeps ---
 
 // Streams `rows` rows of NS DP halves into LDS, BV at a time, double-buffered through registers: the loads of the next
-// tile are in flight while this one is used.  A row takes NS DP + 8 halves of LDS: the padding spreads the 16-byte reads of
-// 16 neighbouring rows over all banks.
+// tile are in flight while this one is used.  A row takes NS DP + 16 halves of LDS: neighbouring rows then start 8 banks
+// apart (modulo 64, in some order), which serves the 16-byte reads of 8 rows and the transposing reads of 4 x 32 bytes
+// without conflicts.
 template <typename E, int NS, int DP>
 struct Tile {
-    static constexpr int BV = NS * DP <= 128 ? 64 : 32, ROW = NS * DP + 8, CHUNKS = NS * DP / 8, PER = BV * CHUNKS / 256;
+    static constexpr int BV = NS * DP <= 128 ? 64 : 32, ROW = NS * DP + 16, CHUNKS = NS * DP / 8, PER = BV * CHUNKS / 256;
     static constexpr int SIZE = BV * ROW;
     uint4 held[PER];
 
@@ -252,19 +260,18 @@ template <typename E, int NS, int DP>
 __device__ inline void load_owned(typename Half<E>::x8 (&f)[NS][DP / 16], const E *p, int64_t ld, int64_t row, int64_t rows, float factor)
 {
     typedef typename Half<E>::x8 x8;
-    const int h = (threadIdx.x & 63) >> 5;
+    const bool there = row < rows;
+    const E *q = p + (there ? row : 0) * ld + ((threadIdx.x & 63) >> 5) * 8;
 #pragma unroll
     for (int s = 0; s < NS; ++s)
 #pragma unroll
-        for (int k = 0; k < DP / 16; ++k) {
-            x8 v = {};
-            if (row < rows) v = *(const x8 *)(p + row * ld + s * DP + k * 16 + h * 8);
-            if (NS == 2 && factor != 1.0f) {
+        for (int k = 0; k < DP / 16; ++k) f[s][k] = there ? *(const x8 *)(q + s * DP + k * 16) : (x8)((E)0.0f);
+    if (NS == 2 && factor != 1.0f) {  // (a power of two that float16 need not hold: what vanishes does not show in a score)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = (E)((float)v[j] * factor);
-            }
-            f[s][k] = v;
-        }
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k) f[s][k] *= (E)factor;
+    }
 }
 
 // acc += 32 rows of the tile (from row r0) x the owned rows
@@ -291,39 +298,93 @@ __device__ inline void scores(f32x16 (&acc)[CW], const typename Half<E>::x8 (&ow
     }
 }
 
-// out[d, owned] += tile^T x value for 16 rows of the tile (from row r0); v: the lane's 8 values of those rows
+// Eight float32 values to a matrix operand: rounded to nearest (bf16, f16), or split into two float16 (hi towards zero, two
+// values per instruction; the remainder is exact and keeps 11 bits more).
+__device__ inline Half<bf16_t>::x8 round_values(const float (&v)[8], Half<bf16_t>::x8)
+{
+    Half<bf16_t>::x8 r;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = (bf16_t)v[j];
+    return r;
+}
+
+__device__ inline Half<f16_t>::x8 round_values(const float (&v)[8], Half<f16_t>::x8)
+{
+    Half<f16_t>::x8 r;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = (f16_t)v[j];
+    return r;
+}
+
+__device__ inline Half<f16_t>::x8 cut_values(const float (&v)[8])
+{
+    typedef __fp16 fp16x2 __attribute__((ext_vector_type(2)));
+    union { fp16x2 p[4]; Half<f16_t>::x8 r; } u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) u.p[j] = __builtin_amdgcn_cvt_pkrtz(v[2 * j], v[2 * j + 1]);
+    return u.r;
+}
+
+template <typename E, int NS, int CW>
+struct Values {  // the probabilities of 32 streamed rows as matrix operands
+    typename Half<E>::x8 hi[CW][2], lo[NS == 2 ? CW : 1][2];
+};
+
+template <typename E, int NS, int CW>
+__device__ inline void clear_values(Values<E, NS, CW> &p)
+{
+#pragma unroll
+    for (int w = 0; w < CW; ++w)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            p.hi[w][k] = (typename Half<E>::x8)((E)0.0f);
+            if (NS == 2) p.lo[w][k] = (typename Half<E>::x8)((E)0.0f);
+        }
+}
+
+template <typename E, int NS, int CW>
+__device__ inline void pack_values(Values<E, NS, CW> &p, const float (&v)[CW][8], int k)
+{
+#pragma unroll
+    for (int w = 0; w < CW; ++w)
+        if constexpr (NS == 2) {
+            float rest[8];
+            p.hi[w][k] = cut_values(v[w]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) rest[j] = __builtin_fmaf((float)p.hi[w][k][j], -1.0f, v[w][j]);
+            p.lo[w][k] = cut_values(rest);
+        } else
+            p.hi[w][k] = round_values(v[w], typename Half<E>::x8());
+}
+
+// out[d, owned] += tile^T x values for 32 rows of the tile (from row r0)
 template <typename E, int NS, int DP, int CW>
-__device__ inline void accumulate(f32x16 (&out)[CW][DP / 32], const float (&v)[CW][8], const E *tile, int r0)
+__device__ inline void accumulate(f32x16 (&out)[CW][DP / 32], const Values<E, NS, CW> &p, const E *tile, int r0)
 {
     typedef typename Half<E>::x8 x8;
     typedef typename Half<E>::x4 x4;
     constexpr int ROW = Tile<E, NS, DP>::ROW;
     const int lane = threadIdx.x & 63;
-    x8 hi[CW], lo[CW];
+    const E *at = tile + (r0 + 4 * (lane >> 5) + ((lane & 15) >> 2)) * ROW + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
 #pragma unroll
-    for (int w = 0; w < CW; ++w)
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            hi[w][j] = (E)v[w][j];
-            if (NS == 2) lo[w][j] = (E)(v[w][j] - (float)hi[w][j]);
-        }
-    const E *p = tile + (r0 + 4 * (lane >> 5) + ((lane & 15) >> 2)) * ROW + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+        for (int b = 0; b < DP / 32; ++b) {
+            const E *c = at + k * 16 * ROW + b * 32;
+            const x4 h0 = read_column(c), h1 = read_column(c + 8 * ROW);
+            const x8 th = __builtin_shufflevector(h0, h1, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-    for (int b = 0; b < DP / 32; ++b) {
-        const x4 h0 = read_column(p + b * 32), h1 = read_column(p + 8 * ROW + b * 32);
-        const x8 th = __builtin_shufflevector(h0, h1, 0, 1, 2, 3, 4, 5, 6, 7);
+            for (int w = 0; w < CW; ++w) out[w][b] = mfma(th, p.hi[w][k], out[w][b]);
+            if (NS == 2) {
+                const x4 l0 = read_column(c + DP), l1 = read_column(c + DP + 8 * ROW);
+                const x8 tl = __builtin_shufflevector(l0, l1, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-        for (int w = 0; w < CW; ++w) out[w][b] = mfma(th, hi[w], out[w][b]);
-        if (NS == 2) {
-            const x4 l0 = read_column(p + DP + b * 32), l1 = read_column(p + DP + 8 * ROW + b * 32);
-            const x8 tl = __builtin_shufflevector(l0, l1, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-            for (int w = 0; w < CW; ++w) {
-                out[w][b] = mfma(tl, hi[w], out[w][b]);
-                out[w][b] = mfma(th, lo[w], out[w][b]);
+                for (int w = 0; w < CW; ++w) {
+                    out[w][b] = mfma(tl, p.hi[w][k], out[w][b]);
+                    out[w][b] = mfma(th, p.lo[w][k], out[w][b]);
+                }
             }
         }
-    }
 }
 
 struct SweepArgs {
@@ -332,114 +393,135 @@ struct SweepArgs {
     int64_t rows, vocab;
     const float *bias;
     const Scales *scales;
+    const void *targets;    // rows_kernel: [rows], id_bytes wide
+    int id_bytes;
     int splits;             // parts of the streamed side
     int d, dp;
     int chunks;             // of 256 columns (WIDE; else 1): the second product's columns are blockIdx.y's
-    // rows_kernel: per chunk, part and row
+    // rows_kernel: per chunk, part and row, the row's target left out
     float *pm, *pl, *po;    // maximum (matrix units), sum of 2^7 p; per part and row: sum of 2^7 p w [dp]
     // table_kernel: per row
-    const float *row_max, *row_rate, *row_weight;  // maximum (matrix units; +inf: no target), 2^shift g / sum, 2^shift g
+    const float *row_max, *row_rate, *row_weight;  // maximum (matrix units; +inf: no target), 2^shift g / sum, 2^shift g (1 - p[target])
     const int32_t *row_target;
     void *dw;               // one part: the result
     float *db, *pw, *pb;    // several: partial sums per part [vocab][dp], [vocab]
     int shifted;            // q is scaled by 2^(14 - eg): 0 no (bfloat16), 1 with eg = 0, 2 with eg of scales
 };
 
-// WIDE: more than 256 columns, taken 256 at a time.  The scores add up over the chunks (the owned operand is read again for
-// each, from the caches); a block accumulates the second product of one chunk, the one that it streams last.
-template <typename E, int NS, int DP, int CW, bool GRAD, bool WIDE>
-__global__ __launch_bounds__(256, GRAD && (NS * DP >= 384 || WIDE) ? 1 : 2) void rows_kernel(SweepArgs a)
+// Both sweeps are pipelined over blocks of 32 streamed rows: a step makes the scores of block b + 1 and the second product
+// of block b - 1 on the matrix cores while the vector units turn the scores of block b into probabilities.  None of the
+// three waits for another, so a wave keeps both busy by itself.  Tiles rotate through BUFS buffers of LDS, so that a tile
+// is free again two steps after its last score and one barrier per tile does.
+template <typename E, int NS, int DP>
+struct Rotation {
+    static constexpr int BLOCKS = Tile<E, NS, DP>::BV / 32, BUFS = BLOCKS == 2 ? 3 : 4;
+    // tiles stored ahead of the first step, before which the next tile is stored
+    static constexpr int AHEAD = BLOCKS == 2 ? 1 : 2;
+};
+
+// What a step has to hide: one matrix instruction, an LDS read, a few vector instructions, and so on
+template <int MATRIX, int VECTOR>
+__device__ inline void interleave()
+{
+#ifndef LFM_NO_INTERLEAVE
+#pragma unroll
+    for (int i = 0; i < MATRIX; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, VECTOR, 0);
+    }
+#endif
+}
+
+template <typename E, int NS, int DP, int CW, bool GRAD>
+__global__ __launch_bounds__(256, (GRAD ? NS * DP >= 384 : NS * DP >= 512) ? 1 : LFM_ROWS_WAVES) void rows_kernel(SweepArgs a)
 {
     typedef Tile<E, NS, DP> Tl;
+    typedef Rotation<E, NS, DP> Ro;
     typedef typename Half<E>::x8 x8;
-    constexpr int VB = Tl::BV / 32;
-    __shared__ __attribute__((aligned(16))) E tile[2][Tl::SIZE];
-    __shared__ __attribute__((aligned(16))) float sb[2][Tl::BV];
+    __shared__ __attribute__((aligned(16))) E tile[Ro::BUFS][Tl::SIZE];
+    __shared__ __attribute__((aligned(16))) float sb[Ro::BUFS][Tl::BV];
     const Derived dv = derive(NS == 2 ? a.scales : nullptr);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-    const int part = blockIdx.x % a.splits;
-    const int64_t n0 = (int64_t)(blockIdx.x / a.splits) * (128 * CW) + wave * (32 * CW) + (lane & 31);
-    const int64_t tiles = ceil_div(a.vocab, Tl::BV);
-    const int64_t t0 = tiles * part / a.splits, t1 = tiles * (part + 1) / a.splits;
+    const uint32_t part = blockIdx.x % (uint32_t)a.splits;
+    const int64_t n0 = (int64_t)(blockIdx.x / (uint32_t)a.splits) * (128 * CW) + wave * (32 * CW) + (lane & 31);
+    const uint32_t tiles = (uint32_t)((a.vocab + Tl::BV - 1) / Tl::BV);
+    const uint32_t t0 = (uint32_t)((uint64_t)tiles * part / (uint32_t)a.splits);
+    const int nt = (int)((uint64_t)tiles * (part + 1) / (uint32_t)a.splits) - (int)t0;
 
-    const int chunks = WIDE ? a.chunks : 1, first = WIDE ? (int)blockIdx.y + 1 : 0;
-    auto offset = [&](int j) { return WIDE ? ((first + j) % chunks) * (NS * DP) : 0; };  // of the j-th chunk; the last is blockIdx.y's
     x8 own[CW][NS][DP / 16];
-    auto take = [&](int j) {
-#pragma unroll
-        for (int w = 0; w < CW; ++w) load_owned<E, NS, DP>(own[w], (const E *)a.x + offset(j), a.ldx, n0 + 32 * w, a.rows, dv.owned);
-    };
-    if (!WIDE) take(0);
-    f32x16 out[CW][DP / 32];
+    f32x16 out[CW][DP / 32], cur[CW], next[CW];
+    Values<E, NS, CW> p;
     float m[CW], l[CW];
+    int32_t target[CW];
 #pragma unroll
     for (int w = 0; w < CW; ++w) {
+        const int64_t n = n0 + 32 * w;
+        load_owned<E, NS, DP>(own[w], (const E *)a.x, a.ldx, n, a.rows, dv.owned);
+        const int64_t at = n >= a.rows ? -1 : a.id_bytes == 8 ? ((const int64_t *)a.targets)[n] : (int64_t)((const int32_t *)a.targets)[n];
+        target[w] = (uint64_t)at < (uint64_t)a.vocab ? (int32_t)at - 4 * h : INT32_MIN / 2;
         m[w] = dv.low * 1.01f;
         l[w] = 0.0f;
-        if (GRAD)
+        if (GRAD) {
 #pragma unroll
             for (int b = 0; b < DP / 32; ++b) out[w][b] = (f32x16)(0.0f);
+        }
     }
+    clear_values(p);
 
     Tl t;
     float next_bias = 0.0f;
-    auto fetch = [&](int64_t i, int j) {
-        t.fetch((const E *)a.w + offset(j), a.ldw, i * Tl::BV, a.vocab);
-        const int64_t v = i * Tl::BV + threadIdx.x;
-        if (j == 0 && threadIdx.x < Tl::BV) next_bias = v >= a.vocab ? -INFINITY : a.bias ? bias_units(a.bias[v], dv) : 0.0f;
+    auto fetch = [&](int i) {
+        const int64_t r = (int64_t)(t0 + i) * Tl::BV;
+        t.fetch((const E *)a.w, a.ldw, r, a.vocab);
+        const int64_t v = r + threadIdx.x;
+        if (threadIdx.x < Tl::BV) next_bias = v >= a.vocab ? -INFINITY : a.bias ? bias_units(a.bias[v], dv) : 0.0f;
     };
-    auto store = [&](int64_t i, int j, int buf) {
+    auto store = [&](int buf) {
         t.store(tile[buf]);
-        if (j == 0 && threadIdx.x < Tl::BV) sb[(i - t0) & 1][threadIdx.x] = next_bias;
+        if (threadIdx.x < Tl::BV) sb[buf][threadIdx.x] = next_bias;
     };
-    if (t0 < t1) {
-        fetch(t0, 0);
-        store(t0, 0, 0);
-    }
-    __syncthreads();
-    int buf = 0;
-    for (int64_t i = t0; i < t1; ++i) {
-        f32x16 s[VB][CW];
+    auto score = [&](f32x16 (&s)[CW], int buf, int r0) {
 #pragma unroll
-        for (int vb = 0; vb < VB; ++vb) {
+        for (int g = 0; g < 4; ++g) {
+            const float4 b = *(const float4 *)&sb[buf][r0 + 8 * g + 4 * h];
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const float4 b = *(const float4 *)&sb[(i - t0) & 1][vb * 32 + 8 * g + 4 * h];
-#pragma unroll
-                for (int w = 0; w < CW; ++w) {
-                    s[vb][w][4 * g + 0] = b.x;
-                    s[vb][w][4 * g + 1] = b.y;
-                    s[vb][w][4 * g + 2] = b.z;
-                    s[vb][w][4 * g + 3] = b.w;
-                }
+            for (int w = 0; w < CW; ++w) {
+                s[w][4 * g + 0] = b.x;
+                s[w][4 * g + 1] = b.y;
+                s[w][4 * g + 2] = b.z;
+                s[w][4 * g + 3] = b.w;
             }
         }
-        for (int j = 0; j < chunks - 1; ++j) {  // WIDE: the other chunks first
-            take(j);
-            fetch(i, j + 1);
+        scores<E, NS, DP, CW>(s, own, tile[buf], r0);
+    };
+    // the step of the block whose first vocabulary row is v: before_* the block before it, after_* the one behind it
+    auto step = [&](int32_t v, int before, int before_r, int after, int after_r) {
+        // the target's own score is left to the join, in float32: what remains is not a difference of near-equals
+        bool here = false;
 #pragma unroll
-            for (int vb = 0; vb < VB; ++vb) scores<E, NS, DP, CW>(s[vb], own, tile[buf], vb * 32);
-            store(i, j + 1, buf ^ 1);
-            __syncthreads();
-            buf ^= 1;
+        for (int w = 0; w < CW; ++w) here |= (uint32_t)target[w] + 4 * h - (uint32_t)v < 32u;
+        if (__any(here)) {  // one block in some
+#pragma unroll
+            for (int w = 0; w < CW; ++w)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) cur[w][j] = (uint32_t)target[w] - (uint32_t)v == 8u * (j / 4) + j % 4 ? -INFINITY : cur[w][j];
         }
-        if (WIDE) take(chunks - 1);
-        if (i + 1 < t1) fetch(i + 1, 0);
-#pragma unroll
-        for (int vb = 0; vb < VB; ++vb) scores<E, NS, DP, CW>(s[vb], own, tile[buf], vb * 32);
         bool grows = false;
         float mx[CW];
 #pragma unroll
         for (int w = 0; w < CW; ++w) {
-            mx[w] = s[0][w][0];
+            mx[w] = cur[w][0];
 #pragma unroll
-            for (int vb = 0; vb < VB; ++vb)
-#pragma unroll
-                for (int j = 0; j < 16; ++j) mx[w] = fmaxf(mx[w], s[vb][w][j]);
+            for (int j = 1; j < 16; ++j) mx[w] = fmaxf(mx[w], cur[w][j]);
             mx[w] = half_wave_max(mx[w]);
             grows |= (mx[w] - m[w]) * dv.c > LAG;
         }
-        if (__any(grows)) {  // seldom after the first tiles; by row, so that no row's bits depend on its neighbours
+        if (__any(grows)) {  // seldom after the first blocks; by row, so that no row's bits depend on its neighbours
+            if (GRAD) {
+                accumulate<E, NS, DP, CW>(out, p, tile[before], before_r);  // still about the old maximum
+                clear_values(p);
+            }
 #pragma unroll
             for (int w = 0; w < CW; ++w) {
                 const float up = (mx[w] - m[w]) * dv.c > LAG ? mx[w] : m[w], f = exp2_fast((m[w] - up) * dv.c);
@@ -463,28 +545,61 @@ __global__ __launch_bounds__(256, GRAD && (NS * DP >= 384 || WIDE) ? 1 : 2) void
                 const bool mine = fabsf(m[w] * dv.c) > FAR;
                 const float less = mine ? m[w] : 0.0f;
                 base[w] = mine ? P_SHIFT : base[w];
-#pragma unroll
-                for (int vb = 0; vb < VB; ++vb) s[vb][w] -= less;
+                cur[w] -= less;
             }
         }
+        score(next, after, after_r);
+        if (GRAD) accumulate<E, NS, DP, CW>(out, p, tile[before], before_r);
 #pragma unroll
-        for (int vb = 0; vb < VB; ++vb)
+        for (int k = 0; k < 2; ++k) {
+            float v8[CW][8];
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
-                float p[CW][8];
+            for (int w = 0; w < CW; ++w)
 #pragma unroll
-                for (int w = 0; w < CW; ++w)
+                for (int j = 0; j < 8; ++j) {
+                    v8[w][j] = exp2_fast(__builtin_fmaf(cur[w][8 * k + j], dv.c, base[w]));
+                    l[w] += v8[w][j];
+                }
+            if (GRAD) pack_values<E, NS, CW>(p, v8, k);
+        }
+        constexpr int MATRIX = CW * (NS == 2 ? 3 : 1) * (DP / 16) * (GRAD ? 2 : 1), VECTOR = CW * (GRAD ? NS == 2 ? 96 : 72 : 56);
+        interleave<MATRIX, (VECTOR + MATRIX - 1) / MATRIX>();
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        p[w][j] = exp2_fast(__builtin_fmaf(s[vb][w][8 * kb + j], dv.c, base[w]));
-                        l[w] += p[w][j];
-                    }
-                if (GRAD) accumulate<E, NS, DP, CW>(out, p, tile[buf], vb * 32 + kb * 16);
-            }
-        if (i + 1 < t1) store(i + 1, 0, buf ^ 1);
+        for (int w = 0; w < CW; ++w) cur[w] = next[w];
+    };
+
+    if (nt > 0) {
+        fetch(0);
+        store(0);
+        if (Ro::AHEAD == 2 && nt > 1) {
+            fetch(1);
+            store(1);
+        }
+        if (nt > Ro::AHEAD) fetch(Ro::AHEAD);
         __syncthreads();
-        buf ^= 1;
+        score(cur, 0, 0);
     }
+    int b0 = 0, b1 = 1, before = 0;  // the buffers of tile i, i + 1, i - 1
+    for (int i = 0; i < nt; ++i) {
+        int b2 = b1 + 1 == Ro::BUFS ? 0 : b1 + 1;
+        const int into = Ro::BLOCKS == 2 ? b1 : b2;
+        if (i + Ro::AHEAD < nt) store(into);
+        if (i + Ro::AHEAD + 1 < nt) fetch(i + Ro::AHEAD + 1);
+        const int32_t v = (int32_t)((t0 + i) * Tl::BV);
+        const int after = i + 1 < nt ? b1 : b0;  // (behind the last block: scores that nobody looks at)
+        if (Ro::BLOCKS == 2) {
+            step(v, before, i ? 32 : 0, b0, 32);
+            __syncthreads();
+            step(v + 32, b0, 0, after, 0);
+        } else {
+            step(v, before, 0, after, 0);
+            __syncthreads();
+        }
+        before = b0;
+        b0 = b1;
+        b1 = b2;
+    }
+    if (GRAD && nt > 0) accumulate<E, NS, DP, CW>(out, p, tile[before], Tl::BV - 32);
 #pragma unroll
     for (int w = 0; w < CW; ++w) {
         const int64_t n = n0 + 32 * w;
@@ -492,161 +607,32 @@ __global__ __launch_bounds__(256, GRAD && (NS * DP >= 384 || WIDE) ? 1 : 2) void
         if (n >= a.rows) continue;
         const int64_t at = (int64_t)part * a.rows + n;
         if (h == 0) {
-            const int64_t to = at + (WIDE ? (int64_t)blockIdx.y * a.splits * a.rows : 0);
-            a.pm[to] = m[w];
-            a.pl[to] = sum;
+            a.pm[at] = m[w];
+            a.pl[at] = sum;
         }
         if (GRAD)
 #pragma unroll
             for (int b = 0; b < DP / 32; ++b)
 #pragma unroll
                 for (int g = 0; g < 4; ++g)
-                    *(float4 *)(a.po + at * a.dp + (WIDE ? (int)blockIdx.y * DP : 0) + b * 32 + 8 * g + 4 * h) =
+                    *(float4 *)(a.po + at * DP + b * 32 + 8 * g + 4 * h) =
                         make_float4(out[w][b][4 * g], out[w][b][4 * g + 1], out[w][b][4 * g + 2], out[w][b][4 * g + 3]);
     }
 }
 
-template <typename T, typename E, int NS, int DP, int CW, bool WIDE>
-__global__ __launch_bounds__(256, NS * DP >= 256 || DP >= 192 ? 1 : 2) void table_kernel(SweepArgs a)
+// Writes a wave's part of dw (or its partial sums) and db
+template <typename T, int NS, int DP, int CW>
+__device__ inline void write_table(const SweepArgs &a, const f32x16 (&out)[CW][DP / 32], const float (&db)[CW], int64_t v0, int64_t part, int c0)
 {
-    typedef Tile<E, NS, DP> Tl;
-    typedef typename Half<E>::x8 x8;
-    constexpr int NB = Tl::BV / 32;
-    __shared__ __attribute__((aligned(16))) E tile[2][Tl::SIZE];
-    __shared__ __attribute__((aligned(16))) float sm[2][Tl::BV], sr[2][Tl::BV], sg[2][Tl::BV], sf[2][Tl::BV];
-    __shared__ __attribute__((aligned(16))) int32_t st[2][Tl::BV];
-    const Derived dv = derive(NS == 2 ? a.scales : nullptr);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-    const int part = blockIdx.x % a.splits;
-    const int64_t w0 = (int64_t)(blockIdx.x / a.splits) * (128 * CW) + wave * (32 * CW), v0 = w0 + (lane & 31);
-    const int64_t tiles = ceil_div(a.rows, Tl::BV);
-    const int64_t t0 = tiles * part / a.splits, t1 = tiles * (part + 1) / a.splits;
-
-    const int chunks = WIDE ? a.chunks : 1, first = WIDE ? (int)blockIdx.y + 1 : 0;
-    auto offset = [&](int j) { return WIDE ? ((first + j) % chunks) * (NS * DP) : 0; };
-    x8 own[CW][NS][DP / 16];
-    auto take = [&](int j) {
-#pragma unroll
-        for (int w = 0; w < CW; ++w) load_owned<E, NS, DP>(own[w], (const E *)a.w + offset(j), a.ldw, v0 + 32 * w, a.vocab, dv.owned);
-    };
-    if (!WIDE) take(0);
-    f32x16 out[CW][DP / 32];
-    float bias[CW], db[CW];
-#pragma unroll
-    for (int w = 0; w < CW; ++w) {
-        const int64_t v = v0 + 32 * w;
-        bias[w] = a.bias && v < a.vocab ? bias_units(a.bias[v], dv) : 0.0f;
-        db[w] = 0.0f;
-#pragma unroll
-        for (int b = 0; b < DP / 32; ++b) out[w][b] = (f32x16)(0.0f);
-    }
-
-    Tl t;
-    float next_m = 0.0f, next_r = 0.0f, next_g = 0.0f;
-    int32_t next_t = -1;
-    auto fetch = [&](int64_t i, int j) {
-        t.fetch((const E *)a.x + offset(j), a.ldx, i * Tl::BV, a.rows);
-#pragma unroll
-        for (int q = 0; q < Tl::PER; ++q) {  // a row without a target is not read: zeros in its place
-            const int64_t n = i * Tl::BV + (q * 256 + (int)threadIdx.x) / Tl::CHUNKS;
-            if (n < a.rows && a.row_target[n] < 0) t.held[q] = make_uint4(0, 0, 0, 0);
-        }
-        if (j == 0 && threadIdx.x < Tl::BV) {
-            const int64_t n = i * Tl::BV + threadIdx.x;
-            const bool ok = n < a.rows;
-            next_m = ok ? a.row_max[n] : INFINITY;
-            next_r = ok ? a.row_rate[n] : 0.0f;
-            next_g = ok ? a.row_weight[n] : 0.0f;
-            next_t = ok ? a.row_target[n] : -1;
-        }
-    };
-    auto store = [&](int64_t i, int j, int buf) {
-        t.store(tile[buf]);
-        if (j == 0 && threadIdx.x < Tl::BV) {
-            const int o = (int)(i - t0) & 1;
-            const bool far = fabsf(next_m * dv.c) > FAR && next_m < INFINITY;
-            sm[o][threadIdx.x] = far ? 0.0f : -next_m * dv.c;
-            sf[o][threadIdx.x] = far ? next_m : 0.0f;
-            sr[o][threadIdx.x] = next_r;
-            sg[o][threadIdx.x] = next_g;
-            st[o][threadIdx.x] = next_t;
-        }
-    };
-    if (t0 < t1) {
-        fetch(t0, 0);
-        store(t0, 0, 0);
-    }
-    __syncthreads();
-    int buf = 0;
-    for (int64_t i = t0; i < t1; ++i) {
-        const int o = (int)(i - t0) & 1;
-        f32x16 s[NB][CW];
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-            for (int w = 0; w < CW; ++w) s[nb][w] = (f32x16)(bias[w]);
-        for (int j = 0; j < chunks - 1; ++j) {  // WIDE: the other chunks first
-            take(j);
-            fetch(i, j + 1);
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) scores<E, NS, DP, CW>(s[nb], own, tile[buf], nb * 32);
-            store(i, j + 1, buf ^ 1);
-            __syncthreads();
-            buf ^= 1;
-        }
-        if (WIDE) take(chunks - 1);
-        if (i + 1 < t1) fetch(i + 1, 0);
-        const int32_t mine = st[o][lane & (Tl::BV - 1)];
-        const bool hits = __any(mine >= w0 && mine < w0 + 32 * CW);  // a target among this wave's table rows
-        const bool far = __any(sf[o][lane & (Tl::BV - 1)] != 0.0f);
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            scores<E, NS, DP, CW>(s[nb], own, tile[buf], nb * 32);
-            if (far)  // see FAR
-#pragma unroll
-                for (int w = 0; w < CW; ++w)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) s[nb][w][j] -= sf[o][nb * 32 + 8 * (j / 4) + 4 * h + j % 4];
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
-                float q[CW][8];
-#pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    const int r = nb * 32 + kb * 16 + 8 * g + 4 * h;
-                    const float4 mm = *(const float4 *)&sm[o][r], rr = *(const float4 *)&sr[o][r];
-                    const float ms[4] = {mm.x, mm.y, mm.z, mm.w}, rs[4] = {rr.x, rr.y, rr.z, rr.w};
-#pragma unroll
-                    for (int w = 0; w < CW; ++w)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            q[w][4 * g + j] = exp2_fast(__builtin_fmaf(s[nb][w][8 * kb + 4 * g + j], dv.c, ms[j])) * rs[j];
-                    if (hits)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-#pragma unroll
-                            for (int w = 0; w < CW; ++w)
-                                if ((int64_t)st[o][r + j] == v0 + 32 * w) q[w][4 * g + j] -= sg[o][r + j];
-                }
-#pragma unroll
-                for (int w = 0; w < CW; ++w)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) db[w] += q[w][j];
-                accumulate<E, NS, DP, CW>(out, q, tile[buf], nb * 32 + kb * 16);
-            }
-        }
-        if (i + 1 < t1) store(i + 1, 0, buf ^ 1);
-        __syncthreads();
-        buf ^= 1;
-    }
+    const int h = (threadIdx.x & 63) >> 5;
     const int shift = a.shifted == 2 ? a.scales->eg - 14 : a.shifted ? -14 : 0, kx = NS == 2 ? a.scales->kx : 0;
-    const int c0 = WIDE ? (int)blockIdx.y * DP : 0;
 #pragma unroll
     for (int w = 0; w < CW; ++w) {
         const int64_t v = v0 + 32 * w;
         const float total = half_wave_sum(db[w]);
         if (v >= a.vocab) continue;
         if (a.splits > 1) {
-            const int64_t at = (int64_t)part * a.vocab + v;
+            const int64_t at = part * a.vocab + v;
             if (h == 0 && c0 == 0) a.pb[at] = total;
 #pragma unroll
             for (int b = 0; b < DP / 32; ++b)
@@ -673,6 +659,396 @@ __global__ __launch_bounds__(256, NS * DP >= 256 || DP >= 192 ? 1 : 2) void tabl
                 }
         }
     }
+}
+
+// What table_kernel needs to know of the rows of a tile
+template <int BV>
+struct RowFacts {
+    float m[BV];        // -maximum in base 2 (0 where FAR is about the row)
+    float rate[BV];     // 2^shift g / sum
+    float weight[BV];   // 2^shift g (1 - p[target])
+    float far[BV];      // the maximum in matrix units where FAR is about the row, else 0
+    int32_t target[BV];
+};
+
+// The rare part of a block of scores: rows whose target is among the owned table rows leave the sum here and enter it as
+// -g (1 - p) x, in float32; rows that FAR is about lose their maximum first.
+template <typename E, int NS, int DP, int CW, int BV>
+__device__ inline void special_rows(f32x16 (&s)[CW], f32x16 (&out)[CW][DP / 32], float (&db)[CW], const RowFacts<BV> &f, const E *tile, int r0,
+                                    int32_t w0, bool hit)
+{
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        const int r = r0 + 8 * (j / 4) + 4 * h + j % 4;
+#pragma unroll
+        for (int w = 0; w < CW; ++w) s[w][j] = f.target[r] == w0 + (lane & 31) + 32 * w ? -INFINITY : s[w][j] - f.far[r];
+    }
+    uint32_t hits = (uint32_t)__ballot(hit);  // (the half-waves say the same)
+    while (hits) {
+        const int r = r0 + __ffs(hits) - 1;
+        hits &= hits - 1;
+        const int32_t at = f.target[r] - w0 - (lane & 31);
+        const float g = f.weight[r];
+        const E *x = tile + r * Tile<E, NS, DP>::ROW + 4 * h;
+#pragma unroll
+        for (int w = 0; w < CW; ++w) {
+            const float mg = at == 32 * w ? g : 0.0f;
+            if (h == 0) db[w] -= mg;
+#pragma unroll
+            for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const int c = b * 32 + 8 * (j / 4) + j % 4;
+                    const float xv = NS == 2 ? (float)x[c] + (float)x[(NS - 1) * DP + c] : (float)x[c];
+                    out[w][b][j] = __builtin_fmaf(-mg, xv, out[w][b][j]);
+                }
+        }
+    }
+}
+
+template <typename T, typename E, int NS, int DP, int CW>
+__global__ __launch_bounds__(256, NS * DP >= 384 ? 1 : LFM_TABLE_WAVES) void table_kernel(SweepArgs a)
+{
+    typedef Tile<E, NS, DP> Tl;
+    typedef Rotation<E, NS, DP> Ro;
+    typedef typename Half<E>::x8 x8;
+    __shared__ __attribute__((aligned(16))) E tile[Ro::BUFS][Tl::SIZE];
+    __shared__ __attribute__((aligned(16))) RowFacts<Tl::BV> facts[Ro::BUFS];
+    const Derived dv = derive(NS == 2 ? a.scales : nullptr);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    const uint32_t part = blockIdx.x % (uint32_t)a.splits;
+    const int64_t w0 = (int64_t)(blockIdx.x / (uint32_t)a.splits) * (128 * CW) + wave * (32 * CW), v0 = w0 + (lane & 31);
+    const uint32_t tiles = (uint32_t)((a.rows + Tl::BV - 1) / Tl::BV);
+    const uint32_t t0 = (uint32_t)((uint64_t)tiles * part / (uint32_t)a.splits);
+    const int nt = (int)((uint64_t)tiles * (part + 1) / (uint32_t)a.splits) - (int)t0;
+
+    x8 own[CW][NS][DP / 16];
+    f32x16 out[CW][DP / 32], cur[CW], next[CW];
+    Values<E, NS, CW> q;
+    float bias[CW], db[CW];
+#pragma unroll
+    for (int w = 0; w < CW; ++w) {
+        const int64_t v = v0 + 32 * w;
+        load_owned<E, NS, DP>(own[w], (const E *)a.w, a.ldw, v, a.vocab, dv.owned);
+        bias[w] = a.bias && v < a.vocab ? bias_units(a.bias[v], dv) : 0.0f;
+        db[w] = 0.0f;
+#pragma unroll
+        for (int b = 0; b < DP / 32; ++b) out[w][b] = (f32x16)(0.0f);
+    }
+    clear_values(q);
+
+    Tl t;
+    bool keep[Tl::PER];
+    float next_m = 0.0f, next_r = 0.0f, next_g = 0.0f;
+    int32_t next_t = -1;
+    auto fetch = [&](int i) {
+        const int64_t r = (int64_t)(t0 + i) * Tl::BV;
+        t.fetch((const E *)a.x, a.ldx, r, a.rows);
+#pragma unroll
+        for (int k = 0; k < Tl::PER; ++k) {
+            const int64_t n = r + (k * 256 + (int)threadIdx.x) / Tl::CHUNKS;
+            keep[k] = n < a.rows && a.row_target[n] >= 0;
+        }
+        if (threadIdx.x < Tl::BV) {
+            const int64_t n = r + threadIdx.x;
+            const bool ok = n < a.rows;
+            next_m = ok ? a.row_max[n] : INFINITY;
+            next_r = ok ? a.row_rate[n] : 0.0f;
+            next_g = ok ? a.row_weight[n] : 0.0f;
+            next_t = ok ? a.row_target[n] : -1;
+        }
+    };
+    auto store = [&](int buf) {
+#pragma unroll
+        for (int k = 0; k < Tl::PER; ++k)  // a row without a target is not read: zeros in its place
+            if (!keep[k]) t.held[k] = make_uint4(0, 0, 0, 0);
+        t.store(tile[buf]);
+        if (threadIdx.x < Tl::BV) {
+            const bool far = fabsf(next_m * dv.c) > FAR && next_m < INFINITY;
+            RowFacts<Tl::BV> &f = facts[buf];
+            f.m[threadIdx.x] = far ? 0.0f : -next_m * dv.c;
+            f.far[threadIdx.x] = far ? next_m : 0.0f;
+            f.rate[threadIdx.x] = next_r;
+            f.weight[threadIdx.x] = next_g;
+            f.target[threadIdx.x] = next_t;
+        }
+    };
+    auto score = [&](f32x16 (&s)[CW], int buf, int r0) {
+#pragma unroll
+        for (int w = 0; w < CW; ++w) s[w] = (f32x16)(bias[w]);
+        scores<E, NS, DP, CW>(s, own, tile[buf], r0);
+    };
+    auto step = [&](int here, int r0, int before, int before_r, int after, int after_r) {
+        const RowFacts<Tl::BV> &f = facts[here];
+        const bool hit = (uint32_t)(f.target[r0 + (lane & 31)] - (int32_t)w0) < 32u * CW;
+        if (__any(hit || f.far[r0 + (lane & 31)] != 0.0f))  // seldom
+            special_rows<E, NS, DP, CW, Tl::BV>(cur, out, db, f, tile[here], r0, (int32_t)w0, hit);
+        score(next, after, after_r);
+        accumulate<E, NS, DP, CW>(out, q, tile[before], before_r);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            float v8[CW][8];
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const int r = r0 + k * 16 + 8 * g + 4 * h;
+                const float4 mm = *(const float4 *)&f.m[r], rr = *(const float4 *)&f.rate[r];
+                const float ms[4] = {mm.x, mm.y, mm.z, mm.w}, rs[4] = {rr.x, rr.y, rr.z, rr.w};
+#pragma unroll
+                for (int w = 0; w < CW; ++w)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float v = exp2_fast(__builtin_fmaf(cur[w][8 * k + 4 * g + j], dv.c, ms[j])) * rs[j];
+                        db[w] += v;
+                        v8[w][4 * g + j] = v;
+                    }
+            }
+            pack_values<E, NS, CW>(q, v8, k);
+        }
+        constexpr int MATRIX = 2 * CW * (NS == 2 ? 3 : 1) * (DP / 16), VECTOR = CW * (NS == 2 ? 112 : 88);
+        interleave<MATRIX, (VECTOR + MATRIX - 1) / MATRIX>();
+#pragma unroll
+        for (int w = 0; w < CW; ++w) cur[w] = next[w];
+    };
+
+    if (nt > 0) {
+        fetch(0);
+        store(0);
+        if (Ro::AHEAD == 2 && nt > 1) {
+            fetch(1);
+            store(1);
+        }
+        if (nt > Ro::AHEAD) fetch(Ro::AHEAD);
+        __syncthreads();
+        score(cur, 0, 0);
+    }
+    int b0 = 0, b1 = 1, before = 0;  // the buffers of tile i, i + 1, i - 1
+    for (int i = 0; i < nt; ++i) {
+        int b2 = b1 + 1 == Ro::BUFS ? 0 : b1 + 1;
+        const int into = Ro::BLOCKS == 2 ? b1 : b2;
+        if (i + Ro::AHEAD < nt) store(into);
+        if (i + Ro::AHEAD + 1 < nt) fetch(i + Ro::AHEAD + 1);
+        const int after = i + 1 < nt ? b1 : b0;  // (behind the last block: scores that nobody looks at)
+        if (Ro::BLOCKS == 2) {
+            step(b0, 0, before, i ? 32 : 0, b0, 32);
+            __syncthreads();
+            step(b0, 32, b0, 0, after, 0);
+        } else {
+            step(b0, 0, before, 0, after, 0);
+            __syncthreads();
+        }
+        before = b0;
+        b0 = b1;
+        b1 = b2;
+    }
+    if (nt > 0) accumulate<E, NS, DP, CW>(out, q, tile[before], Tl::BV - 32);
+    write_table<T, NS, DP, CW>(a, out, db, v0, part, 0);
+}
+
+// More than 256 columns, taken 256 at a time.  The scores add up over the chunks (the owned operand is read again for each,
+// from the caches); a block accumulates the second product of one chunk, blockIdx.y's, which it streams last.  The work of
+// the scores is repeated for every chunk of the result: a width that is rare is not worth a second shape of block.
+template <typename E, int NS, bool GRAD>
+__global__ __launch_bounds__(256, 1) void wide_rows_kernel(SweepArgs a)
+{
+    constexpr int DP = 256;
+    typedef Tile<E, NS, DP> Tl;
+    typedef typename Half<E>::x8 x8;
+    static_assert(Tl::BV == 32, "one block of scores per tile");
+    __shared__ __attribute__((aligned(16))) E tile[2][Tl::SIZE];
+    __shared__ __attribute__((aligned(16))) float sb[2][32];
+    const Derived dv = derive(NS == 2 ? a.scales : nullptr);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    const int part = blockIdx.x % a.splits;
+    const int64_t n = (int64_t)(blockIdx.x / a.splits) * 128 + wave * 32 + (lane & 31);
+    const int64_t tiles = ceil_div(a.vocab, 32), t0 = tiles * part / a.splits, t1 = tiles * (part + 1) / a.splits;
+    const int chunks = a.chunks, first = (int)blockIdx.y + 1;
+    auto offset = [&](int j) { return ((first + j) % chunks) * (NS * DP); };  // of the j-th chunk; the last is blockIdx.y's
+    f32x16 out[1][DP / 32];
+    Values<E, NS, 1> p;
+    float m = dv.low * 1.01f, l = 0.0f;
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b) out[0][b] = (f32x16)(0.0f);
+    const int64_t at = n >= a.rows ? -1 : a.id_bytes == 8 ? ((const int64_t *)a.targets)[n] : (int64_t)((const int32_t *)a.targets)[n];
+    const int64_t target = (uint64_t)at < (uint64_t)a.vocab ? at - 4 * h : -1000;
+    Tl t;
+    float next_bias = 0.0f;
+    auto fetch = [&](int64_t i, int j) {
+        t.fetch((const E *)a.w + offset(j), a.ldw, i * 32, a.vocab);
+        const int64_t v = i * 32 + threadIdx.x;
+        if (j == 0 && threadIdx.x < 32) next_bias = v >= a.vocab ? -INFINITY : a.bias ? bias_units(a.bias[v], dv) : 0.0f;
+    };
+    auto store = [&](int64_t i, int j, int buf) {
+        t.store(tile[buf]);
+        if (j == 0 && threadIdx.x < 32) sb[(i - t0) & 1][threadIdx.x] = next_bias;
+    };
+    if (t0 < t1) {
+        fetch(t0, 0);
+        store(t0, 0, 0);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int64_t i = t0; i < t1; ++i) {
+        f32x16 s[1];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[0][j] = sb[(i - t0) & 1][8 * (j / 4) + 4 * h + j % 4];
+        for (int j = 0; j < chunks; ++j) {
+            x8 own[1][NS][DP / 16];
+            load_owned<E, NS, DP>(own[0], (const E *)a.x + offset(j), a.ldx, n, a.rows, dv.owned);
+            const bool more = j + 1 < chunks || i + 1 < t1;
+            if (more) fetch(j + 1 < chunks ? i : i + 1, j + 1 < chunks ? j + 1 : 0);
+            scores<E, NS, DP, 1>(s, own, tile[buf], 0);
+            if (j + 1 < chunks) {
+                store(i, j + 1, buf ^ 1);
+                __syncthreads();
+                buf ^= 1;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[0][j] = target - i * 32 == 8 * (j / 4) + j % 4 ? -INFINITY : s[0][j];
+        float mx = s[0][0];
+#pragma unroll
+        for (int j = 1; j < 16; ++j) mx = fmaxf(mx, s[0][j]);
+        mx = half_wave_max(mx);
+        if (__any((mx - m) * dv.c > LAG)) {
+            const float up = (mx - m) * dv.c > LAG ? mx : m, f = exp2_fast((m - up) * dv.c);
+            m = up;
+            l *= f;
+            if (GRAD)
+#pragma unroll
+                for (int b = 0; b < DP / 32; ++b) out[0][b] *= f;
+        }
+        const bool far = fabsf(m * dv.c) > FAR;
+        const float base = far ? P_SHIFT : P_SHIFT - m * dv.c, less = far ? m : 0.0f;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            float v8[1][8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v8[0][j] = exp2_fast(__builtin_fmaf(s[0][8 * k + j] - less, dv.c, base));
+                l += v8[0][j];
+            }
+            if (GRAD) pack_values<E, NS, 1>(p, v8, k);
+        }
+        if (GRAD) accumulate<E, NS, DP, 1>(out, p, tile[buf], 0);
+        if (i + 1 < t1) store(i + 1, 0, buf ^ 1);
+        __syncthreads();
+        buf ^= 1;
+    }
+    const float sum = half_wave_sum(l);
+    if (n >= a.rows) return;
+    const int64_t to = (int64_t)part * a.rows + n;
+    if (h == 0) {
+        a.pm[to + (int64_t)blockIdx.y * a.splits * a.rows] = m;
+        a.pl[to + (int64_t)blockIdx.y * a.splits * a.rows] = sum;
+    }
+    if (GRAD)
+#pragma unroll
+        for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *(float4 *)(a.po + to * a.dp + (int)blockIdx.y * DP + b * 32 + 8 * g + 4 * h) =
+                    make_float4(out[0][b][4 * g], out[0][b][4 * g + 1], out[0][b][4 * g + 2], out[0][b][4 * g + 3]);
+}
+
+template <typename T, typename E, int NS>
+__global__ __launch_bounds__(256, 1) void wide_table_kernel(SweepArgs a)
+{
+    constexpr int DP = 256;
+    typedef Tile<E, NS, DP> Tl;
+    typedef typename Half<E>::x8 x8;
+    static_assert(Tl::BV == 32, "one block of scores per tile");
+    __shared__ __attribute__((aligned(16))) E tile[2][Tl::SIZE];
+    __shared__ __attribute__((aligned(16))) RowFacts<32> facts[2];
+    const Derived dv = derive(NS == 2 ? a.scales : nullptr);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    const int part = blockIdx.x % a.splits;
+    const int64_t w0 = (int64_t)(blockIdx.x / a.splits) * 128 + wave * 32, v = w0 + (lane & 31);
+    const int64_t tiles = ceil_div(a.rows, 32), t0 = tiles * part / a.splits, t1 = tiles * (part + 1) / a.splits;
+    const int chunks = a.chunks, first = (int)blockIdx.y + 1;
+    auto offset = [&](int j) { return ((first + j) % chunks) * (NS * DP); };
+    f32x16 out[1][DP / 32];
+    Values<E, NS, 1> q;
+    const float bias = a.bias && v < a.vocab ? bias_units(a.bias[v], dv) : 0.0f;
+    float db[1] = {0.0f};
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b) out[0][b] = (f32x16)(0.0f);
+    Tl t;
+    bool keep[Tl::PER];
+    float next_m = 0.0f, next_r = 0.0f, next_g = 0.0f;
+    int32_t next_t = -1;
+    auto fetch = [&](int64_t i, int j) {
+        t.fetch((const E *)a.x + offset(j), a.ldx, i * 32, a.rows);
+#pragma unroll
+        for (int k = 0; k < Tl::PER; ++k) {
+            const int64_t n = i * 32 + (k * 256 + (int)threadIdx.x) / Tl::CHUNKS;
+            keep[k] = n < a.rows && a.row_target[n] >= 0;
+        }
+        if (j == 0 && threadIdx.x < 32) {
+            const int64_t n = i * 32 + threadIdx.x;
+            const bool ok = n < a.rows;
+            next_m = ok ? a.row_max[n] : INFINITY;
+            next_r = ok ? a.row_rate[n] : 0.0f;
+            next_g = ok ? a.row_weight[n] : 0.0f;
+            next_t = ok ? a.row_target[n] : -1;
+        }
+    };
+    auto store = [&](int64_t i, int j, int buf) {
+#pragma unroll
+        for (int k = 0; k < Tl::PER; ++k)
+            if (!keep[k]) t.held[k] = make_uint4(0, 0, 0, 0);
+        t.store(tile[buf]);
+        if (j == 0 && threadIdx.x < 32) {
+            const bool far = fabsf(next_m * dv.c) > FAR && next_m < INFINITY;
+            RowFacts<32> &f = facts[(i - t0) & 1];
+            f.m[threadIdx.x] = far ? 0.0f : -next_m * dv.c;
+            f.far[threadIdx.x] = far ? next_m : 0.0f;
+            f.rate[threadIdx.x] = next_r;
+            f.weight[threadIdx.x] = next_g;
+            f.target[threadIdx.x] = next_t;
+        }
+    };
+    if (t0 < t1) {
+        fetch(t0, 0);
+        store(t0, 0, 0);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int64_t i = t0; i < t1; ++i) {
+        const RowFacts<32> &f = facts[(i - t0) & 1];
+        f32x16 s[1] = {(f32x16)(bias)};
+        for (int j = 0; j < chunks; ++j) {
+            x8 own[1][NS][DP / 16];
+            load_owned<E, NS, DP>(own[0], (const E *)a.w + offset(j), a.ldw, v, a.vocab, dv.owned);
+            const bool more = j + 1 < chunks || i + 1 < t1;
+            if (more) fetch(j + 1 < chunks ? i : i + 1, j + 1 < chunks ? j + 1 : 0);
+            scores<E, NS, DP, 1>(s, own, tile[buf], 0);
+            if (j + 1 < chunks) {
+                store(i, j + 1, buf ^ 1);
+                __syncthreads();
+                buf ^= 1;
+            }
+        }
+        const bool hit = (uint32_t)(f.target[lane & 31] - (int32_t)w0) < 32u;
+        if (__any(hit || f.far[lane & 31] != 0.0f))
+            special_rows<E, NS, DP, 1, 32>(s, out, db, f, tile[buf], 0, (int32_t)w0, hit);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            float v8[1][8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int r = k * 16 + 8 * (j / 4) + 4 * h + j % 4;
+                v8[0][j] = exp2_fast(__builtin_fmaf(s[0][8 * k + j], dv.c, f.m[r])) * f.rate[r];
+                db[0] += v8[0][j];
+            }
+            pack_values<E, NS, 1>(q, v8, k);
+        }
+        accumulate<E, NS, DP, 1>(out, q, tile[buf], 0);
+        if (i + 1 < t1) store(i + 1, 0, buf ^ 1);
+        __syncthreads();
+        buf ^= 1;
+    }
+    write_table<T, NS, DP, 1>(a, out, db, v, part, (int)blockIdx.y * DP);
 }
 
 // ------------------------------------------------------------------- joins ---
@@ -724,7 +1100,27 @@ __global__ __launch_bounds__(256) void join_rows_kernel(JoinArgs j)
         l += j.pl[(int64_t)s * a.rows + n] * exp2_fast((j.pm[(int64_t)s * a.rows + n] - m) * dv.c);
     l = wave_sum(l);
     const T *x = (const T *)a.hidden + n * a.hidden_stride;
-    float lse = l == 0.0f ? -INFINITY : m <= dv.low * 0.999f ? -3.402823466e38f : ldexpf(m, -dv.k) + (logf(l) - P_SHIFT * LN2);
+    const int64_t t = target_of(a, n);
+    const float g = t < 0 ? 0.0f : a.weights ? a.weights[n] : 1.0f;
+    const T *wt = (const T *)a.table + (t < 0 ? 0 : t) * a.table_stride;
+    // l = sum without the target (times 2^7, about m).  With the target's score st and everything about the larger of the two:
+    // 1 - p[target] = l / (l + e), loss = log1p(l / e): nothing is lost where p[target] is near 1.
+    float st = 0.0f, e = 0.0f, loss = 0.0f;
+    if (t >= 0) {
+        for (int c = lane; c < a.d; c += 64) st = __builtin_fmaf((float)x[c], (float)wt[c], st);
+        st = wave_sum(st);
+        if (a.bias) st += a.bias[t];
+        const float su = bias_units(st, dv);  // (not only a bias: any score)
+        const float up = fmaxf(m, su);
+        e = exp2_fast((su - up) * dv.c + P_SHIFT);
+        const float f = exp2_fast((m - up) * dv.c);
+        l *= f;
+        m = up;
+        loss = st == -INFINITY ? INFINITY : l <= e ? log1pf(l / e) : ldexpf(m - su, -dv.k) + (logf(l + e) - P_SHIFT * LN2);
+    }
+    const float sum = l + e;
+    float lse = sum == 0.0f ? -INFINITY : m <= dv.low * 0.999f ? -3.402823466e38f : ldexpf(m, -dv.k) + (logf(sum) - P_SHIFT * LN2);
+    const float other = sum == 0.0f ? 1.0f : l / sum;  // 1 - p[target]
     const bool odd = j.ns == 2 && j.outlier[n];
     if (odd) {  // a row beyond x's scale: not finite, or without a target and far larger than the others
         bool finite = true;
@@ -743,18 +1139,8 @@ __global__ __launch_bounds__(256) void join_rows_kernel(JoinArgs j)
             lse = up + logf(sum);
         }
     }
-    const int64_t t = target_of(a, n);
-    const float g = t < 0 ? 0.0f : a.weights ? a.weights[n] : 1.0f;
-    float loss = 0.0f;
-    const T *wt = (const T *)a.table + (t < 0 ? 0 : t) * a.table_stride;
-    if (t >= 0) {
-        float s = 0.0f;
-        for (int c = lane; c < a.d; c += 64) s = __builtin_fmaf((float)x[c], (float)wt[c], s);
-        s = wave_sum(s);
-        if (a.bias) s += a.bias[t];
-        loss = s == -INFINITY ? INFINITY : lse - s;
-        loss *= g;
-    }
+    if (odd && t >= 0) loss = NAN;
+    loss = t < 0 ? 0.0f : g * loss;
     if (lane == 0) {
         a.lse[n] = lse;
         a.loss[n] = loss;
@@ -766,8 +1152,8 @@ __global__ __launch_bounds__(256) void join_rows_kernel(JoinArgs j)
         const float gs = ldexpf(g, shift);
         j.row_target[n] = (int32_t)t;
         j.row_max[n] = t < 0 ? INFINITY : m;
-        j.row_rate[n] = lost ? NAN : t < 0 || l == 0.0f ? 0.0f : gs * exp2_fast(P_SHIFT) / l;
-        j.row_weight[n] = gs;
+        j.row_rate[n] = lost ? NAN : t < 0 || sum == 0.0f ? 0.0f : gs * exp2_fast(P_SHIFT) / sum;
+        j.row_weight[n] = gs * other;
     }
     const int kw = j.ns == 2 ? j.scales->kw : 0;
     for (int c = lane; c < a.d; c += 64) {
@@ -778,8 +1164,8 @@ __global__ __launch_bounds__(256) void join_rows_kernel(JoinArgs j)
                 const int64_t at = (int64_t)s * a.rows + n;
                 o += j.po[at * j.dp + c] * exp2_fast((pm[at] - m) * dv.c);
             }
-            o = l == 0.0f ? 0.0f : ldexpf(o / l, -kw);
-            o = lost ? NAN : g * (o - (float)wt[c]);
+            o = sum == 0.0f ? 0.0f : ldexpf(o / sum, -kw);
+            o = lost ? NAN : g * (o - other * (float)wt[c]);
         }
         ((T *)a.d_hidden)[n * a.d + c] = (T)o;
     }
@@ -890,18 +1276,23 @@ Space space_for(const Plan &p, int64_t rows, int64_t vocab, bool grad, void *ws)
 template <typename E, int NS, int DP, bool WIDE>
 hipError_t sweep_rows(const SweepArgs &s, bool grad, hipStream_t st)
 {
-    // without the gradient one chunk's sweep does
-    const dim3 grid((unsigned)(ceil_div(s.rows, 128) * s.splits), WIDE && grad ? (unsigned)s.chunks : 1);
-    if (grad) rows_kernel<E, NS, DP, 1, true, WIDE><<<grid, 256, 0, st>>>(s);
-    else rows_kernel<E, NS, DP, 1, false, WIDE><<<grid, 256, 0, st>>>(s);
+    const unsigned blocks = (unsigned)(ceil_div(s.rows, 128) * s.splits);
+    if constexpr (WIDE) {
+        if (grad) wide_rows_kernel<E, NS, true><<<dim3(blocks, (unsigned)s.chunks), 256, 0, st>>>(s);
+        else wide_rows_kernel<E, NS, false><<<dim3(blocks), 256, 0, st>>>(s);  // without the gradient one chunk's sweep does
+    } else {
+        if (grad) rows_kernel<E, NS, DP, 1, true><<<dim3(blocks), 256, 0, st>>>(s);
+        else rows_kernel<E, NS, DP, 1, false><<<dim3(blocks), 256, 0, st>>>(s);
+    }
     return hipGetLastError();
 }
 
 template <typename T, typename E, int NS, int DP, bool WIDE>
 hipError_t sweep_table(const SweepArgs &s, hipStream_t st)
 {
-    const dim3 grid((unsigned)(ceil_div(s.vocab, 128) * s.splits), WIDE ? (unsigned)s.chunks : 1);
-    table_kernel<T, E, NS, DP, 1, WIDE><<<grid, 256, 0, st>>>(s);
+    const unsigned blocks = (unsigned)(ceil_div(s.vocab, 128) * s.splits);
+    if constexpr (WIDE) wide_table_kernel<T, E, NS><<<dim3(blocks, (unsigned)s.chunks), 256, 0, st>>>(s);
+    else table_kernel<T, E, NS, DP, 1><<<dim3(blocks), 256, 0, st>>>(s);
     return hipGetLastError();
 }
 
@@ -963,6 +1354,8 @@ hipError_t run(const lfm_softmax_args &a, bool grad, void *ws, hipStream_t st)
     w.rows = a.rows;
     w.vocab = a.vocab;
     w.bias = a.bias;
+    w.targets = a.targets;
+    w.id_bytes = a.id_bytes;
     w.scales = s.scales;
     w.splits = p.row_splits;
     w.d = a.d;

@@ -282,6 +282,41 @@ def test_softmax_same_bits_every_time(env, dtype):
             assert torch.equal(i, j)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows", [6, 70])
+def test_softmax_rows_that_fit_well(env, dtype, rows):
+    """Targets with a probability near 1: loss and gradient are small differences and keep their relative precision (the
+    target's part is formed from the sum over the OTHER items).  Bounds: a probability is off by ds + dlse as in `reference`,
+    relatively; every product's operand by `half` of its own size; so all errors are relative to sums of |q|-like terms."""
+    torch, ops = env
+    x, w, t, b, _ = make(torch, rows, 400, 64, dtype, seed=21, weights=False, ignored=False)
+    t = torch.randperm(400, device="cuda")[:rows]
+    x = (w[t].double() * 0.9 + x.double() * 0.1).to(x.dtype)   # s[target] ~ 0.9 |w|^2 ~ 14, the others ~ N(0, 4)
+    loss, lse, dx, dw, db = ops.softmax_loss_grad(x, w, t, bias=b)
+    xx, ww = x.double(), w.double()
+    s = xx @ ww.t() + b.double()
+    ds = (64 * U32 + 2.0 ** -20) * (xx.abs() @ ww.abs().t()) + 8 * U32 * s.abs()
+    rel = 2 * ds.max(1).values[:, None] + (400 + 128) * U32       # of exp(s - s_target) and of sums of them
+    st = s.gather(1, t[:, None])
+    e = torch.exp(s - st)
+    e[torch.arange(rows, device="cuda"), t] = 0.0
+    others = e.sum(1, keepdim=True)
+    assert float(others.median()) < 0.05
+    want = torch.log1p(others).squeeze(1)
+    near(torch, loss, want, (rel.squeeze(1) + 8 * U32) * want, "loss")
+    q, rest = e / (1 + others), others / (1 + others)
+    half = 2.0 ** -21 if dtype == "f32" else unit(torch, x.dtype)
+    u = 2 * unit(torch, x.dtype)
+    gx = q @ ww - rest * ww[t]
+    near(torch, dx, gx, (2 * rel + half + 2.0 ** -19) * (q @ ww.abs() + rest * ww[t].abs()) + u * gx.abs() + 2.0 ** -24, "d_hidden")
+    hot = torch.zeros_like(q)
+    hot[torch.arange(rows, device="cuda"), t] = 1.0
+    gw = q.t() @ xx - hot.t() @ (rest * xx)
+    near(torch, dw, gw, ((2 * rel + half + 2.0 ** -19) * q).t() @ xx.abs() + hot.t() @ ((2 * rel + half) * rest * xx.abs()) + u * gw.abs() + 2.0 ** -24, "d_table")
+    gb = q.sum(0) - (hot * rest).sum(0)
+    near(torch, db, gb, ((2 * rel + 128 * U32) * (q + hot * rest)).sum(0) + 1e-30, "d_bias")
+
+
 def test_softmax_gradient_against_differences(env):
     """sum(loss) along random directions: (L(+h) - L(-h)) / 2h, from a 64-bit restatement of the LOSS alone, against the
     kernel's gradients.  The difference's own error: h^2 / 6 times the third derivative along the direction, at most
