@@ -26,13 +26,6 @@
 
 #include <math.h>
 
-#ifndef LFM_ROWS_WAVES
-#define LFM_ROWS_WAVES 2
-#endif
-#ifndef LFM_TABLE_WAVES
-#define LFM_TABLE_WAVES 2
-#endif
-
 namespace lfm {
 namespace ops {
 namespace {
@@ -274,26 +267,55 @@ __device__ inline void load_owned(typename Half<E>::x8 (&f)[NS][DP / 16], const 
     }
 }
 
-// acc += 32 rows of the tile (from row r0) x the owned rows
-template <typename E, int NS, int DP, int CW>
-__device__ inline void scores(f32x16 (&acc)[CW], const typename Half<E>::x8 (&own)[CW][NS][DP / 16], const E *tile, int r0)
+// The two shapes in which a block of 32 streamed rows (from row r0 of the tile) enters the products.  They are read ahead of
+// the instructions that use them: the reads of one are in flight while the other's products or the exponentials run.
+template <typename E, int NS, int DP>
+struct ScoreOperand {  // rows of the block: lane = row, 8 columns at a time
+    typename Half<E>::x8 v[NS][DP / 16];
+
+    __device__ inline void read(const E *tile, int r0)
+    {
+        const int lane = threadIdx.x & 63;
+        const E *p = tile + (r0 + (lane & 31)) * Tile<E, NS, DP>::ROW + (lane >> 5) * 8;
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k) v[s][k] = *(const typename Half<E>::x8 *)(p + s * DP + k * 16);
+    }
+};
+
+template <typename E, int NS, int DP>
+struct SumOperand {  // columns of the block: lane = column, the rows in the order in which a lane holds its scores
+    typename Half<E>::x8 v[NS][2][DP / 32];
+
+    __device__ inline void read(const E *tile, int r0)
+    {
+        typedef typename Half<E>::x4 x4;
+        constexpr int ROW = Tile<E, NS, DP>::ROW;
+        const int lane = threadIdx.x & 63;
+        const E *p = tile + (r0 + 4 * (lane >> 5) + ((lane & 15) >> 2)) * ROW + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int b = 0; b < DP / 32; ++b) {
+                    const x4 lo = read_column(p + s * DP + k * 16 * ROW + b * 32), hi = read_column(p + s * DP + (k * 16 + 8) * ROW + b * 32);
+                    v[s][k][b] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                }
+    }
+};
+
+// acc += block x owned rows
+template <typename E, int NS, int DP>
+__device__ inline void scores(f32x16 &acc, const typename Half<E>::x8 (&own)[NS][DP / 16], const ScoreOperand<E, NS, DP> &a)
 {
-    typedef typename Half<E>::x8 x8;
-    constexpr int ROW = Tile<E, NS, DP>::ROW;
-    const int lane = threadIdx.x & 63;
-    const E *p = tile + (r0 + (lane & 31)) * ROW + (lane >> 5) * 8;
 #pragma unroll
     for (int k = 0; k < DP / 16; ++k) {
-        const x8 hi = *(const x8 *)(p + k * 16);
-#pragma unroll
-        for (int w = 0; w < CW; ++w) acc[w] = mfma(hi, own[w][0][k], acc[w]);
+        acc = mfma(a.v[0][k], own[0][k], acc);
         if (NS == 2) {
-            const x8 lo = *(const x8 *)(p + DP + k * 16);
-#pragma unroll
-            for (int w = 0; w < CW; ++w) {
-                acc[w] = mfma(lo, own[w][0][k], acc[w]);
-                acc[w] = mfma(hi, own[w][NS - 1][k], acc[w]);
-            }
+            acc = mfma(a.v[NS - 1][k], own[0][k], acc);
+            acc = mfma(a.v[0][k], own[NS - 1][k], acc);
         }
     }
 }
@@ -325,67 +347,59 @@ __device__ inline Half<f16_t>::x8 cut_values(const float (&v)[8])
     return u.r;
 }
 
-template <typename E, int NS, int CW>
+template <typename E, int NS>
 struct Values {  // the probabilities of 32 streamed rows as matrix operands
-    typename Half<E>::x8 hi[CW][2], lo[NS == 2 ? CW : 1][2];
-};
+    typename Half<E>::x8 v[NS][2];
 
-template <typename E, int NS, int CW>
-__device__ inline void clear_values(Values<E, NS, CW> &p)
-{
-#pragma unroll
-    for (int w = 0; w < CW; ++w)
+    __device__ inline void pack(const float (&q)[16])
+    {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            p.hi[w][k] = (typename Half<E>::x8)((E)0.0f);
-            if (NS == 2) p.lo[w][k] = (typename Half<E>::x8)((E)0.0f);
+            float part[8], rest[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) part[j] = q[8 * k + j];
+            if constexpr (NS == 2) {
+                v[0][k] = cut_values(part);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) rest[j] = __builtin_fmaf((float)v[0][k][j], -1.0f, part[j]);
+                v[NS - 1][k] = cut_values(rest);
+            } else
+                v[0][k] = round_values(part, typename Half<E>::x8());
         }
-}
+    }
+};
 
-template <typename E, int NS, int CW>
-__device__ inline void pack_values(Values<E, NS, CW> &p, const float (&v)[CW][8], int k)
+// out[d, owned] += block^T x values
+template <typename E, int NS, int DP>
+__device__ inline void accumulate(f32x16 (&out)[DP / 32], const Values<E, NS> &p, const SumOperand<E, NS, DP> &a)
 {
-#pragma unroll
-    for (int w = 0; w < CW; ++w)
-        if constexpr (NS == 2) {
-            float rest[8];
-            p.hi[w][k] = cut_values(v[w]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) rest[j] = __builtin_fmaf((float)p.hi[w][k][j], -1.0f, v[w][j]);
-            p.lo[w][k] = cut_values(rest);
-        } else
-            p.hi[w][k] = round_values(v[w], typename Half<E>::x8());
-}
-
-// out[d, owned] += tile^T x values for 32 rows of the tile (from row r0)
-template <typename E, int NS, int DP, int CW>
-__device__ inline void accumulate(f32x16 (&out)[CW][DP / 32], const Values<E, NS, CW> &p, const E *tile, int r0)
-{
-    typedef typename Half<E>::x8 x8;
-    typedef typename Half<E>::x4 x4;
-    constexpr int ROW = Tile<E, NS, DP>::ROW;
-    const int lane = threadIdx.x & 63;
-    const E *at = tile + (r0 + 4 * (lane >> 5) + ((lane & 15) >> 2)) * ROW + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int b = 0; b < DP / 32; ++b) {
-            const E *c = at + k * 16 * ROW + b * 32;
-            const x4 h0 = read_column(c), h1 = read_column(c + 8 * ROW);
-            const x8 th = __builtin_shufflevector(h0, h1, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-            for (int w = 0; w < CW; ++w) out[w][b] = mfma(th, p.hi[w][k], out[w][b]);
+            out[b] = mfma(a.v[0][k][b], p.v[0][k], out[b]);
             if (NS == 2) {
-                const x4 l0 = read_column(c + DP), l1 = read_column(c + DP + 8 * ROW);
-                const x8 tl = __builtin_shufflevector(l0, l1, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-                for (int w = 0; w < CW; ++w) {
-                    out[w][b] = mfma(tl, p.hi[w][k], out[w][b]);
-                    out[w][b] = mfma(th, p.lo[w][k], out[w][b]);
-                }
+                out[b] = mfma(a.v[NS - 1][k][b], p.v[0][k], out[b]);
+                out[b] = mfma(a.v[0][k][b], p.v[NS - 1][k], out[b]);
             }
         }
 }
+
+// The plane of (owned rows, streamed tiles) is cut into as many equal pieces as blocks fit on the card, whatever the sizes: a
+// block takes `tiles` consecutive tiles, the last of one owner and the first of the next among them.
+struct Pieces {
+    uint32_t owners, tiles, blocks;  // owners * tiles units, dealt to `blocks` blocks
+
+    __host__ __device__ inline uint64_t begin(uint32_t block) const { return (uint64_t)owners * tiles * block / blocks; }
+    __host__ __device__ inline uint32_t block_of(uint64_t unit) const
+    {
+        return (uint32_t)(((unit + 1) * blocks - 1) / ((uint64_t)owners * tiles));
+    }
+    __host__ __device__ inline uint32_t first_block(uint32_t owner) const { return block_of((uint64_t)owner * tiles); }
+    __host__ __device__ inline uint32_t last_block(uint32_t owner) const { return block_of((uint64_t)owner * tiles + tiles - 1); }
+    // most blocks that one owner is spread over
+    __host__ __device__ inline uint32_t most() const { return (blocks + owners - 1) / owners + 1; }
+};
 
 struct SweepArgs {
     const void *x, *w;      // packed or in place
@@ -395,269 +409,186 @@ struct SweepArgs {
     const Scales *scales;
     const void *targets;    // rows_kernel: [rows], id_bytes wide
     int id_bytes;
-    int splits;             // parts of the streamed side
+    Pieces pieces;
     int d, dp;
     int chunks;             // of 256 columns (WIDE; else 1): the second product's columns are blockIdx.y's
-    // rows_kernel: per chunk, part and row, the row's target left out
+    // rows_kernel: per chunk, part and row, the row's target left out (the parts of a row are the blocks of its owner)
     float *pm, *pl, *po;    // maximum (matrix units), sum of 2^7 p; per part and row: sum of 2^7 p w [dp]
+    int parts;
     // table_kernel: per row
     const float *row_max, *row_rate, *row_weight;  // maximum (matrix units; +inf: no target), 2^shift g / sum, 2^shift g (1 - p[target])
     const int32_t *row_target;
-    void *dw;               // one part: the result
-    float *db, *pw, *pb;    // several: partial sums per part [vocab][dp], [vocab]
+    void *dw;               // table rows that one block has to itself
+    float *db, *pw, *pb;    // the others': per block its first and its last owner, [128][dp], [128]
     int shifted;            // q is scaled by 2^(14 - eg): 0 no (bfloat16), 1 with eg = 0, 2 with eg of scales
 };
 
-// Both sweeps are pipelined over blocks of 32 streamed rows: a step makes the scores of block b + 1 and the second product
-// of block b - 1 on the matrix cores while the vector units turn the scores of block b into probabilities.  None of the
-// three waits for another, so a wave keeps both busy by itself.  Tiles rotate through BUFS buffers of LDS, so that a tile
-// is free again two steps after its last score and one barrier per tile does.
-template <typename E, int NS, int DP>
-struct Rotation {
-    static constexpr int BLOCKS = Tile<E, NS, DP>::BV / 32, BUFS = BLOCKS == 2 ? 3 : 4;
-    // tiles stored ahead of the first step, before which the next tile is stored
-    static constexpr int AHEAD = BLOCKS == 2 ? 1 : 2;
+// WIDE: more than 256 columns, taken 256 at a time.  The scores add up over the chunks (the owned operand is read again for
+// each, from the caches); a block accumulates the second product of one chunk, blockIdx.y's, which it streams last.  The
+// scores' work is repeated for every chunk of the result: a width that is rare is not worth a second shape of block.
+template <typename E, int NS, int DP, bool WIDE>
+struct Stream {
+    typedef Tile<E, NS, DP> Tl;
+    static constexpr int BLOCKS = Tl::BV / 32;
+    int chunks, first;
+    __device__ inline explicit Stream(int chunks_) : chunks(WIDE ? chunks_ : 1), first(WIDE ? (int)blockIdx.y + 1 : 0) {}
+    __device__ inline int offset(int j) const { return WIDE ? ((first + j) % chunks) * (NS * DP) : 0; }  // of the j-th chunk
 };
 
-// What a step has to hide: one matrix instruction, an LDS read, a few vector instructions, and so on
-template <int MATRIX, int VECTOR>
-__device__ inline void interleave()
-{
-#ifndef LFM_NO_INTERLEAVE
-#pragma unroll
-    for (int i = 0; i < MATRIX; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x002, VECTOR, 0);
-    }
+// registers: two waves per SIMD while the operands leave room for it, one beyond
+#ifndef W1
+constexpr int waves_for(int ns, int dp, bool sums) { return ns * dp > (sums ? 192 : 256) ? 1 : 2; }
+#else
+constexpr int waves_for(int ns, int dp, bool sums) { return W1; }
 #endif
-}
+#ifdef RA
+#define READ_AHEAD() __builtin_amdgcn_sched_barrier(0)
+#else
+#define READ_AHEAD()
+#endif
 
-template <typename E, int NS, int DP, int CW, bool GRAD>
-__global__ __launch_bounds__(256, (GRAD ? NS * DP >= 384 : NS * DP >= 512) ? 1 : LFM_ROWS_WAVES) void rows_kernel(SweepArgs a)
+
+template <typename E, int NS, int DP, bool GRAD, bool WIDE>
+__global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, GRAD)) void rows_kernel(SweepArgs a)
 {
     typedef Tile<E, NS, DP> Tl;
-    typedef Rotation<E, NS, DP> Ro;
-    typedef typename Half<E>::x8 x8;
-    __shared__ __attribute__((aligned(16))) E tile[Ro::BUFS][Tl::SIZE];
-    __shared__ __attribute__((aligned(16))) float sb[Ro::BUFS][Tl::BV];
+    typedef Stream<E, NS, DP, WIDE> St;
+    static_assert(!WIDE || St::BLOCKS == 1, "a chunk per tile");
+    __shared__ __attribute__((aligned(16))) E tile[2][Tl::SIZE];
+    __shared__ __attribute__((aligned(16))) float sb[2][Tl::BV];
     const Derived dv = derive(NS == 2 ? a.scales : nullptr);
+    const St sm(a.chunks);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-    const uint32_t part = blockIdx.x % (uint32_t)a.splits;
-    const int64_t n0 = (int64_t)(blockIdx.x / (uint32_t)a.splits) * (128 * CW) + wave * (32 * CW) + (lane & 31);
-    const uint32_t tiles = (uint32_t)((a.vocab + Tl::BV - 1) / Tl::BV);
-    const uint32_t t0 = (uint32_t)((uint64_t)tiles * part / (uint32_t)a.splits);
-    const int nt = (int)((uint64_t)tiles * (part + 1) / (uint32_t)a.splits) - (int)t0;
-
-    x8 own[CW][NS][DP / 16];
-    f32x16 out[CW][DP / 32], cur[CW], next[CW];
-    Values<E, NS, CW> p;
-    float m[CW], l[CW];
-    int32_t target[CW];
-#pragma unroll
-    for (int w = 0; w < CW; ++w) {
-        const int64_t n = n0 + 32 * w;
-        load_owned<E, NS, DP>(own[w], (const E *)a.x, a.ldx, n, a.rows, dv.owned);
+    uint64_t unit = a.pieces.begin(blockIdx.x);
+    const uint64_t end = a.pieces.begin(blockIdx.x + 1);
+    while (unit < end) {
+        const uint32_t owner = (uint32_t)(unit / a.pieces.tiles), t0 = (uint32_t)(unit - (uint64_t)owner * a.pieces.tiles);
+        const uint64_t left = end - unit;
+        const int nt = (int)(a.pieces.tiles - t0 < left ? a.pieces.tiles - t0 : left);
+        unit += nt;
+        const int64_t n = (int64_t)owner * 128 + wave * 32 + (lane & 31);
+        typename Half<E>::x8 own[NS][DP / 16];
+        if (!WIDE) load_owned<E, NS, DP>(own, (const E *)a.x, a.ldx, n, a.rows, dv.owned);
         const int64_t at = n >= a.rows ? -1 : a.id_bytes == 8 ? ((const int64_t *)a.targets)[n] : (int64_t)((const int32_t *)a.targets)[n];
-        target[w] = (uint64_t)at < (uint64_t)a.vocab ? (int32_t)at - 4 * h : INT32_MIN / 2;
-        m[w] = dv.low * 1.01f;
-        l[w] = 0.0f;
-        if (GRAD) {
+        const uint32_t target = (uint64_t)at < (uint64_t)a.vocab ? (uint32_t)at : 0xc0000000u;  // (no row of the table)
+        f32x16 out[DP / 32];
+        float m = dv.low * 1.01f, l = 0.0f;
+        if (GRAD)
 #pragma unroll
-            for (int b = 0; b < DP / 32; ++b) out[w][b] = (f32x16)(0.0f);
-        }
-    }
-    clear_values(p);
+            for (int b = 0; b < DP / 32; ++b) out[b] = (f32x16)(0.0f);
 
-    Tl t;
-    float next_bias = 0.0f;
-    auto fetch = [&](int i) {
-        const int64_t r = (int64_t)(t0 + i) * Tl::BV;
-        t.fetch((const E *)a.w, a.ldw, r, a.vocab);
-        const int64_t v = r + threadIdx.x;
-        if (threadIdx.x < Tl::BV) next_bias = v >= a.vocab ? -INFINITY : a.bias ? bias_units(a.bias[v], dv) : 0.0f;
-    };
-    auto store = [&](int buf) {
-        t.store(tile[buf]);
-        if (threadIdx.x < Tl::BV) sb[buf][threadIdx.x] = next_bias;
-    };
-    auto score = [&](f32x16 (&s)[CW], int buf, int r0) {
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const float4 b = *(const float4 *)&sb[buf][r0 + 8 * g + 4 * h];
-#pragma unroll
-            for (int w = 0; w < CW; ++w) {
-                s[w][4 * g + 0] = b.x;
-                s[w][4 * g + 1] = b.y;
-                s[w][4 * g + 2] = b.z;
-                s[w][4 * g + 3] = b.w;
-            }
-        }
-        scores<E, NS, DP, CW>(s, own, tile[buf], r0);
-    };
-    // the step of the block whose first vocabulary row is v: before_* the block before it, after_* the one behind it
-    auto step = [&](int32_t v, int before, int before_r, int after, int after_r) {
-        // the target's own score is left to the join, in float32: what remains is not a difference of near-equals
-        bool here = false;
-#pragma unroll
-        for (int w = 0; w < CW; ++w) here |= (uint32_t)target[w] + 4 * h - (uint32_t)v < 32u;
-        if (__any(here)) {  // one block in some
-#pragma unroll
-            for (int w = 0; w < CW; ++w)
-#pragma unroll
-                for (int j = 0; j < 16; ++j) cur[w][j] = (uint32_t)target[w] - (uint32_t)v == 8u * (j / 4) + j % 4 ? -INFINITY : cur[w][j];
-        }
-        bool grows = false;
-        float mx[CW];
-#pragma unroll
-        for (int w = 0; w < CW; ++w) {
-            mx[w] = cur[w][0];
-#pragma unroll
-            for (int j = 1; j < 16; ++j) mx[w] = fmaxf(mx[w], cur[w][j]);
-            mx[w] = half_wave_max(mx[w]);
-            grows |= (mx[w] - m[w]) * dv.c > LAG;
-        }
-        if (__any(grows)) {  // seldom after the first blocks; by row, so that no row's bits depend on its neighbours
-            if (GRAD) {
-                accumulate<E, NS, DP, CW>(out, p, tile[before], before_r);  // still about the old maximum
-                clear_values(p);
-            }
-#pragma unroll
-            for (int w = 0; w < CW; ++w) {
-                const float up = (mx[w] - m[w]) * dv.c > LAG ? mx[w] : m[w], f = exp2_fast((m[w] - up) * dv.c);
-                m[w] = up;
-                l[w] *= f;
-                if (GRAD)
-#pragma unroll
-                    for (int b = 0; b < DP / 32; ++b) out[w][b] *= f;
-            }
-        }
-        float base[CW];
-        bool far = false;
-#pragma unroll
-        for (int w = 0; w < CW; ++w) {
-            base[w] = P_SHIFT - m[w] * dv.c;
-            far |= fabsf(m[w] * dv.c) > FAR;
-        }
-        if (__any(far)) {  // the rounding of m c would show: subtract first
-#pragma unroll
-            for (int w = 0; w < CW; ++w) {
-                const bool mine = fabsf(m[w] * dv.c) > FAR;
-                const float less = mine ? m[w] : 0.0f;
-                base[w] = mine ? P_SHIFT : base[w];
-                cur[w] -= less;
-            }
-        }
-        score(next, after, after_r);
-        if (GRAD) accumulate<E, NS, DP, CW>(out, p, tile[before], before_r);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            float v8[CW][8];
-#pragma unroll
-            for (int w = 0; w < CW; ++w)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    v8[w][j] = exp2_fast(__builtin_fmaf(cur[w][8 * k + j], dv.c, base[w]));
-                    l[w] += v8[w][j];
-                }
-            if (GRAD) pack_values<E, NS, CW>(p, v8, k);
-        }
-        constexpr int MATRIX = CW * (NS == 2 ? 3 : 1) * (DP / 16) * (GRAD ? 2 : 1), VECTOR = CW * (GRAD ? NS == 2 ? 96 : 72 : 56);
-        interleave<MATRIX, (VECTOR + MATRIX - 1) / MATRIX>();
-#pragma unroll
-        for (int w = 0; w < CW; ++w) cur[w] = next[w];
-    };
-
-    if (nt > 0) {
-        fetch(0);
-        store(0);
-        if (Ro::AHEAD == 2 && nt > 1) {
-            fetch(1);
-            store(1);
-        }
-        if (nt > Ro::AHEAD) fetch(Ro::AHEAD);
+        Tl t;
+        float next_bias = 0.0f;
+        auto fetch = [&](int i, int j) {
+            const int64_t r = (int64_t)(t0 + i) * Tl::BV, v = r + threadIdx.x;
+            t.fetch((const E *)a.w + sm.offset(j), a.ldw, r, a.vocab);
+            if (j == 0 && threadIdx.x < Tl::BV) next_bias = v >= a.vocab ? -INFINITY : a.bias ? bias_units(a.bias[v], dv) : 0.0f;
+        };
+        auto store = [&](int i, int j, int buf) {
+            t.store(tile[buf]);
+            if (j == 0 && threadIdx.x < Tl::BV) sb[i & 1][threadIdx.x] = next_bias;
+        };
+        __syncthreads();  // (the owner before is done with the tiles)
+        fetch(0, 0);
+        store(0, 0, 0);
         __syncthreads();
-        score(cur, 0, 0);
-    }
-    int b0 = 0, b1 = 1, before = 0;  // the buffers of tile i, i + 1, i - 1
-    for (int i = 0; i < nt; ++i) {
-        int b2 = b1 + 1 == Ro::BUFS ? 0 : b1 + 1;
-        const int into = Ro::BLOCKS == 2 ? b1 : b2;
-        if (i + Ro::AHEAD < nt) store(into);
-        if (i + Ro::AHEAD + 1 < nt) fetch(i + Ro::AHEAD + 1);
-        const int32_t v = (int32_t)((t0 + i) * Tl::BV);
-        const int after = i + 1 < nt ? b1 : b0;  // (behind the last block: scores that nobody looks at)
-        if (Ro::BLOCKS == 2) {
-            step(v, before, i ? 32 : 0, b0, 32);
-            __syncthreads();
-            step(v + 32, b0, 0, after, 0);
-        } else {
-            step(v, before, 0, after, 0);
-            __syncthreads();
-        }
-        before = b0;
-        b0 = b1;
-        b1 = b2;
-    }
-    if (GRAD && nt > 0) accumulate<E, NS, DP, CW>(out, p, tile[before], Tl::BV - 32);
+        int buf = 0;
+        ScoreOperand<E, NS, DP> so;
+        so.read(tile[0], 0);
+        for (int i = 0; i < nt; ++i) {
+            if (!WIDE && i + 1 < nt) fetch(i + 1, 0);
 #pragma unroll
-    for (int w = 0; w < CW; ++w) {
-        const int64_t n = n0 + 32 * w;
-        const float sum = half_wave_sum(l[w]);
+            for (int blk = 0; blk < St::BLOCKS; ++blk) {
+                SumOperand<E, NS, DP> to;
+                f32x16 s;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const float4 b = *(const float4 *)&sb[i & 1][blk * 32 + 8 * g + 4 * h];
+                    s[4 * g + 0] = b.x;
+                    s[4 * g + 1] = b.y;
+                    s[4 * g + 2] = b.z;
+                    s[4 * g + 3] = b.w;
+                }
+                if (WIDE) {
+                    for (int j = 0; j < sm.chunks; ++j) {
+                        load_owned<E, NS, DP>(own, (const E *)a.x + sm.offset(j), a.ldx, n, a.rows, dv.owned);
+                        const bool last = j + 1 == sm.chunks;
+                        if (!last || i + 1 < nt) fetch(last ? i + 1 : i, last ? 0 : j + 1);
+                        scores<E, NS, DP>(s, own, so);
+                        if (last) break;
+                        store(i, j + 1, buf ^ 1);
+                        __syncthreads();
+                        buf ^= 1;
+                        so.read(tile[buf], 0);
+                    }
+                    if (GRAD) to.read(tile[buf], 0);
+                } else {
+                    if (GRAD) to.read(tile[buf], blk * 32);
+                    READ_AHEAD();
+                    scores<E, NS, DP>(s, own, so);
+                }
+                // what comes next is on its way while this block's exponentials run
+                if (blk + 1 < St::BLOCKS) so.read(tile[buf], 32);
+                else {
+                    if (i + 1 < nt) store(i + 1, 0, buf ^ 1);
+                    __syncthreads();
+                    so.read(tile[i + 1 < nt ? buf ^ 1 : buf], 0);
+                }
+                READ_AHEAD();
+                // the target's own score is left to the join, in float32: what remains is not a difference of near-equals
+                const uint32_t hit = target - ((t0 + i) * (uint32_t)Tl::BV + blk * 32u);
+                if (__any(hit < 32u)) {  // one block in some
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) s[j] = hit == 8u * (j / 4) + 4u * h + j % 4 ? -INFINITY : s[j];
+                }
+                float mx = s[0];
+#pragma unroll
+                for (int j = 1; j < 16; ++j) mx = fmaxf(mx, s[j]);
+                mx = half_wave_max(mx);
+                const bool grows = (mx - m) * dv.c > LAG;
+                if (__any(grows)) {  // seldom after the first blocks; by row, so that no row's bits depend on its neighbours
+                    const float up = grows ? mx : m, f = exp2_fast((m - up) * dv.c);
+                    m = up;
+                    l *= f;
+                    if (GRAD)
+#pragma unroll
+                        for (int b = 0; b < DP / 32; ++b) out[b] *= f;
+                }
+                float base = P_SHIFT - m * dv.c;
+                const bool far = fabsf(m * dv.c) > FAR;
+                if (__any(far)) {  // the rounding of m c would show: subtract first
+                    s -= far ? m : 0.0f;
+                    base = far ? P_SHIFT : base;
+                }
+                float q[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    q[j] = exp2_fast(__builtin_fmaf(s[j], dv.c, base));
+                    l += q[j];
+                }
+                if (GRAD) {
+                    Values<E, NS> p;
+                    p.pack(q);
+                    accumulate<E, NS, DP>(out, p, to);
+                }
+            }
+            buf ^= 1;
+        }
+        const float sum = half_wave_sum(l);
         if (n >= a.rows) continue;
-        const int64_t at = (int64_t)part * a.rows + n;
+        const int64_t part = (int64_t)(blockIdx.x - a.pieces.first_block(owner)) * a.rows + n;
         if (h == 0) {
-            a.pm[at] = m[w];
-            a.pl[at] = sum;
+            const int64_t to = part + (WIDE ? (int64_t)blockIdx.y * a.parts * a.rows : 0);
+            a.pm[to] = m;
+            a.pl[to] = sum;
         }
         if (GRAD)
 #pragma unroll
             for (int b = 0; b < DP / 32; ++b)
 #pragma unroll
                 for (int g = 0; g < 4; ++g)
-                    *(float4 *)(a.po + at * DP + b * 32 + 8 * g + 4 * h) =
-                        make_float4(out[w][b][4 * g], out[w][b][4 * g + 1], out[w][b][4 * g + 2], out[w][b][4 * g + 3]);
-    }
-}
-
-// Writes a wave's part of dw (or its partial sums) and db
-template <typename T, int NS, int DP, int CW>
-__device__ inline void write_table(const SweepArgs &a, const f32x16 (&out)[CW][DP / 32], const float (&db)[CW], int64_t v0, int64_t part, int c0)
-{
-    const int h = (threadIdx.x & 63) >> 5;
-    const int shift = a.shifted == 2 ? a.scales->eg - 14 : a.shifted ? -14 : 0, kx = NS == 2 ? a.scales->kx : 0;
-#pragma unroll
-    for (int w = 0; w < CW; ++w) {
-        const int64_t v = v0 + 32 * w;
-        const float total = half_wave_sum(db[w]);
-        if (v >= a.vocab) continue;
-        if (a.splits > 1) {
-            const int64_t at = part * a.vocab + v;
-            if (h == 0 && c0 == 0) a.pb[at] = total;
-#pragma unroll
-            for (int b = 0; b < DP / 32; ++b)
-#pragma unroll
-                for (int g = 0; g < 4; ++g)
-                    *(float4 *)(a.pw + at * a.dp + c0 + b * 32 + 8 * g + 4 * h) =
-                        make_float4(out[w][b][4 * g], out[w][b][4 * g + 1], out[w][b][4 * g + 2], out[w][b][4 * g + 3]);
-        } else {
-            if (a.db && h == 0 && c0 == 0) a.db[v] = ldexpf(total, shift);
-            T *row = (T *)a.dw + v * a.d;
-#pragma unroll
-            for (int b = 0; b < DP / 32; ++b)
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int c = c0 + b * 32 + 8 * g + 4 * h;
-                    Vec<T, 4> o;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) o.v[j] = (T)ldexpf(out[w][b][4 * g + j], shift - kx);
-                    if (c + 4 <= a.d && (a.d & 3) == 0) *(Vec<T, 4> *)(row + c) = o;
-                    else
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            if (c + j < a.d) row[c + j] = o.v[j];
-                }
-        }
+                    *(float4 *)(a.po + part * a.dp + (WIDE ? (int)blockIdx.y * DP : 0) + b * 32 + 8 * g + 4 * h) =
+                        make_float4(out[b][4 * g], out[b][4 * g + 1], out[b][4 * g + 2], out[b][4 * g + 3]);
     }
 }
 
@@ -671,384 +602,184 @@ struct RowFacts {
     int32_t target[BV];
 };
 
-// The rare part of a block of scores: rows whose target is among the owned table rows leave the sum here and enter it as
-// -g (1 - p) x, in float32; rows that FAR is about lose their maximum first.
-template <typename E, int NS, int DP, int CW, int BV>
-__device__ inline void special_rows(f32x16 (&s)[CW], f32x16 (&out)[CW][DP / 32], float (&db)[CW], const RowFacts<BV> &f, const E *tile, int r0,
-                                    int32_t w0, bool hit)
+template <typename T, typename E, int NS, int DP, bool WIDE>
+__global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, true)) void table_kernel(SweepArgs a)
 {
-    const int lane = threadIdx.x & 63, h = lane >> 5;
+    typedef Tile<E, NS, DP> Tl;
+    typedef Stream<E, NS, DP, WIDE> St;
+    static_assert(!WIDE || St::BLOCKS == 1, "a chunk per tile");
+    __shared__ __attribute__((aligned(16))) E tile[2][Tl::SIZE];
+    __shared__ __attribute__((aligned(16))) RowFacts<Tl::BV> facts[2];
+    const Derived dv = derive(NS == 2 ? a.scales : nullptr);
+    const St sm(a.chunks);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    const int shift = a.shifted == 2 ? a.scales->eg - 14 : a.shifted ? -14 : 0, kx = NS == 2 ? a.scales->kx : 0;
+    const int c0 = WIDE ? (int)blockIdx.y * DP : 0;
+    const uint64_t begin = a.pieces.begin(blockIdx.x), end = a.pieces.begin(blockIdx.x + 1);
+    uint64_t unit = begin;
+    while (unit < end) {
+        const uint32_t owner = (uint32_t)(unit / a.pieces.tiles), t0 = (uint32_t)(unit - (uint64_t)owner * a.pieces.tiles);
+        const uint64_t left = end - unit;
+        const int nt = (int)(a.pieces.tiles - t0 < left ? a.pieces.tiles - t0 : left);
+        unit += nt;
+        const int32_t w0 = (int32_t)(owner * 128 + wave * 32);
+        const int64_t v = (int64_t)w0 + (lane & 31);
+        typename Half<E>::x8 own[NS][DP / 16];
+        if (!WIDE) load_owned<E, NS, DP>(own, (const E *)a.w, a.ldw, v, a.vocab, dv.owned);
+        const float bias = a.bias && v < a.vocab ? bias_units(a.bias[v], dv) : 0.0f;
+        float db = 0.0f;
+        f32x16 out[DP / 32];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-        const int r = r0 + 8 * (j / 4) + 4 * h + j % 4;
+        for (int b = 0; b < DP / 32; ++b) out[b] = (f32x16)(0.0f);
+
+        Tl t;
+        bool keep[Tl::PER];
+        float next_m = 0.0f, next_r = 0.0f, next_g = 0.0f;
+        int32_t next_t = -1;
+        auto fetch = [&](int i, int j) {
+            const int64_t r = (int64_t)(t0 + i) * Tl::BV;
+            t.fetch((const E *)a.x + sm.offset(j), a.ldx, r, a.rows);
 #pragma unroll
-        for (int w = 0; w < CW; ++w) s[w][j] = f.target[r] == w0 + (lane & 31) + 32 * w ? -INFINITY : s[w][j] - f.far[r];
-    }
-    uint32_t hits = (uint32_t)__ballot(hit);  // (the half-waves say the same)
-    while (hits) {
-        const int r = r0 + __ffs(hits) - 1;
-        hits &= hits - 1;
-        const int32_t at = f.target[r] - w0 - (lane & 31);
-        const float g = f.weight[r];
-        const E *x = tile + r * Tile<E, NS, DP>::ROW + 4 * h;
+            for (int k = 0; k < Tl::PER; ++k) {
+                const int64_t n = r + (k * 256 + (int)threadIdx.x) / Tl::CHUNKS;
+                keep[k] = n < a.rows && a.row_target[n] >= 0;
+            }
+            if (j == 0 && threadIdx.x < Tl::BV) {
+                const int64_t n = r + threadIdx.x;
+                const bool ok = n < a.rows;
+                next_m = ok ? a.row_max[n] : INFINITY;
+                next_r = ok ? a.row_rate[n] : 0.0f;
+                next_g = ok ? a.row_weight[n] : 0.0f;
+                next_t = ok ? a.row_target[n] : -1;
+            }
+        };
+        auto store = [&](int i, int j, int buf) {
 #pragma unroll
-        for (int w = 0; w < CW; ++w) {
-            const float mg = at == 32 * w ? g : 0.0f;
-            if (h == 0) db[w] -= mg;
+            for (int k = 0; k < Tl::PER; ++k)  // a row without a target is not read: zeros in its place
+                if (!keep[k]) t.held[k] = make_uint4(0, 0, 0, 0);
+            t.store(tile[buf]);
+            if (j == 0 && threadIdx.x < Tl::BV) {
+                const bool far = fabsf(next_m * dv.c) > FAR && next_m < INFINITY;
+                RowFacts<Tl::BV> &f = facts[i & 1];
+                f.m[threadIdx.x] = far ? 0.0f : -next_m * dv.c;
+                f.far[threadIdx.x] = far ? next_m : 0.0f;
+                f.rate[threadIdx.x] = next_r;
+                f.weight[threadIdx.x] = next_g;
+                f.target[threadIdx.x] = next_t;
+            }
+        };
+        __syncthreads();  // (the owner before is done with the tiles)
+        fetch(0, 0);
+        store(0, 0, 0);
+        __syncthreads();
+        int buf = 0;
+        ScoreOperand<E, NS, DP> so;
+        so.read(tile[0], 0);
+        for (int i = 0; i < nt; ++i) {
+            if (!WIDE && i + 1 < nt) fetch(i + 1, 0);
+            const RowFacts<Tl::BV> &f = facts[i & 1];
+#pragma unroll
+            for (int blk = 0; blk < St::BLOCKS; ++blk) {
+                SumOperand<E, NS, DP> to;
+                f32x16 s = (f32x16)(bias);
+                const int r0 = blk * 32;
+                const int32_t mine = f.target[r0 + (lane & 31)] - w0;
+                const float fars = f.far[r0 + (lane & 31)];
+                if (WIDE) {
+                    for (int j = 0; j < sm.chunks; ++j) {
+                        load_owned<E, NS, DP>(own, (const E *)a.w + sm.offset(j), a.ldw, v, a.vocab, dv.owned);
+                        const bool last = j + 1 == sm.chunks;
+                        if (!last || i + 1 < nt) fetch(last ? i + 1 : i, last ? 0 : j + 1);
+                        scores<E, NS, DP>(s, own, so);
+                        if (last) break;
+                        store(i, j + 1, buf ^ 1);
+                        __syncthreads();
+                        buf ^= 1;
+                        so.read(tile[buf], 0);
+                    }
+                    to.read(tile[buf], 0);
+                } else {
+                    to.read(tile[buf], r0);
+                    READ_AHEAD();
+                    scores<E, NS, DP>(s, own, so);
+                }
+                if (blk + 1 < St::BLOCKS) so.read(tile[buf], 32);
+                else {
+                    if (i + 1 < nt) store(i + 1, 0, buf ^ 1);  // (facts: the other one of the two)
+                    __syncthreads();
+                    so.read(tile[i + 1 < nt ? buf ^ 1 : buf], 0);
+                }
+                READ_AHEAD();
+                // Where a row's target is among the owned table rows q is -g (1 - p), formed from the sum over the other
+                // items: popular items are targets in every block, so this has to be cheap.  A lane collects the rows
+                // whose target is its own table row as bits.
+                uint32_t hits = 0, any = (uint32_t)__ballot((uint32_t)mine < 32u);  // (both half-waves say the same)
+                for (uint32_t rows = any; rows; rows &= rows - 1) {
+                    const int r = __ffs(rows) - 1;
+                    hits |= (lane & 31) == __builtin_amdgcn_readlane(mine, r) ? 1u << r : 0u;
+                }
+                if (__any(fars != 0.0f)) {  // see FAR
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) s[j] -= f.far[r0 + 8 * (j / 4) + 4 * h + j % 4];
+                }
+                float q[16];
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int r = r0 + 8 * g + 4 * h;
+                    const float4 mm = *(const float4 *)&f.m[r], rr = *(const float4 *)&f.rate[r];
+                    const float ms[4] = {mm.x, mm.y, mm.z, mm.w}, rs[4] = {rr.x, rr.y, rr.z, rr.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) q[4 * g + j] = exp2_fast(__builtin_fmaf(s[4 * g + j], dv.c, ms[j])) * rs[j];
+                }
+                if (any) {
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const float4 ww = *(const float4 *)&f.weight[r0 + 8 * g + 4 * h];
+                        const float ws[4] = {ww.x, ww.y, ww.z, ww.w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) q[4 * g + j] = (hits >> (4 * h)) & (1u << (8 * g + j)) ? -ws[j] : q[4 * g + j];
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 16; ++j) db += q[j];
+                Values<E, NS> p;
+                p.pack(q);
+                accumulate<E, NS, DP>(out, p, to);
+            }
+            buf ^= 1;
+        }
+        const float total = half_wave_sum(db);
+        const uint32_t b0 = a.pieces.first_block(owner), b1 = a.pieces.last_block(owner);
+        if (b0 != b1) {  // shared with other blocks: the block's first owner, or its last
+            const int64_t part = 2 * (int64_t)blockIdx.x + (begin > (uint64_t)owner * a.pieces.tiles ? 0 : 1);
+            const int64_t at = part * 128 + (v - (int64_t)owner * 128);
+            if (h == 0 && c0 == 0) a.pb[at] = total;
 #pragma unroll
             for (int b = 0; b < DP / 32; ++b)
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const int c = b * 32 + 8 * (j / 4) + j % 4;
-                    const float xv = NS == 2 ? (float)x[c] + (float)x[(NS - 1) * DP + c] : (float)x[c];
-                    out[w][b][j] = __builtin_fmaf(-mg, xv, out[w][b][j]);
-                }
+                for (int g = 0; g < 4; ++g)
+                    *(float4 *)(a.pw + at * a.dp + c0 + b * 32 + 8 * g + 4 * h) =
+                        make_float4(out[b][4 * g], out[b][4 * g + 1], out[b][4 * g + 2], out[b][4 * g + 3]);
+            continue;
         }
-    }
-}
-
-template <typename T, typename E, int NS, int DP, int CW>
-__global__ __launch_bounds__(256, NS * DP >= 384 ? 1 : LFM_TABLE_WAVES) void table_kernel(SweepArgs a)
-{
-    typedef Tile<E, NS, DP> Tl;
-    typedef Rotation<E, NS, DP> Ro;
-    typedef typename Half<E>::x8 x8;
-    __shared__ __attribute__((aligned(16))) E tile[Ro::BUFS][Tl::SIZE];
-    __shared__ __attribute__((aligned(16))) RowFacts<Tl::BV> facts[Ro::BUFS];
-    const Derived dv = derive(NS == 2 ? a.scales : nullptr);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-    const uint32_t part = blockIdx.x % (uint32_t)a.splits;
-    const int64_t w0 = (int64_t)(blockIdx.x / (uint32_t)a.splits) * (128 * CW) + wave * (32 * CW), v0 = w0 + (lane & 31);
-    const uint32_t tiles = (uint32_t)((a.rows + Tl::BV - 1) / Tl::BV);
-    const uint32_t t0 = (uint32_t)((uint64_t)tiles * part / (uint32_t)a.splits);
-    const int nt = (int)((uint64_t)tiles * (part + 1) / (uint32_t)a.splits) - (int)t0;
-
-    x8 own[CW][NS][DP / 16];
-    f32x16 out[CW][DP / 32], cur[CW], next[CW];
-    Values<E, NS, CW> q;
-    float bias[CW], db[CW];
-#pragma unroll
-    for (int w = 0; w < CW; ++w) {
-        const int64_t v = v0 + 32 * w;
-        load_owned<E, NS, DP>(own[w], (const E *)a.w, a.ldw, v, a.vocab, dv.owned);
-        bias[w] = a.bias && v < a.vocab ? bias_units(a.bias[v], dv) : 0.0f;
-        db[w] = 0.0f;
-#pragma unroll
-        for (int b = 0; b < DP / 32; ++b) out[w][b] = (f32x16)(0.0f);
-    }
-    clear_values(q);
-
-    Tl t;
-    bool keep[Tl::PER];
-    float next_m = 0.0f, next_r = 0.0f, next_g = 0.0f;
-    int32_t next_t = -1;
-    auto fetch = [&](int i) {
-        const int64_t r = (int64_t)(t0 + i) * Tl::BV;
-        t.fetch((const E *)a.x, a.ldx, r, a.rows);
-#pragma unroll
-        for (int k = 0; k < Tl::PER; ++k) {
-            const int64_t n = r + (k * 256 + (int)threadIdx.x) / Tl::CHUNKS;
-            keep[k] = n < a.rows && a.row_target[n] >= 0;
-        }
-        if (threadIdx.x < Tl::BV) {
-            const int64_t n = r + threadIdx.x;
-            const bool ok = n < a.rows;
-            next_m = ok ? a.row_max[n] : INFINITY;
-            next_r = ok ? a.row_rate[n] : 0.0f;
-            next_g = ok ? a.row_weight[n] : 0.0f;
-            next_t = ok ? a.row_target[n] : -1;
-        }
-    };
-    auto store = [&](int buf) {
-#pragma unroll
-        for (int k = 0; k < Tl::PER; ++k)  // a row without a target is not read: zeros in its place
-            if (!keep[k]) t.held[k] = make_uint4(0, 0, 0, 0);
-        t.store(tile[buf]);
-        if (threadIdx.x < Tl::BV) {
-            const bool far = fabsf(next_m * dv.c) > FAR && next_m < INFINITY;
-            RowFacts<Tl::BV> &f = facts[buf];
-            f.m[threadIdx.x] = far ? 0.0f : -next_m * dv.c;
-            f.far[threadIdx.x] = far ? next_m : 0.0f;
-            f.rate[threadIdx.x] = next_r;
-            f.weight[threadIdx.x] = next_g;
-            f.target[threadIdx.x] = next_t;
-        }
-    };
-    auto score = [&](f32x16 (&s)[CW], int buf, int r0) {
-#pragma unroll
-        for (int w = 0; w < CW; ++w) s[w] = (f32x16)(bias[w]);
-        scores<E, NS, DP, CW>(s, own, tile[buf], r0);
-    };
-    auto step = [&](int here, int r0, int before, int before_r, int after, int after_r) {
-        const RowFacts<Tl::BV> &f = facts[here];
-        const bool hit = (uint32_t)(f.target[r0 + (lane & 31)] - (int32_t)w0) < 32u * CW;
-        if (__any(hit || f.far[r0 + (lane & 31)] != 0.0f))  // seldom
-            special_rows<E, NS, DP, CW, Tl::BV>(cur, out, db, f, tile[here], r0, (int32_t)w0, hit);
-        score(next, after, after_r);
-        accumulate<E, NS, DP, CW>(out, q, tile[before], before_r);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            float v8[CW][8];
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                const int r = r0 + k * 16 + 8 * g + 4 * h;
-                const float4 mm = *(const float4 *)&f.m[r], rr = *(const float4 *)&f.rate[r];
-                const float ms[4] = {mm.x, mm.y, mm.z, mm.w}, rs[4] = {rr.x, rr.y, rr.z, rr.w};
-#pragma unroll
-                for (int w = 0; w < CW; ++w)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float v = exp2_fast(__builtin_fmaf(cur[w][8 * k + 4 * g + j], dv.c, ms[j])) * rs[j];
-                        db[w] += v;
-                        v8[w][4 * g + j] = v;
-                    }
-            }
-            pack_values<E, NS, CW>(q, v8, k);
-        }
-        constexpr int MATRIX = 2 * CW * (NS == 2 ? 3 : 1) * (DP / 16), VECTOR = CW * (NS == 2 ? 112 : 88);
-        interleave<MATRIX, (VECTOR + MATRIX - 1) / MATRIX>();
-#pragma unroll
-        for (int w = 0; w < CW; ++w) cur[w] = next[w];
-    };
-
-    if (nt > 0) {
-        fetch(0);
-        store(0);
-        if (Ro::AHEAD == 2 && nt > 1) {
-            fetch(1);
-            store(1);
-        }
-        if (nt > Ro::AHEAD) fetch(Ro::AHEAD);
-        __syncthreads();
-        score(cur, 0, 0);
-    }
-    int b0 = 0, b1 = 1, before = 0;  // the buffers of tile i, i + 1, i - 1
-    for (int i = 0; i < nt; ++i) {
-        int b2 = b1 + 1 == Ro::BUFS ? 0 : b1 + 1;
-        const int into = Ro::BLOCKS == 2 ? b1 : b2;
-        if (i + Ro::AHEAD < nt) store(into);
-        if (i + Ro::AHEAD + 1 < nt) fetch(i + Ro::AHEAD + 1);
-        const int after = i + 1 < nt ? b1 : b0;  // (behind the last block: scores that nobody looks at)
-        if (Ro::BLOCKS == 2) {
-            step(b0, 0, before, i ? 32 : 0, b0, 32);
-            __syncthreads();
-            step(b0, 32, b0, 0, after, 0);
-        } else {
-            step(b0, 0, before, 0, after, 0);
-            __syncthreads();
-        }
-        before = b0;
-        b0 = b1;
-        b1 = b2;
-    }
-    if (nt > 0) accumulate<E, NS, DP, CW>(out, q, tile[before], Tl::BV - 32);
-    write_table<T, NS, DP, CW>(a, out, db, v0, part, 0);
-}
-
-// More than 256 columns, taken 256 at a time.  The scores add up over the chunks (the owned operand is read again for each,
-// from the caches); a block accumulates the second product of one chunk, blockIdx.y's, which it streams last.  The work of
-// the scores is repeated for every chunk of the result: a width that is rare is not worth a second shape of block.
-template <typename E, int NS, bool GRAD>
-__global__ __launch_bounds__(256, 1) void wide_rows_kernel(SweepArgs a)
-{
-    constexpr int DP = 256;
-    typedef Tile<E, NS, DP> Tl;
-    typedef typename Half<E>::x8 x8;
-    static_assert(Tl::BV == 32, "one block of scores per tile");
-    __shared__ __attribute__((aligned(16))) E tile[2][Tl::SIZE];
-    __shared__ __attribute__((aligned(16))) float sb[2][32];
-    const Derived dv = derive(NS == 2 ? a.scales : nullptr);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-    const int part = blockIdx.x % a.splits;
-    const int64_t n = (int64_t)(blockIdx.x / a.splits) * 128 + wave * 32 + (lane & 31);
-    const int64_t tiles = ceil_div(a.vocab, 32), t0 = tiles * part / a.splits, t1 = tiles * (part + 1) / a.splits;
-    const int chunks = a.chunks, first = (int)blockIdx.y + 1;
-    auto offset = [&](int j) { return ((first + j) % chunks) * (NS * DP); };  // of the j-th chunk; the last is blockIdx.y's
-    f32x16 out[1][DP / 32];
-    Values<E, NS, 1> p;
-    float m = dv.low * 1.01f, l = 0.0f;
-#pragma unroll
-    for (int b = 0; b < DP / 32; ++b) out[0][b] = (f32x16)(0.0f);
-    const int64_t at = n >= a.rows ? -1 : a.id_bytes == 8 ? ((const int64_t *)a.targets)[n] : (int64_t)((const int32_t *)a.targets)[n];
-    const int64_t target = (uint64_t)at < (uint64_t)a.vocab ? at - 4 * h : -1000;
-    Tl t;
-    float next_bias = 0.0f;
-    auto fetch = [&](int64_t i, int j) {
-        t.fetch((const E *)a.w + offset(j), a.ldw, i * 32, a.vocab);
-        const int64_t v = i * 32 + threadIdx.x;
-        if (j == 0 && threadIdx.x < 32) next_bias = v >= a.vocab ? -INFINITY : a.bias ? bias_units(a.bias[v], dv) : 0.0f;
-    };
-    auto store = [&](int64_t i, int j, int buf) {
-        t.store(tile[buf]);
-        if (j == 0 && threadIdx.x < 32) sb[(i - t0) & 1][threadIdx.x] = next_bias;
-    };
-    if (t0 < t1) {
-        fetch(t0, 0);
-        store(t0, 0, 0);
-    }
-    __syncthreads();
-    int buf = 0;
-    for (int64_t i = t0; i < t1; ++i) {
-        f32x16 s[1];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) s[0][j] = sb[(i - t0) & 1][8 * (j / 4) + 4 * h + j % 4];
-        for (int j = 0; j < chunks; ++j) {
-            x8 own[1][NS][DP / 16];
-            load_owned<E, NS, DP>(own[0], (const E *)a.x + offset(j), a.ldx, n, a.rows, dv.owned);
-            const bool more = j + 1 < chunks || i + 1 < t1;
-            if (more) fetch(j + 1 < chunks ? i : i + 1, j + 1 < chunks ? j + 1 : 0);
-            scores<E, NS, DP, 1>(s, own, tile[buf], 0);
-            if (j + 1 < chunks) {
-                store(i, j + 1, buf ^ 1);
-                __syncthreads();
-                buf ^= 1;
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < 16; ++j) s[0][j] = target - i * 32 == 8 * (j / 4) + j % 4 ? -INFINITY : s[0][j];
-        float mx = s[0][0];
-#pragma unroll
-        for (int j = 1; j < 16; ++j) mx = fmaxf(mx, s[0][j]);
-        mx = half_wave_max(mx);
-        if (__any((mx - m) * dv.c > LAG)) {
-            const float up = (mx - m) * dv.c > LAG ? mx : m, f = exp2_fast((m - up) * dv.c);
-            m = up;
-            l *= f;
-            if (GRAD)
-#pragma unroll
-                for (int b = 0; b < DP / 32; ++b) out[0][b] *= f;
-        }
-        const bool far = fabsf(m * dv.c) > FAR;
-        const float base = far ? P_SHIFT : P_SHIFT - m * dv.c, less = far ? m : 0.0f;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            float v8[1][8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                v8[0][j] = exp2_fast(__builtin_fmaf(s[0][8 * k + j] - less, dv.c, base));
-                l += v8[0][j];
-            }
-            if (GRAD) pack_values<E, NS, 1>(p, v8, k);
-        }
-        if (GRAD) accumulate<E, NS, DP, 1>(out, p, tile[buf], 0);
-        if (i + 1 < t1) store(i + 1, 0, buf ^ 1);
-        __syncthreads();
-        buf ^= 1;
-    }
-    const float sum = half_wave_sum(l);
-    if (n >= a.rows) return;
-    const int64_t to = (int64_t)part * a.rows + n;
-    if (h == 0) {
-        a.pm[to + (int64_t)blockIdx.y * a.splits * a.rows] = m;
-        a.pl[to + (int64_t)blockIdx.y * a.splits * a.rows] = sum;
-    }
-    if (GRAD)
+        if (v >= a.vocab) continue;
+        if (a.db && h == 0 && c0 == 0) a.db[v] = ldexpf(total, shift);
+        T *row = (T *)a.dw + v * a.d;
 #pragma unroll
         for (int b = 0; b < DP / 32; ++b)
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
-                *(float4 *)(a.po + to * a.dp + (int)blockIdx.y * DP + b * 32 + 8 * g + 4 * h) =
-                    make_float4(out[0][b][4 * g], out[0][b][4 * g + 1], out[0][b][4 * g + 2], out[0][b][4 * g + 3]);
-}
-
-template <typename T, typename E, int NS>
-__global__ __launch_bounds__(256, 1) void wide_table_kernel(SweepArgs a)
-{
-    constexpr int DP = 256;
-    typedef Tile<E, NS, DP> Tl;
-    typedef typename Half<E>::x8 x8;
-    static_assert(Tl::BV == 32, "one block of scores per tile");
-    __shared__ __attribute__((aligned(16))) E tile[2][Tl::SIZE];
-    __shared__ __attribute__((aligned(16))) RowFacts<32> facts[2];
-    const Derived dv = derive(NS == 2 ? a.scales : nullptr);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-    const int part = blockIdx.x % a.splits;
-    const int64_t w0 = (int64_t)(blockIdx.x / a.splits) * 128 + wave * 32, v = w0 + (lane & 31);
-    const int64_t tiles = ceil_div(a.rows, 32), t0 = tiles * part / a.splits, t1 = tiles * (part + 1) / a.splits;
-    const int chunks = a.chunks, first = (int)blockIdx.y + 1;
-    auto offset = [&](int j) { return ((first + j) % chunks) * (NS * DP); };
-    f32x16 out[1][DP / 32];
-    Values<E, NS, 1> q;
-    const float bias = a.bias && v < a.vocab ? bias_units(a.bias[v], dv) : 0.0f;
-    float db[1] = {0.0f};
+            for (int g = 0; g < 4; ++g) {
+                const int c = c0 + b * 32 + 8 * g + 4 * h;
+                Vec<T, 4> o;
 #pragma unroll
-    for (int b = 0; b < DP / 32; ++b) out[0][b] = (f32x16)(0.0f);
-    Tl t;
-    bool keep[Tl::PER];
-    float next_m = 0.0f, next_r = 0.0f, next_g = 0.0f;
-    int32_t next_t = -1;
-    auto fetch = [&](int64_t i, int j) {
-        t.fetch((const E *)a.x + offset(j), a.ldx, i * 32, a.rows);
+                for (int j = 0; j < 4; ++j) o.v[j] = (T)ldexpf(out[b][4 * g + j], shift - kx);
+                if (c + 4 <= a.d && (a.d & 3) == 0) *(Vec<T, 4> *)(row + c) = o;
+                else
 #pragma unroll
-        for (int k = 0; k < Tl::PER; ++k) {
-            const int64_t n = i * 32 + (k * 256 + (int)threadIdx.x) / Tl::CHUNKS;
-            keep[k] = n < a.rows && a.row_target[n] >= 0;
-        }
-        if (j == 0 && threadIdx.x < 32) {
-            const int64_t n = i * 32 + threadIdx.x;
-            const bool ok = n < a.rows;
-            next_m = ok ? a.row_max[n] : INFINITY;
-            next_r = ok ? a.row_rate[n] : 0.0f;
-            next_g = ok ? a.row_weight[n] : 0.0f;
-            next_t = ok ? a.row_target[n] : -1;
-        }
-    };
-    auto store = [&](int64_t i, int j, int buf) {
-#pragma unroll
-        for (int k = 0; k < Tl::PER; ++k)
-            if (!keep[k]) t.held[k] = make_uint4(0, 0, 0, 0);
-        t.store(tile[buf]);
-        if (j == 0 && threadIdx.x < 32) {
-            const bool far = fabsf(next_m * dv.c) > FAR && next_m < INFINITY;
-            RowFacts<32> &f = facts[(i - t0) & 1];
-            f.m[threadIdx.x] = far ? 0.0f : -next_m * dv.c;
-            f.far[threadIdx.x] = far ? next_m : 0.0f;
-            f.rate[threadIdx.x] = next_r;
-            f.weight[threadIdx.x] = next_g;
-            f.target[threadIdx.x] = next_t;
-        }
-    };
-    if (t0 < t1) {
-        fetch(t0, 0);
-        store(t0, 0, 0);
-    }
-    __syncthreads();
-    int buf = 0;
-    for (int64_t i = t0; i < t1; ++i) {
-        const RowFacts<32> &f = facts[(i - t0) & 1];
-        f32x16 s[1] = {(f32x16)(bias)};
-        for (int j = 0; j < chunks; ++j) {
-            x8 own[1][NS][DP / 16];
-            load_owned<E, NS, DP>(own[0], (const E *)a.w + offset(j), a.ldw, v, a.vocab, dv.owned);
-            const bool more = j + 1 < chunks || i + 1 < t1;
-            if (more) fetch(j + 1 < chunks ? i : i + 1, j + 1 < chunks ? j + 1 : 0);
-            scores<E, NS, DP, 1>(s, own, tile[buf], 0);
-            if (j + 1 < chunks) {
-                store(i, j + 1, buf ^ 1);
-                __syncthreads();
-                buf ^= 1;
+                    for (int j = 0; j < 4; ++j)
+                        if (c + j < a.d) row[c + j] = o.v[j];
             }
-        }
-        const bool hit = (uint32_t)(f.target[lane & 31] - (int32_t)w0) < 32u;
-        if (__any(hit || f.far[lane & 31] != 0.0f))
-            special_rows<E, NS, DP, 1, 32>(s, out, db, f, tile[buf], 0, (int32_t)w0, hit);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            float v8[1][8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int r = k * 16 + 8 * (j / 4) + 4 * h + j % 4;
-                v8[0][j] = exp2_fast(__builtin_fmaf(s[0][8 * k + j], dv.c, f.m[r])) * f.rate[r];
-                db[0] += v8[0][j];
-            }
-            pack_values<E, NS, 1>(q, v8, k);
-        }
-        accumulate<E, NS, DP, 1>(out, q, tile[buf], 0);
-        if (i + 1 < t1) store(i + 1, 0, buf ^ 1);
-        __syncthreads();
-        buf ^= 1;
     }
-    write_table<T, NS, DP, 1>(a, out, db, v, part, (int)blockIdx.y * DP);
 }
 
 // ------------------------------------------------------------------- joins ---
@@ -1057,7 +788,8 @@ struct JoinArgs {
     lfm_softmax_args a;
     const Scales *scales;
     const uint8_t *outlier;
-    int splits, dp, ns, grad, shifted;
+    Pieces pieces;
+    int parts, dp, ns, grad, shifted;
     const float *pm, *pl, *po;
     float *row_max, *row_rate, *row_weight;
     int32_t *row_target;
@@ -1092,11 +824,13 @@ __global__ __launch_bounds__(256) void join_rows_kernel(JoinArgs j)
     if (n >= a.rows) return;
     const int lane = threadIdx.x & 63;
     const Derived dv = derive(j.ns == 2 ? j.scales : nullptr);
+    const uint32_t owner = (uint32_t)(n / 128);
+    const int splits = (int)(j.pieces.last_block(owner) - j.pieces.first_block(owner)) + 1;
     float m = -INFINITY;
-    for (int s = lane; s < j.splits; s += 64) m = fmaxf(m, j.pm[(int64_t)s * a.rows + n]);
+    for (int s = lane; s < splits; s += 64) m = fmaxf(m, j.pm[(int64_t)s * a.rows + n]);
     m = wave_max(m);
     float l = 0.0f;
-    for (int s = lane; s < j.splits; s += 64)
+    for (int s = lane; s < splits; s += 64)
         l += j.pl[(int64_t)s * a.rows + n] * exp2_fast((j.pm[(int64_t)s * a.rows + n] - m) * dv.c);
     l = wave_sum(l);
     const T *x = (const T *)a.hidden + n * a.hidden_stride;
@@ -1159,8 +893,8 @@ __global__ __launch_bounds__(256) void join_rows_kernel(JoinArgs j)
     for (int c = lane; c < a.d; c += 64) {
         float o = 0.0f;
         if (t >= 0) {
-            const float *pm = j.pm + (int64_t)(c >> 8) * j.splits * a.rows;  // the maxima that chunk c / 256 went by
-            for (int s = 0; s < j.splits; ++s) {
+            const float *pm = j.pm + (int64_t)(c >> 8) * j.parts * a.rows;  // the maxima that chunk c / 256 went by
+            for (int s = 0; s < splits; ++s) {
                 const int64_t at = (int64_t)s * a.rows + n;
                 o += j.po[at * j.dp + c] * exp2_fast((pm[at] - m) * dv.c);
             }
@@ -1171,22 +905,25 @@ __global__ __launch_bounds__(256) void join_rows_kernel(JoinArgs j)
     }
 }
 
-// dw and db from the parts of the rows, added in order
+// dw and db of the table rows that several blocks share, added in the order of the blocks
 template <typename T>
-__global__ __launch_bounds__(256) void join_table_kernel(SweepArgs a, int dp, int ns)
+__global__ __launch_bounds__(256) void join_table_kernel(SweepArgs a, int ns)
 {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, v = i / a.d;
     if (v >= a.vocab) return;
+    const uint32_t owner = (uint32_t)(v / 128), b0 = a.pieces.first_block(owner), b1 = a.pieces.last_block(owner);
+    if (b0 == b1) return;
     const int c = (int)(i - v * a.d);
     const int shift = a.shifted == 2 ? a.scales->eg - 14 : a.shifted ? -14 : 0, kx = ns == 2 ? a.scales->kx : 0;
-    float s = 0.0f;
-    for (int p = 0; p < a.splits; ++p) s += a.pw[((int64_t)p * a.vocab + v) * dp + c];
-    ((T *)a.dw)[i] = (T)ldexpf(s, shift - kx);
-    if (c == 0 && a.db) {
-        float b = 0.0f;
-        for (int p = 0; p < a.splits; ++p) b += a.pb[(int64_t)p * a.vocab + v];
-        a.db[v] = ldexpf(b, shift);
+    float s = 0.0f, t = 0.0f;
+    for (uint32_t b = b0; b <= b1; ++b) {
+        const int64_t part = 2 * (int64_t)b + (a.pieces.begin(b) > (uint64_t)owner * a.pieces.tiles ? 0 : 1);
+        const int64_t at = part * 128 + (v - (int64_t)owner * 128);
+        s += a.pw[at * a.dp + c];
+        if (c == 0) t += a.pb[at];
     }
+    ((T *)a.dw)[i] = (T)ldexpf(s, shift - kx);
+    if (c == 0 && a.db) a.db[v] = ldexpf(t, shift);
 }
 
 template <typename T>
@@ -1200,11 +937,9 @@ __global__ __launch_bounds__(256) void clear_kernel(T *p, int64_t n, float *q, i
 // -------------------------------------------------------------------- host ---
 
 struct Plan {
-    int dp, ns, cw;
+    int dp, ns;
     int chunks;             // of 256 columns
-    int bv;                 // rows of a streamed tile
-    int row_splits, table_splits;
-    bool largest;           // scales are wanted (float32 operands; float16 with weights)
+    Pieces rows, table;
 };
 
 int width_for(int d)
@@ -1215,27 +950,26 @@ int width_for(int d)
     return (d + 255) / 256 * 256;
 }
 
-int splits_for(int64_t owners, int64_t tiles, int64_t slots)
+Pieces pieces_for(int64_t owned, int64_t streamed, int bv, int64_t slots)
 {
-    int64_t s = slots / owners;
-    if (s < 1) s = 1;
-    if (s > 8) s = s / 8 * 8;  // a part of the streamed side then stays with one XCD's L2
-    if (s > tiles) s = tiles;
-    if (s < 1) s = 1;
-    return (int)s;
+    Pieces p;
+    p.owners = (uint32_t)ceil_div(owned < 1 ? 1 : owned, 128);
+    p.tiles = (uint32_t)ceil_div(streamed < 1 ? 1 : streamed, bv);
+    const uint64_t units = (uint64_t)p.owners * p.tiles;
+    p.blocks = (uint32_t)(units < (uint64_t)slots ? units : (uint64_t)slots);
+    return p;
 }
 
-Plan plan_for(int64_t rows, int64_t vocab, int d, int dtype, bool weights)
+Plan plan_for(int64_t rows, int64_t vocab, int d, int dtype, bool grad)
 {
     Plan p;
     p.dp = width_for(d);
     p.ns = dtype == LFM_F32 ? 2 : 1;
-    p.cw = 1;
     p.chunks = p.dp > 256 ? p.dp / 256 : 1;
-    p.bv = p.ns * p.dp <= 128 ? 64 : 32;
-    p.largest = dtype == LFM_F32 || (dtype == LFM_F16 && weights);
-    p.row_splits = splits_for(ceil_div(rows < 1 ? 1 : rows, 128 * p.cw), ceil_div(vocab, p.bv), 512);
-    p.table_splits = splits_for(ceil_div(vocab, 128 * p.cw), ceil_div(rows < 1 ? 1 : rows, p.bv), 512);
+    const int w = p.dp > 256 ? 256 : p.dp, bv = p.ns * w <= 128 ? 64 : 32;
+    // as many blocks as run at once on the card's 256 compute units
+    p.rows = pieces_for(rows, vocab, bv, 256 * (p.chunks > 1 ? 1 : waves_for(p.ns, w, grad)));
+    p.table = pieces_for(vocab, rows, bv, 256 * (p.chunks > 1 ? 1 : waves_for(p.ns, w, true)));
     return p;
 }
 
@@ -1260,11 +994,12 @@ Space space_for(const Plan &p, int64_t rows, int64_t vocab, bool grad, void *ws)
     s.outlier = c.take<uint8_t>(rows);
     s.x = c.take<uint16_t>(rows * p.ns * p.dp);
     s.w = c.take<uint16_t>(vocab * p.ns * p.dp);
-    s.pm = c.take<float>(rows * p.row_splits * p.chunks);
-    s.pl = c.take<float>(rows * p.row_splits * p.chunks);
-    s.po = c.take<float>(grad ? rows * p.row_splits * p.dp : 0);
-    s.pw = c.take<float>(grad && p.table_splits > 1 ? vocab * p.table_splits * p.dp : 0);
-    s.pb = c.take<float>(grad && p.table_splits > 1 ? vocab * p.table_splits : 0);
+    const int64_t parts = rows * p.rows.most(), shared = (int64_t)p.table.blocks * 2 * 128;
+    s.pm = c.take<float>(parts * p.chunks);
+    s.pl = c.take<float>(parts * p.chunks);
+    s.po = c.take<float>(grad ? parts * p.dp : 0);
+    s.pw = c.take<float>(grad ? shared * p.dp : 0);
+    s.pb = c.take<float>(grad ? shared : 0);
     s.row_max = c.take<float>(grad ? rows : 0);
     s.row_rate = c.take<float>(grad ? rows : 0);
     s.row_weight = c.take<float>(grad ? rows : 0);
@@ -1276,23 +1011,16 @@ Space space_for(const Plan &p, int64_t rows, int64_t vocab, bool grad, void *ws)
 template <typename E, int NS, int DP, bool WIDE>
 hipError_t sweep_rows(const SweepArgs &s, bool grad, hipStream_t st)
 {
-    const unsigned blocks = (unsigned)(ceil_div(s.rows, 128) * s.splits);
-    if constexpr (WIDE) {
-        if (grad) wide_rows_kernel<E, NS, true><<<dim3(blocks, (unsigned)s.chunks), 256, 0, st>>>(s);
-        else wide_rows_kernel<E, NS, false><<<dim3(blocks), 256, 0, st>>>(s);  // without the gradient one chunk's sweep does
-    } else {
-        if (grad) rows_kernel<E, NS, DP, 1, true><<<dim3(blocks), 256, 0, st>>>(s);
-        else rows_kernel<E, NS, DP, 1, false><<<dim3(blocks), 256, 0, st>>>(s);
-    }
+    // without the gradient one chunk's sweep does
+    if (grad) rows_kernel<E, NS, DP, true, WIDE><<<dim3(s.pieces.blocks, (unsigned)s.chunks), 256, 0, st>>>(s);
+    else rows_kernel<E, NS, DP, false, WIDE><<<dim3(s.pieces.blocks), 256, 0, st>>>(s);
     return hipGetLastError();
 }
 
 template <typename T, typename E, int NS, int DP, bool WIDE>
 hipError_t sweep_table(const SweepArgs &s, hipStream_t st)
 {
-    const unsigned blocks = (unsigned)(ceil_div(s.vocab, 128) * s.splits);
-    if constexpr (WIDE) wide_table_kernel<T, E, NS><<<dim3(blocks, (unsigned)s.chunks), 256, 0, st>>>(s);
-    else table_kernel<T, E, NS, DP, 1><<<dim3(blocks), 256, 0, st>>>(s);
+    table_kernel<T, E, NS, DP, WIDE><<<dim3(s.pieces.blocks, (unsigned)s.chunks), 256, 0, st>>>(s);
     return hipGetLastError();
 }
 
@@ -1310,7 +1038,7 @@ hipError_t sweep_table(const SweepArgs &s, hipStream_t st)
 template <typename T, typename E, int NS>
 hipError_t run(const lfm_softmax_args &a, bool grad, void *ws, hipStream_t st)
 {
-    const Plan p = plan_for(a.rows, a.vocab, a.d, a.dtype, a.weights != nullptr);
+    const Plan p = plan_for(a.rows, a.vocab, a.d, a.dtype, grad);
     const Space s = space_for(p, a.rows, a.vocab, grad, ws);
     hipError_t e;
     if (a.rows == 0) {
@@ -1318,7 +1046,8 @@ hipError_t run(const lfm_softmax_args &a, bool grad, void *ws, hipStream_t st)
         clear_kernel<T><<<dim3((unsigned)ceil_div(a.vocab * a.d, 256)), 256, 0, st>>>((T *)a.d_table, a.vocab * a.d, a.d_bias, a.vocab);
         return hipGetLastError();
     }
-    const bool scales = p.largest && (grad || NS == 2);
+    // scales are wanted for float32 operands, and of the weights for float16 gradients
+    const bool scales = NS == 2 || (a.dtype == LFM_F16 && a.weights && grad);
     auto in_place = [&](const void *q, int64_t stride) { return NS == 1 && a.d == p.dp && stride % 8 == 0 && ((uintptr_t)q & 15) == 0; };
     const bool x_there = in_place(a.hidden, a.hidden_stride), w_there = in_place(a.table, a.table_stride);
     PackArgs pk;
@@ -1357,7 +1086,8 @@ hipError_t run(const lfm_softmax_args &a, bool grad, void *ws, hipStream_t st)
     w.targets = a.targets;
     w.id_bytes = a.id_bytes;
     w.scales = s.scales;
-    w.splits = p.row_splits;
+    w.pieces = p.rows;
+    w.parts = (int)p.rows.most();
     w.d = a.d;
     w.dp = p.dp;
     w.chunks = p.chunks;
@@ -1380,7 +1110,8 @@ hipError_t run(const lfm_softmax_args &a, bool grad, void *ws, hipStream_t st)
     j.a = a;
     j.scales = s.scales;
     j.outlier = s.outlier;
-    j.splits = p.row_splits;
+    j.pieces = p.rows;
+    j.parts = w.parts;
     j.dp = p.dp;
     j.ns = NS;
     j.grad = grad ? 1 : 0;
@@ -1394,11 +1125,11 @@ hipError_t run(const lfm_softmax_args &a, bool grad, void *ws, hipStream_t st)
     j.row_target = s.row_target;
     join_rows_kernel<T><<<dim3((unsigned)ceil_div(a.rows, 4)), 256, 0, st>>>(j);
     if ((e = hipGetLastError()) != hipSuccess || !grad) return e;
-    w.splits = p.table_splits;
+    w.pieces = p.table;
 #define TABLE(DP, WIDE) sweep_table<T, E, NS, DP, WIDE>(w, st)
     BY_WIDTH(p.dp, TABLE)
-    if (e != hipSuccess || p.table_splits == 1) return e;
-    join_table_kernel<T><<<dim3((unsigned)ceil_div(a.vocab * a.d, 256)), 256, 0, st>>>(w, p.dp, NS);
+    if (e != hipSuccess || p.table.owners % p.table.blocks == 0) return e;  // (no block shares an owner)
+    join_table_kernel<T><<<dim3((unsigned)ceil_div(a.vocab * a.d, 256)), 256, 0, st>>>(w, NS);
     return hipGetLastError();
 }
 
@@ -1406,7 +1137,7 @@ hipError_t run(const lfm_softmax_args &a, bool grad, void *ws, hipStream_t st)
 
 int64_t softmax_workspace(int64_t rows, int64_t vocab, int d, int dtype, bool grad)
 {
-    return space_for(plan_for(rows, vocab, d, dtype, true), rows, vocab, grad, nullptr).bytes;
+    return space_for(plan_for(rows, vocab, d, dtype, grad), rows, vocab, grad, nullptr).bytes;
 }
 
 hipError_t softmax_loss(const lfm_softmax_args &a, bool grad, void *ws, hipStream_t st)
