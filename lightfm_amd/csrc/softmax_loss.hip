@@ -220,32 +220,41 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs p, int dp, int width
 
 // ------------------------------------------------------------- the sweeps ---
 
-// Streams `rows` rows of NS DP halves into LDS, BV at a time, double-buffered through registers: the loads of the next
-// tile are in flight while this one is used.  A row takes NS DP + 16 halves of LDS: neighbouring rows then start 8 banks
-// apart (modulo 64, in some order), which serves the 16-byte reads of 8 rows and the transposing reads of 4 x 32 bytes
-// without conflicts.
+// Streams rows of NS DP halves into LDS, BV at a time, double-buffered through registers: the loads of the next tile are in
+// flight while this one is used.
+// LDS has 64 banks and serves the 16-byte reads of 16 lanes, or the 8-byte reads of 32, at once.  The products read a tile
+// in two ways: 16 bytes of 16 neighbouring rows, and (transposing) 64 bytes of 4 neighbouring rows.  Both are free of
+// conflicts when a row takes NS DP + 8 halves (4 banks more than a multiple of 64, times an odd number) and the rows of a
+// group of 16 are stored transposed as a 4 x 4 square: neighbours then lie 16 banks apart, and all 16 rows 4 banks apart.
+__host__ __device__ constexpr int slot_of(int r) { return (r & ~15) | ((r & 3) << 2) | ((r >> 2) & 3); }
+
 template <typename E, int NS, int DP>
 struct Tile {
-    static constexpr int BV = NS * DP <= 128 ? 64 : 32, ROW = NS * DP + 16, CHUNKS = NS * DP / 8, PER = BV * CHUNKS / 256;
+    static constexpr int BV = NS * DP <= 128 ? 64 : 32, ROW = NS * DP + 8, CHUNKS = NS * DP / 8, PER = BV * CHUNKS / 256;
     static constexpr int SIZE = BV * ROW;
     uint4 held[PER];
 
+    __device__ static inline int row_of(int q) { return (q * 256 + (int)threadIdx.x) / CHUNKS; }
+    // the tile's first row is row0 < rows; rows behind the last are zeros
     __device__ inline void fetch(const E *p, int64_t ld, int64_t row0, int64_t rows)
     {
+        const E *base = p + row0 * ld;  // the same for all lanes
+        const uint32_t ld32 = (uint32_t)ld;
+        if (row0 + BV <= rows) {
 #pragma unroll
-        for (int q = 0; q < PER; ++q) {
-            const int i = q * 256 + threadIdx.x, r = i / CHUNKS, c = i % CHUNKS;
-            held[q] = make_uint4(0, 0, 0, 0);
-            if (row0 + r < rows) held[q] = *(const uint4 *)(p + (row0 + r) * ld + c * 8);
+            for (int q = 0; q < PER; ++q) held[q] = *(const uint4 *)(base + ((uint32_t)row_of(q) * ld32 + (uint32_t)((q * 256 + threadIdx.x) % CHUNKS) * 8u));
+        } else {
+#pragma unroll
+            for (int q = 0; q < PER; ++q) {
+                held[q] = make_uint4(0, 0, 0, 0);
+                if (row0 + row_of(q) < rows) held[q] = *(const uint4 *)(base + ((uint32_t)row_of(q) * ld32 + (uint32_t)((q * 256 + threadIdx.x) % CHUNKS) * 8u));
+            }
         }
     }
     __device__ inline void store(E *tile) const
     {
 #pragma unroll
-        for (int q = 0; q < PER; ++q) {
-            const int i = q * 256 + threadIdx.x, r = i / CHUNKS, c = i % CHUNKS;
-            *(uint4 *)(tile + r * ROW + c * 8) = held[q];
-        }
+        for (int q = 0; q < PER; ++q) *(uint4 *)(tile + slot_of(row_of(q)) * ROW + (q * 256 + (int)threadIdx.x) % CHUNKS * 8) = held[q];
     }
 };
 
@@ -267,8 +276,7 @@ __device__ inline void load_owned(typename Half<E>::x8 (&f)[NS][DP / 16], const 
     }
 }
 
-// The two shapes in which a block of 32 streamed rows (from row r0 of the tile) enters the products.  They are read ahead of
-// the instructions that use them: the reads of one are in flight while the other's products or the exponentials run.
+// The two shapes in which a block of 32 streamed rows (from row r0 of the tile) enters the products.
 template <typename E, int NS, int DP>
 struct ScoreOperand {  // rows of the block: lane = row, 8 columns at a time
     typename Half<E>::x8 v[NS][DP / 16];
@@ -276,7 +284,7 @@ struct ScoreOperand {  // rows of the block: lane = row, 8 columns at a time
     __device__ inline void read(const E *tile, int r0)
     {
         const int lane = threadIdx.x & 63;
-        const E *p = tile + (r0 + (lane & 31)) * Tile<E, NS, DP>::ROW + (lane >> 5) * 8;
+        const E *p = tile + (r0 + slot_of(lane & 31)) * Tile<E, NS, DP>::ROW + (lane >> 5) * 8;
 #pragma unroll
         for (int s = 0; s < NS; ++s)
 #pragma unroll
@@ -293,14 +301,15 @@ struct SumOperand {  // columns of the block: lane = column, the rows in the ord
         typedef typename Half<E>::x4 x4;
         constexpr int ROW = Tile<E, NS, DP>::ROW;
         const int lane = threadIdx.x & 63;
-        const E *p = tile + (r0 + 4 * (lane >> 5) + ((lane & 15) >> 2)) * ROW + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+        // rows 8 e + 4 (lane / 32) + 0 .. 3 of a group of 16, e = 0, 1
+        const E *p = tile + (r0 + (lane >> 5) + ((lane & 15) >> 2) * 4) * ROW + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
 #pragma unroll
         for (int s = 0; s < NS; ++s)
 #pragma unroll
             for (int k = 0; k < 2; ++k)
 #pragma unroll
                 for (int b = 0; b < DP / 32; ++b) {
-                    const x4 lo = read_column(p + s * DP + k * 16 * ROW + b * 32), hi = read_column(p + s * DP + (k * 16 + 8) * ROW + b * 32);
+                    const x4 lo = read_column(p + s * DP + k * 16 * ROW + b * 32), hi = read_column(p + s * DP + (k * 16 + 2) * ROW + b * 32);
                     v[s][k][b] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
                 }
     }
@@ -441,11 +450,6 @@ constexpr int waves_for(int ns, int dp, bool sums) { return ns * dp > (sums ? 19
 #else
 constexpr int waves_for(int ns, int dp, bool sums) { return W1; }
 #endif
-#ifdef RA
-#define READ_AHEAD() __builtin_amdgcn_sched_barrier(0)
-#else
-#define READ_AHEAD()
-#endif
 
 
 template <typename E, int NS, int DP, bool GRAD, bool WIDE>
@@ -493,12 +497,11 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, GRAD)) void rows_
         store(0, 0, 0);
         __syncthreads();
         int buf = 0;
-        ScoreOperand<E, NS, DP> so;
-        so.read(tile[0], 0);
         for (int i = 0; i < nt; ++i) {
             if (!WIDE && i + 1 < nt) fetch(i + 1, 0);
 #pragma unroll
             for (int blk = 0; blk < St::BLOCKS; ++blk) {
+                ScoreOperand<E, NS, DP> so;
                 SumOperand<E, NS, DP> to;
                 f32x16 s;
 #pragma unroll
@@ -514,27 +517,19 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, GRAD)) void rows_
                         load_owned<E, NS, DP>(own, (const E *)a.x + sm.offset(j), a.ldx, n, a.rows, dv.owned);
                         const bool last = j + 1 == sm.chunks;
                         if (!last || i + 1 < nt) fetch(last ? i + 1 : i, last ? 0 : j + 1);
+                        so.read(tile[buf], 0);
                         scores<E, NS, DP>(s, own, so);
                         if (last) break;
                         store(i, j + 1, buf ^ 1);
                         __syncthreads();
                         buf ^= 1;
-                        so.read(tile[buf], 0);
                     }
                     if (GRAD) to.read(tile[buf], 0);
                 } else {
-                    if (GRAD) to.read(tile[buf], blk * 32);
-                    READ_AHEAD();
+                    so.read(tile[buf], blk * 32);
                     scores<E, NS, DP>(s, own, so);
+                    if (GRAD) to.read(tile[buf], blk * 32);
                 }
-                // what comes next is on its way while this block's exponentials run
-                if (blk + 1 < St::BLOCKS) so.read(tile[buf], 32);
-                else {
-                    if (i + 1 < nt) store(i + 1, 0, buf ^ 1);
-                    __syncthreads();
-                    so.read(tile[i + 1 < nt ? buf ^ 1 : buf], 0);
-                }
-                READ_AHEAD();
                 // the target's own score is left to the join, in float32: what remains is not a difference of near-equals
                 const uint32_t hit = target - ((t0 + i) * (uint32_t)Tl::BV + blk * 32u);
                 if (__any(hit < 32u)) {  // one block in some
@@ -572,6 +567,8 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, GRAD)) void rows_
                     accumulate<E, NS, DP>(out, p, to);
                 }
             }
+            if (i + 1 < nt) store(i + 1, 0, buf ^ 1);
+            __syncthreads();
             buf ^= 1;
         }
         const float sum = half_wave_sum(l);
@@ -673,13 +670,12 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, true)) void table
         store(0, 0, 0);
         __syncthreads();
         int buf = 0;
-        ScoreOperand<E, NS, DP> so;
-        so.read(tile[0], 0);
         for (int i = 0; i < nt; ++i) {
             if (!WIDE && i + 1 < nt) fetch(i + 1, 0);
             const RowFacts<Tl::BV> &f = facts[i & 1];
 #pragma unroll
             for (int blk = 0; blk < St::BLOCKS; ++blk) {
+                ScoreOperand<E, NS, DP> so;
                 SumOperand<E, NS, DP> to;
                 f32x16 s = (f32x16)(bias);
                 const int r0 = blk * 32;
@@ -690,26 +686,19 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, true)) void table
                         load_owned<E, NS, DP>(own, (const E *)a.w + sm.offset(j), a.ldw, v, a.vocab, dv.owned);
                         const bool last = j + 1 == sm.chunks;
                         if (!last || i + 1 < nt) fetch(last ? i + 1 : i, last ? 0 : j + 1);
+                        so.read(tile[buf], 0);
                         scores<E, NS, DP>(s, own, so);
                         if (last) break;
                         store(i, j + 1, buf ^ 1);
                         __syncthreads();
                         buf ^= 1;
-                        so.read(tile[buf], 0);
                     }
                     to.read(tile[buf], 0);
                 } else {
-                    to.read(tile[buf], r0);
-                    READ_AHEAD();
+                    so.read(tile[buf], r0);
                     scores<E, NS, DP>(s, own, so);
+                    to.read(tile[buf], r0);
                 }
-                if (blk + 1 < St::BLOCKS) so.read(tile[buf], 32);
-                else {
-                    if (i + 1 < nt) store(i + 1, 0, buf ^ 1);  // (facts: the other one of the two)
-                    __syncthreads();
-                    so.read(tile[i + 1 < nt ? buf ^ 1 : buf], 0);
-                }
-                READ_AHEAD();
                 // Where a row's target is among the owned table rows q is -g (1 - p), formed from the sum over the other
                 // items: popular items are targets in every block, so this has to be cheap.  A lane collects the rows
                 // whose target is its own table row as bits.
@@ -746,6 +735,8 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, true)) void table
                 p.pack(q);
                 accumulate<E, NS, DP>(out, p, to);
             }
+            if (i + 1 < nt) store(i + 1, 0, buf ^ 1);
+            __syncthreads();
             buf ^= 1;
         }
         const float total = half_wave_sum(db);
