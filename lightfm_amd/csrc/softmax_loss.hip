@@ -116,22 +116,34 @@ __device__ inline int64_t target_of(const lfm_softmax_args &a, int64_t n)
 
 // -------------------------------------------------------------- operands ---
 
-// Largest finite magnitudes: blocks [0, parts) of x (rows with a target), of w, of g.
-template <typename T>
-__global__ __launch_bounds__(256) void largest_kernel(lfm_softmax_args a, int parts, float *largest, int tensors)
+// Largest finite magnitudes: `parts` blocks for x (rows with a target; their outlier flags are cleared on the way), as many
+// for w (float32 operands alone), as many for g.  Threads take four columns of a row each; WIDE_LOADS: at once.
+template <typename T, bool WIDE_LOADS>
+__global__ __launch_bounds__(256) void largest_kernel(lfm_softmax_args a, int parts, float *largest, int tensors, uint8_t *outlier)
 {
     const int which = blockIdx.x / parts, part = blockIdx.x % parts;
     float m = 0.0f;
     if (which < 2 && tensors == 3) {
         const T *p = (const T *)(which ? a.table : a.hidden);
         const int64_t rows = which ? a.vocab : a.rows, stride = which ? a.table_stride : a.hidden_stride;
-        const int64_t n = rows * a.d;
-        for (int64_t i = (int64_t)part * 256 + threadIdx.x; i < n; i += (int64_t)parts * 256) {
-            const int64_t r = i / a.d;
-            if (!which && target_of(a, r) < 0) continue;
-            const float v = fabsf((float)p[r * stride + (i - r * a.d)]);
-            if (v < INFINITY) m = fmaxf(m, v);
-        }
+        const int groups = (a.d + 3) / 4, per = 256 / groups, tr = (int)threadIdx.x / groups, c = ((int)threadIdx.x - tr * groups) * 4;
+        auto look = [&](float v) { if (fabsf(v) < INFINITY) m = fmaxf(m, fabsf(v)); };
+        const int64_t step = (int64_t)parts * per;
+        if (tr < per)
+#pragma unroll 4
+            for (int64_t r = (int64_t)part * per + tr; r < rows; r += step) {
+                if (!which) {
+                    if (c == 0) outlier[r] = 0;
+                    if (target_of(a, r) < 0) continue;
+                }
+                const T *q = p + r * stride + c;
+                if (WIDE_LOADS) {
+                    const Vec<T, 4> v = *(const Vec<T, 4> *)q;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) look((float)v.v[j]);
+                } else
+                    for (int j = 0; j < 4 && c + j < a.d; ++j) look((float)q[j]);
+            }
     } else {
         for (int64_t i = (int64_t)part * 256 + threadIdx.x; i < a.rows; i += (int64_t)parts * 256) {
             if (target_of(a, i) < 0) continue;
@@ -165,8 +177,8 @@ struct PackArgs {
 };
 
 // Rows of x and w to the padded, split form, zeros behind d: per row and chunk of `width` columns [hi: width | lo: width]
-// (width = dp up to 256 columns, 256 beyond).  A thread makes 8 elements.
-template <typename T, typename E, int NS>
+// (width = dp up to 256 columns, 256 beyond).  A thread makes 8 elements; WIDE_LOADS: reads them at once.
+template <typename T, typename E, int NS, bool WIDE_LOADS>
 __global__ __launch_bounds__(256) void pack_kernel(PackArgs p, int dp, int width)
 {
     __shared__ int ks[3];
@@ -188,28 +200,33 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs p, int dp, int width
         }
     }
     typedef typename Half<E>::x8 x8;
-    const int chunks = dp / 8;
-    const int64_t xr = p.x ? p.a.rows : 0, wr = p.w ? p.a.vocab : 0, n = (xr + wr) * chunks;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        int64_t r = i / chunks;
-        const int c = (int)(i - r * chunks) * 8;
-        const bool is_x = r < xr;
-        if (!is_x) r -= xr;
+    const int chunks = dp / 8, per = 256 / chunks, tr = (int)threadIdx.x / chunks, c = ((int)threadIdx.x - tr * chunks) * 8;
+    const int64_t xr = p.x ? p.a.rows : 0, n = xr + (p.w ? p.a.vocab : 0);
+    const int at = (c / width) * (NS * width) + c % width;
+    if (tr >= per) return;
+    for (int64_t i = (int64_t)blockIdx.x * per + tr; i < n; i += (int64_t)gridDim.x * per) {
+        const bool is_x = i < xr;
+        const int64_t r = is_x ? i : i - xr;
         const T *src = is_x ? (const T *)p.a.hidden + r * p.a.hidden_stride : (const T *)p.a.table + r * p.a.table_stride;
-        E *dst = (E *)(is_x ? p.x : p.w) + r * (NS * dp) + (c / width) * (NS * width) + c % width;
+        E *dst = (E *)(is_x ? p.x : p.w) + r * (NS * dp) + at;
+        Vec<T, 8> v;
+        if (WIDE_LOADS && c + 8 <= p.a.d) v = *(const Vec<T, 8> *)(src + c);
+        else
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v.v[j] = c + j < p.a.d ? src[c + j] : (T)0.0f;
         x8 hi, lo;
         if (NS == 1) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) hi[j] = c + j < p.a.d ? (E)src[c + j] : (E)0.0f;
+            for (int j = 0; j < 8; ++j) hi[j] = (E)v.v[j];
         } else {
             const int k = ks[is_x ? 0 : 1];
             bool fits = true;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                float v = c + j < p.a.d ? ldexpf((float)src[c + j], k) : 0.0f;
-                if (is_x && !(fabsf(v) < 65504.0f)) { fits = false; v = 0.0f; }
-                hi[j] = (E)v;
-                lo[j] = (E)(v - (float)hi[j]);
+                float f = ldexpf((float)v.v[j], k);
+                if (is_x && !(fabsf(f) < 65504.0f)) { fits = false; f = 0.0f; }
+                hi[j] = (E)f;
+                lo[j] = (E)(f - (float)hi[j]);
             }
             if (is_x && !fits) p.outlier[r] = 1;
             *(x8 *)(dst + width) = lo;
@@ -773,6 +790,105 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, true)) void table
     }
 }
 
+// ---------------------------------------------------------------- few rows ---
+
+// Without the gradient and with so few rows that the matrix cores would run on padding, the table is read once, as it is,
+// and multiplied in float32: `lanes` neighbouring lanes own a table row, VEC elements each and step.  Bound by reading the
+// table.  A block leaves the maximum and the sum of its part of the table for each of up to ROWS rows, like rows_kernel.
+constexpr int FEW = 8;
+
+template <typename T, int VEC, int ROWS>
+__global__ __launch_bounds__(256) void few_rows_kernel(SweepArgs a, const T *hidden, const T *table, int lanes_log2)
+{
+    constexpr int U = ROWS > 4 ? 2 : 4;  // table rows in flight
+    __shared__ __attribute__((aligned(16))) float xs[ROWS][LFM_MAX_COMPONENTS];
+    __shared__ float ms[ROWS][4], ls[ROWS][4];
+    __shared__ int64_t ts[ROWS];
+    const Derived dv = derive(nullptr);
+    const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> lanes_log2, groups = 256 >> lanes_log2;
+    const int64_t n0 = (int64_t)blockIdx.y * ROWS;
+    const int rows = a.rows - n0 < ROWS ? (int)(a.rows - n0) : ROWS;
+    for (int i = threadIdx.x; i < ROWS * a.d; i += 256) {
+        const int r = i / a.d, c = i - r * a.d;
+        xs[r][c] = r < rows ? (float)hidden[(n0 + r) * a.ldx + c] : 0.0f;
+    }
+    if (threadIdx.x < ROWS) {
+        const int64_t n = n0 + threadIdx.x;
+        ts[threadIdx.x] = (int)threadIdx.x >= rows ? -1 : a.id_bytes == 8 ? ((const int64_t *)a.targets)[n] : (int64_t)((const int32_t *)a.targets)[n];
+    }
+    __syncthreads();
+    float m[ROWS], l[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        m[r] = dv.low * 1.01f;
+        l[r] = 0.0f;
+    }
+    const int64_t lo = a.vocab * blockIdx.x / gridDim.x, hi = a.vocab * (blockIdx.x + 1) / gridDim.x;
+    for (int64_t v0 = lo + group; v0 < hi; v0 += (int64_t)U * groups) {
+        float s[U][ROWS], b[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t v = v0 + (int64_t)u * groups;
+            b[u] = v >= hi ? -INFINITY : a.bias ? bias_units(a.bias[v], dv) : 0.0f;
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) s[u][r] = 0.0f;
+        }
+        for (int c = lane * VEC; c < a.d; c += lanes * VEC) {
+            Vec<T, VEC> w[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t v = v0 + (int64_t)u * groups;
+                w[u] = *(const Vec<T, VEC> *)(table + (v < hi ? v : v0) * a.ldw + c);
+            }
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) {
+                    const float x = xs[r][c + k];
+#pragma unroll
+                    for (int u = 0; u < U; ++u) s[u][r] = __builtin_fmaf(x, (float)w[u].v[k], s[u][r]);
+                }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t v = v0 + (int64_t)u * groups;
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                for (int o = lanes >> 1; o; o >>= 1) s[u][r] += __shfl_xor(s[u][r], o);
+                const float score = v == ts[r] ? -INFINITY : s[u][r] + b[u];  // the target is left to the join
+                const float up = fmaxf(m[r], score);
+                l[r] = l[r] * exp2_fast((m[r] - up) * LOG2E) + exp2_fast((score - up) * LOG2E + P_SHIFT);
+                m[r] = up;
+            }
+        }
+    }
+    // a wave's groups, then the block's waves
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        for (int o = lanes; o < 64; o <<= 1) {
+            const float mo = __shfl_xor(m[r], o), lo2 = __shfl_xor(l[r], o), up = fmaxf(m[r], mo);
+            l[r] = l[r] * exp2_fast((m[r] - up) * LOG2E) + lo2 * exp2_fast((mo - up) * LOG2E);
+            m[r] = up;
+        }
+        if ((threadIdx.x & 63) == 0) {
+            ms[r][threadIdx.x >> 6] = m[r];
+            ls[r][threadIdx.x >> 6] = l[r];
+        }
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < rows) {
+        const int r = threadIdx.x;
+        float mm = ms[r][0], ll = ls[r][0];
+        for (int w = 1; w < 4; ++w) {
+            const float up = fmaxf(mm, ms[r][w]);
+            ll = ll * exp2_fast((mm - up) * LOG2E) + ls[r][w] * exp2_fast((ms[r][w] - up) * LOG2E);
+            mm = up;
+        }
+        a.pm[(int64_t)blockIdx.x * a.rows + n0 + r] = mm;
+        a.pl[(int64_t)blockIdx.x * a.rows + n0 + r] = ll;
+    }
+}
+
 // ------------------------------------------------------------------- joins ---
 
 struct JoinArgs {
@@ -781,6 +897,7 @@ struct JoinArgs {
     const uint8_t *outlier;
     Pieces pieces;
     int parts, dp, ns, grad, shifted;
+    int few;                // few_rows_kernel: every row has `parts` parts
     const float *pm, *pl, *po;
     float *row_max, *row_rate, *row_weight;
     int32_t *row_target;
@@ -806,17 +923,20 @@ __device__ inline float dot_lane(const T *x, const T *w, int d)
     return s;
 }
 
-// One wave per row: joins the parts of the table, finishes lse, loss, dx, and leaves table_kernel what it needs.
-template <typename T>
+// Joins the parts of the table, finishes lse, loss, dx, and leaves table_kernel what it needs.  WAVES waves (1 or 4) per row:
+// one where there are rows enough, four (which share the parts) where a row has many parts and there are few rows.
+template <typename T, int WAVES>
 __global__ __launch_bounds__(256) void join_rows_kernel(JoinArgs j)
 {
+    __shared__ float shared[4][64];
     const lfm_softmax_args &a = j.a;
-    const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (n >= a.rows) return;
+    const int wave = threadIdx.x >> 6;
+    const int64_t n = (int64_t)blockIdx.x * (4 / WAVES) + wave / WAVES;
+    if (n >= a.rows) return;  // (with four waves: all of the block)
     const int lane = threadIdx.x & 63;
     const Derived dv = derive(j.ns == 2 ? j.scales : nullptr);
     const uint32_t owner = (uint32_t)(n / 128);
-    const int splits = (int)(j.pieces.last_block(owner) - j.pieces.first_block(owner)) + 1;
+    const int splits = j.few ? j.parts : (int)(j.pieces.last_block(owner) - j.pieces.first_block(owner)) + 1;
     float m = -INFINITY;
     for (int s = lane; s < splits; s += 64) m = fmaxf(m, j.pm[(int64_t)s * a.rows + n]);
     m = wave_max(m);
@@ -866,13 +986,13 @@ __global__ __launch_bounds__(256) void join_rows_kernel(JoinArgs j)
     }
     if (odd && t >= 0) loss = NAN;
     loss = t < 0 ? 0.0f : g * loss;
-    if (lane == 0) {
+    if (lane == 0 && wave % WAVES == 0) {
         a.lse[n] = lse;
         a.loss[n] = loss;
     }
     if (!j.grad) return;
     const bool lost = odd && t >= 0;  // not finite: its gradients are not either
-    if (lane == 0) {
+    if (lane == 0 && wave % WAVES == 0) {
         const int shift = j.shifted == 2 ? 14 - j.scales->eg : j.shifted ? 14 : 0;
         const float gs = ldexpf(g, shift);
         j.row_target[n] = (int32_t)t;
@@ -881,14 +1001,26 @@ __global__ __launch_bounds__(256) void join_rows_kernel(JoinArgs j)
         j.row_weight[n] = gs * other;
     }
     const int kw = j.ns == 2 ? j.scales->kw : 0;
-    for (int c = lane; c < a.d; c += 64) {
+    for (int c0 = 0; c0 < a.d; c0 += 64) {
+        const int c = c0 + lane;
         float o = 0.0f;
-        if (t >= 0) {
+        if (t >= 0 && c < a.d) {
             const float *pm = j.pm + (int64_t)(c >> 8) * j.parts * a.rows;  // the maxima that chunk c / 256 went by
-            for (int s = 0; s < splits; ++s) {
+#pragma unroll 8
+            for (int s = wave % WAVES; s < splits; s += WAVES) {
                 const int64_t at = (int64_t)s * a.rows + n;
-                o += j.po[at * j.dp + c] * exp2_fast((pm[at] - m) * dv.c);
+                o = __builtin_fmaf(j.po[at * j.dp + c], exp2_fast((pm[at] - m) * dv.c), o);
             }
+        }
+        if (WAVES > 1) {
+            __syncthreads();
+            shared[wave][lane] = o;
+            __syncthreads();
+            if (wave) continue;
+            o = shared[0][lane] + shared[1][lane] + shared[2][lane] + shared[3][lane];
+        }
+        if (c >= a.d) continue;
+        if (t >= 0) {
             o = sum == 0.0f ? 0.0f : ldexpf(o / sum, -kw);
             o = lost ? NAN : g * (o - other * (float)wt[c]);
         }
@@ -896,25 +1028,45 @@ __global__ __launch_bounds__(256) void join_rows_kernel(JoinArgs j)
     }
 }
 
-// dw and db of the table rows that several blocks share, added in the order of the blocks
+// dw and db of the table rows that several blocks share, added in the order of the blocks: block (owner, 32 columns)
 template <typename T>
 __global__ __launch_bounds__(256) void join_table_kernel(SweepArgs a, int ns)
 {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, v = i / a.d;
-    if (v >= a.vocab) return;
-    const uint32_t owner = (uint32_t)(v / 128), b0 = a.pieces.first_block(owner), b1 = a.pieces.last_block(owner);
+    const uint32_t owner = blockIdx.x, b0 = a.pieces.first_block(owner), b1 = a.pieces.last_block(owner);
     if (b0 == b1) return;
-    const int c = (int)(i - v * a.d);
     const int shift = a.shifted == 2 ? a.scales->eg - 14 : a.shifted ? -14 : 0, kx = ns == 2 ? a.scales->kx : 0;
-    float s = 0.0f, t = 0.0f;
-    for (uint32_t b = b0; b <= b1; ++b) {
-        const int64_t part = 2 * (int64_t)b + (a.pieces.begin(b) > (uint64_t)owner * a.pieces.tiles ? 0 : 1);
-        const int64_t at = part * 128 + (v - (int64_t)owner * 128);
-        s += a.pw[at * a.dp + c];
-        if (c == 0) t += a.pb[at];
+    // only the first of the blocks may have begun with an earlier owner
+    const int64_t first = 2 * (int64_t)b0 + (a.pieces.begin(b0) > (uint64_t)owner * a.pieces.tiles ? 0 : 1);
+    auto part = [&](uint32_t b) { return b == b0 ? first : 2 * (int64_t)b; };
+    const int c = (int)blockIdx.y * 32 + (threadIdx.x & 7) * 4;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int r = q * 32 + (threadIdx.x >> 3);
+        const int64_t v = (int64_t)owner * 128 + r;
+        if (v >= a.vocab || c >= a.d) continue;
+        float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (uint32_t b = b0; b <= b1; ++b) {
+            const float4 p = *(const float4 *)(a.pw + (part(b) * 128 + r) * a.dp + c);
+            s.x += p.x;
+            s.y += p.y;
+            s.z += p.z;
+            s.w += p.w;
+        }
+        const float o[4] = {s.x, s.y, s.z, s.w};
+        T *to = (T *)a.dw + v * a.d + c;
+        Vec<T, 4> ov;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ov.v[j] = (T)ldexpf(o[j], shift - kx);
+        if ((a.d & 3) == 0) *(Vec<T, 4> *)to = ov;
+        else
+            for (int j = 0; j < 4; ++j)
+                if (c + j < a.d) to[j] = ov.v[j];
     }
-    ((T *)a.dw)[i] = (T)ldexpf(s, shift - kx);
-    if (c == 0 && a.db) a.db[v] = ldexpf(t, shift);
+    if (a.db && blockIdx.y == 0 && threadIdx.x < 128 && (int64_t)owner * 128 + threadIdx.x < a.vocab) {
+        float t = 0.0f;
+        for (uint32_t b = b0; b <= b1; ++b) t += a.pb[part(b) * 128 + threadIdx.x];
+        a.db[(int64_t)owner * 128 + threadIdx.x] = ldexpf(t, shift);
+    }
 }
 
 template <typename T>
@@ -927,10 +1079,16 @@ __global__ __launch_bounds__(256) void clear_kernel(T *p, int64_t n, float *q, i
 
 // -------------------------------------------------------------------- host ---
 
+// the few-rows form is taken up to here (without the gradient)
+#ifndef FEW_ROWS_MOST
+#define FEW_ROWS_MOST 8
+#endif
+
 struct Plan {
     int dp, ns;
     int chunks;             // of 256 columns
     Pieces rows, table;
+    int few;                // blocks over the table of the few-rows form, 0: the matrix form
 };
 
 int width_for(int d)
@@ -960,6 +1118,11 @@ Plan plan_for(int64_t rows, int64_t vocab, int d, int dtype, bool grad)
     const int w = p.dp > 256 ? 256 : p.dp, bv = p.ns * w <= 128 ? 64 : 32;
     // as many blocks as run at once on the card's 256 compute units
     p.rows = pieces_for(rows, vocab, bv, 256 * (p.chunks > 1 ? 1 : waves_for(p.ns, w, grad)));
+    p.few = 0;
+    if (!grad && rows <= FEW_ROWS_MOST) {
+        const int64_t want = ceil_div(vocab, 16);  // (a block's lane groups have a few table rows each)
+        p.few = (int)(want < 1024 ? want : 1024);
+    }
     p.table = pieces_for(vocab, rows, bv, 256 * (p.chunks > 1 ? 1 : waves_for(p.ns, w, true)));
     return p;
 }
@@ -979,7 +1142,13 @@ struct Space {
 Space space_for(const Plan &p, int64_t rows, int64_t vocab, bool grad, void *ws)
 {
     Carver c(ws);
-    Space s;
+    Space s = {};
+    if (p.few) {
+        s.pm = c.take<float>(rows * p.few);
+        s.pl = c.take<float>(rows * p.few);
+        s.bytes = c.used;
+        return s;
+    }
     s.scales = c.take<Scales>(1);
     s.largest = c.take<float>(3 * MAX_PARTS);
     s.outlier = c.take<uint8_t>(rows);
@@ -1026,6 +1195,26 @@ hipError_t sweep_table(const SweepArgs &s, hipStream_t st)
     default: e = call(256, true); break;        \
     }
 
+template <typename T, int VEC>
+hipError_t launch_few(const SweepArgs &w, const lfm_softmax_args &a, int blocks, hipStream_t st)
+{
+    int ll = 0;
+    while ((1 << ll) * VEC < a.d && ll < 6) ++ll;
+    if (a.rows == 1) few_rows_kernel<T, VEC, 1><<<dim3((unsigned)blocks), 256, 0, st>>>(w, (const T *)a.hidden, (const T *)a.table, ll);
+    else
+        few_rows_kernel<T, VEC, FEW><<<dim3((unsigned)blocks, (unsigned)ceil_div(a.rows, FEW)), 256, 0, st>>>(
+            w, (const T *)a.hidden, (const T *)a.table, ll);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t join_rows(const JoinArgs &j, int64_t parts, hipStream_t st)
+{
+    if (parts > 8 && j.a.rows <= 4096) join_rows_kernel<T, 4><<<dim3((unsigned)j.a.rows), 256, 0, st>>>(j);
+    else join_rows_kernel<T, 1><<<dim3((unsigned)ceil_div(j.a.rows, 4)), 256, 0, st>>>(j);
+    return hipGetLastError();
+}
+
 template <typename T, typename E, int NS>
 hipError_t run(const lfm_softmax_args &a, bool grad, void *ws, hipStream_t st)
 {
@@ -1041,7 +1230,35 @@ hipError_t run(const lfm_softmax_args &a, bool grad, void *ws, hipStream_t st)
     const bool scales = NS == 2 || (a.dtype == LFM_F16 && a.weights && grad);
     auto in_place = [&](const void *q, int64_t stride) { return NS == 1 && a.d == p.dp && stride % 8 == 0 && ((uintptr_t)q & 15) == 0; };
     const bool x_there = in_place(a.hidden, a.hidden_stride), w_there = in_place(a.table, a.table_stride);
-    PackArgs pk;
+    // both operands can be read 16 bytes at a time
+    const int whole = 16 / (int)sizeof(T);
+    const bool wide = a.d % whole == 0 && a.hidden_stride % whole == 0 && a.table_stride % whole == 0 &&
+                      (((uintptr_t)a.hidden | (uintptr_t)a.table) & 15) == 0;
+    SweepArgs w = {};
+    w.rows = a.rows;
+    w.vocab = a.vocab;
+    w.bias = a.bias;
+    w.targets = a.targets;
+    w.id_bytes = a.id_bytes;
+    w.d = a.d;
+    w.pm = s.pm;
+    w.pl = s.pl;
+    JoinArgs j = {};
+    j.a = a;
+    j.grad = grad ? 1 : 0;
+    j.pm = s.pm;
+    j.pl = s.pl;
+    if (p.few) {
+        w.ldx = a.hidden_stride;
+        w.ldw = a.table_stride;
+        e = wide ? launch_few<T, 16 / (int)sizeof(T)>(w, a, p.few, st) : launch_few<T, 1>(w, a, p.few, st);
+        if (e != hipSuccess) return e;
+        j.ns = 1;
+        j.few = 1;
+        j.parts = p.few;
+        return join_rows<T>(j, p.few, st);
+    }
+    PackArgs pk = {};
     pk.a = a;
     pk.largest = scales ? s.largest : nullptr;
     pk.tensors = NS == 2 ? 3 : 1;
@@ -1052,38 +1269,29 @@ hipError_t run(const lfm_softmax_args &a, bool grad, void *ws, hipStream_t st)
     const int64_t most = NS == 2 ? (a.rows > a.vocab ? a.rows : a.vocab) * a.d : a.rows;
     pk.parts = (int)(ceil_div(most, 4096) < MAX_PARTS ? ceil_div(most, 4096) : MAX_PARTS);
     if (scales) {
-        largest_kernel<T><<<dim3((unsigned)(pk.tensors * pk.parts)), 256, 0, st>>>(a, pk.parts, s.largest, pk.tensors);
-        if ((e = hipGetLastError()) != hipSuccess) return e;
-    }
-    if (NS == 2) {
-        clear_kernel<uint8_t><<<dim3((unsigned)ceil_div(a.rows, 256)), 256, 0, st>>>(s.outlier, a.rows, nullptr, 0);
+        const dim3 grid((unsigned)(pk.tensors * pk.parts));
+        if (wide) largest_kernel<T, true><<<grid, 256, 0, st>>>(a, pk.parts, s.largest, pk.tensors, s.outlier);
+        else largest_kernel<T, false><<<grid, 256, 0, st>>>(a, pk.parts, s.largest, pk.tensors, s.outlier);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     if (scales || pk.x || pk.w) {
-        const int64_t work = ((pk.x ? a.rows : 0) + (pk.w ? a.vocab : 0)) * (p.dp / 8);
-        int64_t blocks = ceil_div(work, 256);
+        const int64_t per = 256 / (p.dp / 8);
+        int64_t blocks = ceil_div((pk.x ? a.rows : 0) + (pk.w ? a.vocab : 0), per);
         blocks = blocks < 1 ? 1 : blocks > 4096 ? 4096 : blocks;
-        pack_kernel<T, E, NS><<<dim3((unsigned)blocks), 256, 0, st>>>(pk, p.dp, p.dp < 256 ? p.dp : 256);
+        const int width = p.dp < 256 ? p.dp : 256;
+        if (wide) pack_kernel<T, E, NS, true><<<dim3((unsigned)blocks), 256, 0, st>>>(pk, p.dp, width);
+        else pack_kernel<T, E, NS, false><<<dim3((unsigned)blocks), 256, 0, st>>>(pk, p.dp, width);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
-    SweepArgs w;
     w.x = x_there ? a.hidden : s.x;
     w.ldx = x_there ? a.hidden_stride : NS * p.dp;
     w.w = w_there ? a.table : s.w;
     w.ldw = w_there ? a.table_stride : NS * p.dp;
-    w.rows = a.rows;
-    w.vocab = a.vocab;
-    w.bias = a.bias;
-    w.targets = a.targets;
-    w.id_bytes = a.id_bytes;
     w.scales = s.scales;
     w.pieces = p.rows;
     w.parts = (int)p.rows.most();
-    w.d = a.d;
     w.dp = p.dp;
     w.chunks = p.chunks;
-    w.pm = s.pm;
-    w.pl = s.pl;
     w.po = s.po;
     w.row_max = s.row_max;
     w.row_rate = s.row_rate;
@@ -1097,30 +1305,24 @@ hipError_t run(const lfm_softmax_args &a, bool grad, void *ws, hipStream_t st)
 #define ROWS(DP, WIDE) sweep_rows<E, NS, DP, WIDE>(w, grad, st)
     BY_WIDTH(p.dp, ROWS)
     if (e != hipSuccess) return e;
-    JoinArgs j;
-    j.a = a;
     j.scales = s.scales;
     j.outlier = s.outlier;
     j.pieces = p.rows;
     j.parts = w.parts;
     j.dp = p.dp;
     j.ns = NS;
-    j.grad = grad ? 1 : 0;
     j.shifted = w.shifted;
-    j.pm = s.pm;
-    j.pl = s.pl;
     j.po = s.po;
     j.row_max = s.row_max;
     j.row_rate = s.row_rate;
     j.row_weight = s.row_weight;
     j.row_target = s.row_target;
-    join_rows_kernel<T><<<dim3((unsigned)ceil_div(a.rows, 4)), 256, 0, st>>>(j);
-    if ((e = hipGetLastError()) != hipSuccess || !grad) return e;
+    if ((e = join_rows<T>(j, w.parts, st)) != hipSuccess || !grad) return e;
     w.pieces = p.table;
 #define TABLE(DP, WIDE) sweep_table<T, E, NS, DP, WIDE>(w, st)
     BY_WIDTH(p.dp, TABLE)
     if (e != hipSuccess || p.table.owners % p.table.blocks == 0) return e;  // (no block shares an owner)
-    join_table_kernel<T><<<dim3((unsigned)ceil_div(a.vocab * a.d, 256)), 256, 0, st>>>(w, NS);
+    join_table_kernel<T><<<dim3(p.table.owners, (unsigned)(p.dp / 32)), 256, 0, st>>>(w, NS);
     return hipGetLastError();
 }
 
