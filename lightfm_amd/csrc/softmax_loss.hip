@@ -177,7 +177,7 @@ struct PackArgs {
 };
 
 // Rows of x and w to the padded, split form, zeros behind d: per row and chunk of `width` columns [hi: width | lo: width]
-// (width = dp up to 256 columns, 256 beyond).  A thread makes 8 elements; WIDE_LOADS: reads them at once.
+// (width = dp up to 256 columns, 256 beyond).  A thread makes 8 elements; WIDE_LOADS: reads them 4 at once.
 template <typename T, typename E, int NS, bool WIDE_LOADS>
 __global__ __launch_bounds__(256) void pack_kernel(PackArgs p, int dp, int width)
 {
@@ -209,21 +209,25 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs p, int dp, int width
         const int64_t r = is_x ? i : i - xr;
         const T *src = is_x ? (const T *)p.a.hidden + r * p.a.hidden_stride : (const T *)p.a.table + r * p.a.table_stride;
         E *dst = (E *)(is_x ? p.x : p.w) + r * (NS * dp) + at;
-        Vec<T, 8> v;
-        if (WIDE_LOADS && c + 8 <= p.a.d) v = *(const Vec<T, 8> *)(src + c);
-        else
+        Vec<T, 4> v[2];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v.v[j] = c + j < p.a.d ? src[c + j] : (T)0.0f;
+        for (int q = 0; q < 2; ++q) {
+            const int cq = c + 4 * q;
+            if (WIDE_LOADS && cq + 4 <= p.a.d) v[q] = *(const Vec<T, 4> *)(src + cq);
+            else
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[q].v[j] = cq + j < p.a.d ? src[cq + j] : (T)0.0f;
+        }
         x8 hi, lo;
         if (NS == 1) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) hi[j] = (E)v.v[j];
+            for (int j = 0; j < 8; ++j) hi[j] = (E)v[j >> 2].v[j & 3];
         } else {
             const int k = ks[is_x ? 0 : 1];
             bool fits = true;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                float f = ldexpf((float)v.v[j], k);
+                float f = ldexpf((float)v[j >> 2].v[j & 3], k);
                 if (is_x && !(fabsf(f) < 65504.0f)) { fits = false; f = 0.0f; }
                 hi[j] = (E)f;
                 lo[j] = (E)(f - (float)hi[j]);
@@ -446,6 +450,7 @@ struct SweepArgs {
     const int32_t *row_target;
     void *dw;               // table rows that one block has to itself
     float *db, *pw, *pb;    // the others': per block its first and its last owner, [128][dp], [128]
+    int aligned;            // rows of dw can be written four elements at a time
     int shifted;            // q is scaled by 2^(14 - eg): 0 no (bfloat16), 1 with eg = 0, 2 with eg of scales
 };
 
@@ -781,7 +786,7 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, true)) void table
                 Vec<T, 4> o;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) o.v[j] = (T)ldexpf(out[b][4 * g + j], shift - kx);
-                if (c + 4 <= a.d && (a.d & 3) == 0) *(Vec<T, 4> *)(row + c) = o;
+                if (a.aligned && c < a.d) *(Vec<T, 4> *)(row + c) = o;
                 else
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
@@ -792,13 +797,16 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, true)) void table
 
 // ---------------------------------------------------------------- few rows ---
 
-// Without the gradient and with so few rows that the matrix cores would run on padding, the table is read once, as it is,
-// and multiplied in float32: `lanes` neighbouring lanes own a table row, VEC elements each and step.  Bound by reading the
-// table.  A block leaves the maximum and the sum of its part of the table for each of up to ROWS rows, like rows_kernel.
+// Without the gradient and with up to FEW float32 rows the table is read once, as it is, and multiplied in float32: the
+// matrix form reads it twice and writes it once before it begins.  `lanes` neighbouring lanes own a table row, VEC elements
+// each and step.  Bound by reading the table.  A block leaves the maximum and the sum of its part of the table for each
+// row, like rows_kernel.  Measured (us, with the join; matrix form in brackets): 26744 x 64, one row 14.6 (24), 8 rows 23.8 (24.8), 16 rows
+// 32.5 (24.8); 200003 x 128: 31 (134), 102 (134), 189 (135).  Half-precision tables need no packing where their rows are 16-byte
+// aligned, and the matrix form is then the faster one from one row on (26744 x 64: 10.5).
 constexpr int FEW = 8;
 
-template <typename T, int VEC, int ROWS>
-__global__ __launch_bounds__(256) void few_rows_kernel(SweepArgs a, const T *hidden, const T *table, int lanes_log2)
+template <int VEC, int ROWS>
+__global__ __launch_bounds__(256) void few_rows_kernel(SweepArgs a, const float *hidden, const float *table, int lanes_log2)
 {
     constexpr int U = ROWS > 4 ? 2 : 4;  // table rows in flight
     __shared__ __attribute__((aligned(16))) float xs[ROWS][LFM_MAX_COMPONENTS];
@@ -806,14 +814,13 @@ __global__ __launch_bounds__(256) void few_rows_kernel(SweepArgs a, const T *hid
     __shared__ int64_t ts[ROWS];
     const Derived dv = derive(nullptr);
     const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> lanes_log2, groups = 256 >> lanes_log2;
-    const int64_t n0 = (int64_t)blockIdx.y * ROWS;
-    const int rows = a.rows - n0 < ROWS ? (int)(a.rows - n0) : ROWS;
+    const int rows = (int)a.rows;
     for (int i = threadIdx.x; i < ROWS * a.d; i += 256) {
         const int r = i / a.d, c = i - r * a.d;
-        xs[r][c] = r < rows ? (float)hidden[(n0 + r) * a.ldx + c] : 0.0f;
+        xs[r][c] = r < rows ? hidden[r * a.ldx + c] : 0.0f;
     }
     if (threadIdx.x < ROWS) {
-        const int64_t n = n0 + threadIdx.x;
+        const int n = threadIdx.x;
         ts[threadIdx.x] = (int)threadIdx.x >= rows ? -1 : a.id_bytes == 8 ? ((const int64_t *)a.targets)[n] : (int64_t)((const int32_t *)a.targets)[n];
     }
     __syncthreads();
@@ -834,11 +841,11 @@ __global__ __launch_bounds__(256) void few_rows_kernel(SweepArgs a, const T *hid
             for (int r = 0; r < ROWS; ++r) s[u][r] = 0.0f;
         }
         for (int c = lane * VEC; c < a.d; c += lanes * VEC) {
-            Vec<T, VEC> w[U];
+            Vec<float, VEC> w[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int64_t v = v0 + (int64_t)u * groups;
-                w[u] = *(const Vec<T, VEC> *)(table + (v < hi ? v : v0) * a.ldw + c);
+                w[u] = *(const Vec<float, VEC> *)(table + (v < hi ? v : v0) * a.ldw + c);
             }
 #pragma unroll
             for (int r = 0; r < ROWS; ++r)
@@ -846,7 +853,7 @@ __global__ __launch_bounds__(256) void few_rows_kernel(SweepArgs a, const T *hid
                 for (int k = 0; k < VEC; ++k) {
                     const float x = xs[r][c + k];
 #pragma unroll
-                    for (int u = 0; u < U; ++u) s[u][r] = __builtin_fmaf(x, (float)w[u].v[k], s[u][r]);
+                    for (int u = 0; u < U; ++u) s[u][r] = __builtin_fmaf(x, w[u].v[k], s[u][r]);
                 }
         }
 #pragma unroll
@@ -884,8 +891,8 @@ __global__ __launch_bounds__(256) void few_rows_kernel(SweepArgs a, const T *hid
             ll = ll * exp2_fast((mm - up) * LOG2E) + ls[r][w] * exp2_fast((ms[r][w] - up) * LOG2E);
             mm = up;
         }
-        a.pm[(int64_t)blockIdx.x * a.rows + n0 + r] = mm;
-        a.pl[(int64_t)blockIdx.x * a.rows + n0 + r] = ll;
+        a.pm[(int64_t)blockIdx.x * a.rows + r] = mm;
+        a.pl[(int64_t)blockIdx.x * a.rows + r] = ll;
     }
 }
 
@@ -898,22 +905,11 @@ struct JoinArgs {
     Pieces pieces;
     int parts, dp, ns, grad, shifted;
     int few;                // few_rows_kernel: every row has `parts` parts
+    int aligned;            // rows of d_hidden can be written four elements at a time
     const float *pm, *pl, *po;
     float *row_max, *row_rate, *row_weight;
     int32_t *row_target;
 };
-
-__device__ inline float wave_sum(float v)
-{
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
-
-__device__ inline float wave_max(float v)
-{
-    for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
-}
 
 template <typename T>
 __device__ inline float dot_lane(const T *x, const T *w, int d)
@@ -923,43 +919,67 @@ __device__ inline float dot_lane(const T *x, const T *w, int d)
     return s;
 }
 
-// Joins the parts of the table, finishes lse, loss, dx, and leaves table_kernel what it needs.  WAVES waves (1 or 4) per row:
-// one where there are rows enough, four (which share the parts) where a row has many parts and there are few rows.
-template <typename T, int WAVES>
+// Sums and maxima over the lanes that share a row: 16 neighbouring ones, or the block's 256
+template <int LANES>
+__device__ inline float row_sum(float v, float *shared)
+{
+    for (int o = LANES < 64 ? LANES / 2 : 32; o; o >>= 1) v += __shfl_xor(v, o);
+    if (LANES < 64) return v;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return shared[0] + shared[1] + shared[2] + shared[3];
+}
+
+template <int LANES>
+__device__ inline float row_max(float v, float *shared)
+{
+    for (int o = LANES < 64 ? LANES / 2 : 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    if (LANES < 64) return v;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return fmaxf(fmaxf(shared[0], shared[1]), fmaxf(shared[2], shared[3]));
+}
+
+// Joins the parts of the table, finishes lse, loss, dx, and leaves table_kernel what it needs.  LANES lanes per row: 16 where
+// there are rows enough to fill the card, a block's 256 (which share the parts, too) where there are few.
+template <typename T, int LANES>
 __global__ __launch_bounds__(256) void join_rows_kernel(JoinArgs j)
 {
-    __shared__ float shared[4][64];
+    __shared__ float shared[4];
+    __shared__ __attribute__((aligned(16))) float4 sums[LANES == 256 ? 256 : 1];
     const lfm_softmax_args &a = j.a;
-    const int wave = threadIdx.x >> 6;
-    const int64_t n = (int64_t)blockIdx.x * (4 / WAVES) + wave / WAVES;
-    if (n >= a.rows) return;  // (with four waves: all of the block)
-    const int lane = threadIdx.x & 63;
+    const int64_t n = (int64_t)blockIdx.x * (256 / LANES) + (LANES == 256 ? 0 : threadIdx.x / LANES);
+    const int lane = threadIdx.x % LANES;
+    if (n >= a.rows) return;  // (with 256 lanes: nobody; with 16: all of a row's)
     const Derived dv = derive(j.ns == 2 ? j.scales : nullptr);
     const uint32_t owner = (uint32_t)(n / 128);
     const int splits = j.few ? j.parts : (int)(j.pieces.last_block(owner) - j.pieces.first_block(owner)) + 1;
-    float m = -INFINITY;
-    for (int s = lane; s < splits; s += 64) m = fmaxf(m, j.pm[(int64_t)s * a.rows + n]);
-    m = wave_max(m);
-    float l = 0.0f;
-    for (int s = lane; s < splits; s += 64)
-        l += j.pl[(int64_t)s * a.rows + n] * exp2_fast((j.pm[(int64_t)s * a.rows + n] - m) * dv.c);
-    l = wave_sum(l);
-    const T *x = (const T *)a.hidden + n * a.hidden_stride;
     const int64_t t = target_of(a, n);
     const float g = t < 0 ? 0.0f : a.weights ? a.weights[n] : 1.0f;
+    const T *x = (const T *)a.hidden + n * a.hidden_stride;
     const T *wt = (const T *)a.table + (t < 0 ? 0 : t) * a.table_stride;
+    float m = -INFINITY, l = 0.0f, st = 0.0f;
+#pragma unroll 4
+    for (int s = lane; s < splits; s += LANES) m = fmaxf(m, j.pm[(int64_t)s * a.rows + n]);
+    if (t >= 0)
+        for (int c = lane; c < a.d; c += LANES) st = __builtin_fmaf((float)x[c], (float)wt[c], st);
+    m = row_max<LANES>(m, shared);
+#pragma unroll 4
+    for (int s = lane; s < splits; s += LANES)
+        l += j.pl[(int64_t)s * a.rows + n] * exp2_fast((j.pm[(int64_t)s * a.rows + n] - m) * dv.c);
+    l = row_sum<LANES>(l, shared);
+    st = row_sum<LANES>(st, shared);
     // l = sum without the target (times 2^7, about m).  With the target's score st and everything about the larger of the two:
     // 1 - p[target] = l / (l + e), loss = log1p(l / e): nothing is lost where p[target] is near 1.
-    float st = 0.0f, e = 0.0f, loss = 0.0f;
+    float e = 0.0f, loss = 0.0f;
     if (t >= 0) {
-        for (int c = lane; c < a.d; c += 64) st = __builtin_fmaf((float)x[c], (float)wt[c], st);
-        st = wave_sum(st);
         if (a.bias) st += a.bias[t];
         const float su = bias_units(st, dv);  // (not only a bias: any score)
         const float up = fmaxf(m, su);
         e = exp2_fast((su - up) * dv.c + P_SHIFT);
-        const float f = exp2_fast((m - up) * dv.c);
-        l *= f;
+        l *= exp2_fast((m - up) * dv.c);
         m = up;
         loss = st == -INFINITY ? INFINITY : l <= e ? log1pf(l / e) : ldexpf(m - su, -dv.k) + (logf(l + e) - P_SHIFT * LN2);
     }
@@ -968,31 +988,31 @@ __global__ __launch_bounds__(256) void join_rows_kernel(JoinArgs j)
     const float other = sum == 0.0f ? 1.0f : l / sum;  // 1 - p[target]
     const bool odd = j.ns == 2 && j.outlier[n];
     if (odd) {  // a row beyond x's scale: not finite, or without a target and far larger than the others
-        bool finite = true;
-        for (int c = lane; c < a.d; c += 64) finite &= fabsf((float)x[c]) < INFINITY;
+        float finite = 0.0f;
+        for (int c = lane; c < a.d; c += LANES) finite = fmaxf(finite, fabsf((float)x[c]) < INFINITY ? 0.0f : 1.0f);
         lse = NAN;
-        if (__all(finite)) {
-            float top = -INFINITY, sum = 0.0f;
-            for (int64_t v = lane; v < a.vocab; v += 64) {
+        if (row_max<LANES>(finite, shared) == 0.0f) {
+            float top = -INFINITY, mass = 0.0f;
+            for (int64_t v = lane; v < a.vocab; v += LANES) {
                 const float s = dot_lane(x, (const T *)a.table + v * a.table_stride, a.d) + (a.bias ? a.bias[v] : 0.0f);
                 const float up = fmaxf(top, s);
-                if (up > -INFINITY) sum = sum * expf(top - up) + expf(s - up);
+                if (up > -INFINITY) mass = mass * expf(top - up) + expf(s - up);
                 top = up;
             }
-            const float up = wave_max(top);
-            sum = wave_sum(top > -INFINITY ? sum * expf(top - up) : 0.0f);
-            lse = up + logf(sum);
+            const float up = row_max<LANES>(top, shared);
+            mass = row_sum<LANES>(top > -INFINITY ? mass * expf(top - up) : 0.0f, shared);
+            lse = up + logf(mass);
         }
     }
     if (odd && t >= 0) loss = NAN;
     loss = t < 0 ? 0.0f : g * loss;
-    if (lane == 0 && wave % WAVES == 0) {
+    if (lane == 0) {
         a.lse[n] = lse;
         a.loss[n] = loss;
     }
     if (!j.grad) return;
     const bool lost = odd && t >= 0;  // not finite: its gradients are not either
-    if (lane == 0 && wave % WAVES == 0) {
+    if (lane == 0) {
         const int shift = j.shifted == 2 ? 14 - j.scales->eg : j.shifted ? 14 : 0;
         const float gs = ldexpf(g, shift);
         j.row_target[n] = (int32_t)t;
@@ -1001,34 +1021,57 @@ __global__ __launch_bounds__(256) void join_rows_kernel(JoinArgs j)
         j.row_weight[n] = gs * other;
     }
     const int kw = j.ns == 2 ? j.scales->kw : 0;
-    for (int c0 = 0; c0 < a.d; c0 += 64) {
-        const int c = c0 + lane;
-        float o = 0.0f;
-        if (t >= 0 && c < a.d) {
+    // four columns per lane; with 256 lanes `groups` of them share a column's parts
+    const int columns = j.dp / 4, groups = LANES == 256 ? 256 / columns : 1, group = LANES == 256 ? lane / columns : 0;
+    const int c_first = LANES == 256 ? (lane - group * columns) * 4 : lane * 4;
+    for (int c = c_first; c < j.dp; c += (LANES == 256 ? columns : LANES) * 4) {
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (t >= 0 && c < a.d && group < groups) {
             const float *pm = j.pm + (int64_t)(c >> 8) * j.parts * a.rows;  // the maxima that chunk c / 256 went by
-#pragma unroll 8
-            for (int s = wave % WAVES; s < splits; s += WAVES) {
+#pragma unroll 4
+            for (int s = group; s < splits; s += groups) {
                 const int64_t at = (int64_t)s * a.rows + n;
-                o = __builtin_fmaf(j.po[at * j.dp + c], exp2_fast((pm[at] - m) * dv.c), o);
+                const float4 p = *(const float4 *)(j.po + at * j.dp + c);
+                const float f = exp2_fast((pm[at] - m) * dv.c);
+                o.x = __builtin_fmaf(p.x, f, o.x);
+                o.y = __builtin_fmaf(p.y, f, o.y);
+                o.z = __builtin_fmaf(p.z, f, o.z);
+                o.w = __builtin_fmaf(p.w, f, o.w);
             }
         }
-        if (WAVES > 1) {
+        if (LANES == 256) {
+            sums[lane] = o;
             __syncthreads();
-            shared[wave][lane] = o;
-            __syncthreads();
-            if (wave) continue;
-            o = shared[0][lane] + shared[1][lane] + shared[2][lane] + shared[3][lane];
+            if (group) break;
+            for (int q = 1; q < groups; ++q) {
+                const float4 p = sums[lane + q * columns];
+                o.x += p.x;
+                o.y += p.y;
+                o.z += p.z;
+                o.w += p.w;
+            }
         }
         if (c >= a.d) continue;
-        if (t >= 0) {
-            o = sum == 0.0f ? 0.0f : ldexpf(o / sum, -kw);
-            o = lost ? NAN : g * (o - other * (float)wt[c]);
+        const float ov[4] = {o.x, o.y, o.z, o.w};
+        Vec<T, 4> r;
+        T *to = (T *)a.d_hidden + n * a.d + c;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            float v = 0.0f;
+            if (t >= 0 && c + k < a.d) {
+                v = sum == 0.0f ? 0.0f : ldexpf(ov[k] / sum, -kw);
+                v = lost ? NAN : g * (v - other * (float)wt[c + k]);
+            }
+            r.v[k] = (T)v;
         }
-        ((T *)a.d_hidden)[n * a.d + c] = (T)o;
+        if (j.aligned) *(Vec<T, 4> *)to = r;
+        else
+            for (int k = 0; k < 4; ++k)
+                if (c + k < a.d) to[k] = r.v[k];
     }
 }
 
-// dw and db of the table rows that several blocks share, added in the order of the blocks: block (owner, 32 columns)
+// dw and db of the table rows that several blocks share, added in the order of the blocks: block (owner, 32 columns, 32 rows)
 template <typename T>
 __global__ __launch_bounds__(256) void join_table_kernel(SweepArgs a, int ns)
 {
@@ -1039,12 +1082,11 @@ __global__ __launch_bounds__(256) void join_table_kernel(SweepArgs a, int ns)
     const int64_t first = 2 * (int64_t)b0 + (a.pieces.begin(b0) > (uint64_t)owner * a.pieces.tiles ? 0 : 1);
     auto part = [&](uint32_t b) { return b == b0 ? first : 2 * (int64_t)b; };
     const int c = (int)blockIdx.y * 32 + (threadIdx.x & 7) * 4;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int r = q * 32 + (threadIdx.x >> 3);
-        const int64_t v = (int64_t)owner * 128 + r;
-        if (v >= a.vocab || c >= a.d) continue;
+    const int r = (int)blockIdx.z * 32 + (threadIdx.x >> 3);
+    const int64_t v = (int64_t)owner * 128 + r;
+    if (v < a.vocab && c < a.d) {
         float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
         for (uint32_t b = b0; b <= b1; ++b) {
             const float4 p = *(const float4 *)(a.pw + (part(b) * 128 + r) * a.dp + c);
             s.x += p.x;
@@ -1057,15 +1099,15 @@ __global__ __launch_bounds__(256) void join_table_kernel(SweepArgs a, int ns)
         Vec<T, 4> ov;
 #pragma unroll
         for (int j = 0; j < 4; ++j) ov.v[j] = (T)ldexpf(o[j], shift - kx);
-        if ((a.d & 3) == 0) *(Vec<T, 4> *)to = ov;
+        if (a.aligned) *(Vec<T, 4> *)to = ov;
         else
             for (int j = 0; j < 4; ++j)
                 if (c + j < a.d) to[j] = ov.v[j];
     }
-    if (a.db && blockIdx.y == 0 && threadIdx.x < 128 && (int64_t)owner * 128 + threadIdx.x < a.vocab) {
+    if (a.db && blockIdx.y == 0 && (threadIdx.x & 7) == 0 && v < a.vocab) {
         float t = 0.0f;
-        for (uint32_t b = b0; b <= b1; ++b) t += a.pb[part(b) * 128 + threadIdx.x];
-        a.db[(int64_t)owner * 128 + threadIdx.x] = ldexpf(t, shift);
+        for (uint32_t b = b0; b <= b1; ++b) t += a.pb[part(b) * 128 + r];
+        a.db[v] = ldexpf(t, shift);
     }
 }
 
@@ -1079,10 +1121,6 @@ __global__ __launch_bounds__(256) void clear_kernel(T *p, int64_t n, float *q, i
 
 // -------------------------------------------------------------------- host ---
 
-// the few-rows form is taken up to here (without the gradient)
-#ifndef FEW_ROWS_MOST
-#define FEW_ROWS_MOST 8
-#endif
 
 struct Plan {
     int dp, ns;
@@ -1119,7 +1157,7 @@ Plan plan_for(int64_t rows, int64_t vocab, int d, int dtype, bool grad)
     // as many blocks as run at once on the card's 256 compute units
     p.rows = pieces_for(rows, vocab, bv, 256 * (p.chunks > 1 ? 1 : waves_for(p.ns, w, grad)));
     p.few = 0;
-    if (!grad && rows <= FEW_ROWS_MOST) {
+    if (!grad && dtype == LFM_F32 && rows <= FEW) {
         const int64_t want = ceil_div(vocab, 16);  // (a block's lane groups have a few table rows each)
         p.few = (int)(want < 1024 ? want : 1024);
     }
@@ -1195,23 +1233,23 @@ hipError_t sweep_table(const SweepArgs &s, hipStream_t st)
     default: e = call(256, true); break;        \
     }
 
-template <typename T, int VEC>
+template <int VEC>
 hipError_t launch_few(const SweepArgs &w, const lfm_softmax_args &a, int blocks, hipStream_t st)
 {
     int ll = 0;
     while ((1 << ll) * VEC < a.d && ll < 6) ++ll;
-    if (a.rows == 1) few_rows_kernel<T, VEC, 1><<<dim3((unsigned)blocks), 256, 0, st>>>(w, (const T *)a.hidden, (const T *)a.table, ll);
-    else
-        few_rows_kernel<T, VEC, FEW><<<dim3((unsigned)blocks, (unsigned)ceil_div(a.rows, FEW)), 256, 0, st>>>(
-            w, (const T *)a.hidden, (const T *)a.table, ll);
+    const float *x = (const float *)a.hidden, *t = (const float *)a.table;
+    if (a.rows == 1) few_rows_kernel<VEC, 1><<<dim3((unsigned)blocks), 256, 0, st>>>(w, x, t, ll);
+    else few_rows_kernel<VEC, FEW><<<dim3((unsigned)blocks), 256, 0, st>>>(w, x, t, ll);
     return hipGetLastError();
 }
 
 template <typename T>
-hipError_t join_rows(const JoinArgs &j, int64_t parts, hipStream_t st)
+hipError_t join_rows(JoinArgs j, int64_t parts, hipStream_t st)
 {
-    if (parts > 8 && j.a.rows <= 4096) join_rows_kernel<T, 4><<<dim3((unsigned)j.a.rows), 256, 0, st>>>(j);
-    else join_rows_kernel<T, 1><<<dim3((unsigned)ceil_div(j.a.rows, 4)), 256, 0, st>>>(j);
+    j.aligned = j.a.d % 4 == 0 && ((uintptr_t)j.a.d_hidden & (4 * sizeof(T) - 1)) == 0;
+    if (j.a.rows <= 2048 && parts > 4) join_rows_kernel<T, 256><<<dim3((unsigned)j.a.rows), 256, 0, st>>>(j);
+    else join_rows_kernel<T, 16><<<dim3((unsigned)ceil_div(j.a.rows, 16)), 256, 0, st>>>(j);
     return hipGetLastError();
 }
 
@@ -1230,10 +1268,9 @@ hipError_t run(const lfm_softmax_args &a, bool grad, void *ws, hipStream_t st)
     const bool scales = NS == 2 || (a.dtype == LFM_F16 && a.weights && grad);
     auto in_place = [&](const void *q, int64_t stride) { return NS == 1 && a.d == p.dp && stride % 8 == 0 && ((uintptr_t)q & 15) == 0; };
     const bool x_there = in_place(a.hidden, a.hidden_stride), w_there = in_place(a.table, a.table_stride);
-    // both operands can be read 16 bytes at a time
-    const int whole = 16 / (int)sizeof(T);
-    const bool wide = a.d % whole == 0 && a.hidden_stride % whole == 0 && a.table_stride % whole == 0 &&
-                      (((uintptr_t)a.hidden | (uintptr_t)a.table) & 15) == 0;
+    // both operands can be read four elements at a time
+    const bool wide = a.d % 4 == 0 && a.hidden_stride % 4 == 0 && a.table_stride % 4 == 0 &&
+                      (((uintptr_t)a.hidden | (uintptr_t)a.table) & (4 * sizeof(T) - 1)) == 0;
     SweepArgs w = {};
     w.rows = a.rows;
     w.vocab = a.vocab;
@@ -1248,10 +1285,10 @@ hipError_t run(const lfm_softmax_args &a, bool grad, void *ws, hipStream_t st)
     j.grad = grad ? 1 : 0;
     j.pm = s.pm;
     j.pl = s.pl;
-    if (p.few) {
+    if (NS == 2 && p.few) {
         w.ldx = a.hidden_stride;
         w.ldw = a.table_stride;
-        e = wide ? launch_few<T, 16 / (int)sizeof(T)>(w, a, p.few, st) : launch_few<T, 1>(w, a, p.few, st);
+        e = wide ? launch_few<4>(w, a, p.few, st) : launch_few<1>(w, a, p.few, st);
         if (e != hipSuccess) return e;
         j.ns = 1;
         j.few = 1;
@@ -1298,6 +1335,7 @@ hipError_t run(const lfm_softmax_args &a, bool grad, void *ws, hipStream_t st)
     w.row_weight = s.row_weight;
     w.row_target = s.row_target;
     w.dw = a.d_table;
+    w.aligned = a.d % 4 == 0 && ((uintptr_t)a.d_table & (4 * sizeof(T) - 1)) == 0;
     w.db = a.d_bias;
     w.pw = s.pw;
     w.pb = s.pb;
@@ -1322,7 +1360,7 @@ hipError_t run(const lfm_softmax_args &a, bool grad, void *ws, hipStream_t st)
 #define TABLE(DP, WIDE) sweep_table<T, E, NS, DP, WIDE>(w, st)
     BY_WIDTH(p.dp, TABLE)
     if (e != hipSuccess || p.table.owners % p.table.blocks == 0) return e;  // (no block shares an owner)
-    join_table_kernel<T><<<dim3(p.table.owners, (unsigned)(p.dp / 32)), 256, 0, st>>>(w, NS);
+    join_table_kernel<T><<<dim3(p.table.owners, (unsigned)(p.dp / 32), 4), 256, 0, st>>>(w, NS);
     return hipGetLastError();
 }
 
