@@ -21,6 +21,7 @@ SOURCES = ["fit_kernels.hip", "fit_kernels_wide.hip", "warp_tile.hip", "warp_til
 # the device-memory operators: in liblfm_ops.so with their C ABI
 OPS_SOURCES = ["softmax_loss.hip", "embedding_ops.hip", "clip_norm.hip"]
 OPS_API = ["lfm_ops.hip"]
+TORCH_OPS = "torch_ops.cpp"  # their binding for torch tensors (host code)
 HEADERS = ["ops_common.hpp", os.path.join("..", "..", "include", "lfm_ops.h"), "device.hpp", "kernels.hpp", "pool.hpp", "warp_tile_kernel.hpp", "warp_tile_ahead.hpp", "warp_tile_narrow.hpp", "feat_kernel.hpp", os.path.join("..", "..", "include", "lfm_hip.h")]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
@@ -74,6 +75,17 @@ def build(force=False, verbose=False):
         run([HIPCC, "--offload-arch=gfx950", "-no-hip-rt", "-shared", "-fPIC", "-o", OPS_LIB] + mine
             + ["-Wl,--no-as-needed", stand_in])
         os.remove(stand_in)
+    binding, src = os.path.join(OUT_DIR, "_torch_ops.so"), os.path.join(CSRC, TORCH_OPS)
+    if force or _stale(binding, [src, OPS_LIB, hdrs[1]]):
+        import sysconfig
+
+        import torch
+        root = os.path.dirname(torch.__file__)
+        run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-w", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+             "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI), "-I" + os.path.join(root, "include"),
+             "-I" + os.path.join(os.path.dirname(os.path.dirname(HIPCC)), "include"), "-I" + sysconfig.get_paths()["include"],
+             src, "-o", binding, "-L" + OUT_DIR, "-l:liblfm_ops.so", "-L" + os.path.join(root, "lib"), "-ltorch_python",
+             "-ltorch_cpu", "-lc10", "-lc10_hip", "-Wl,-rpath,$ORIGIN"])
     return LIB
 
 

@@ -100,6 +100,8 @@ __global__ __launch_bounds__(256) void squares_kernel(Table t, double *partial)
     if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
 template <typename T>
 __device__ inline void piece_scale(const T *x, T *y, int64_t n, float f)
 {
@@ -117,7 +119,7 @@ __device__ inline void piece_scale(const T *x, T *y, int64_t n, float f)
             for (int q = 0; q < 4; ++q) {
 #pragma unroll
                 for (int k = 0; k < W; ++k) r[q].v[k] = (T)((float)r[q].v[k] * f);
-                ((V *)y)[i + q * 256] = r[q];
+                __builtin_nontemporal_store(*(u32x4 *)&r[q], (u32x4 *)y + i + q * 256);
             }
         }
         for (; i < words; i += 256) {
@@ -146,7 +148,9 @@ __global__ __launch_bounds__(256) void scale_kernel(Table t, const double *parti
     // a norm that is not finite (an element was not) scales nothing
     const float f = norm > max_norm && norm < HUGE_VAL ? (float)(max_norm / norm) : 1.0f;
     const int pieces = t.first_piece[t.tensors];
-    for (int p = blockIdx.x; p < pieces; p += gridDim.x) {
+    // from the last piece to the first: what the norm read last is still in the 256 MB cache
+    for (int back = blockIdx.x; back < pieces; back += gridDim.x) {
+        const int p = pieces - 1 - back;
         const int i = tensor_of(t, p);
         if (f == 1.0f && t.x[i] == t.out[i]) continue;
         const int64_t lo = (int64_t)(p - t.first_piece[i]) * PIECE;
@@ -183,7 +187,9 @@ hipError_t clip_global_norm(int64_t n_tensors, const void *const *x, void *const
     double *partial = (double *)ws;
     int64_t partials = 0;
     for (int phase = 0; phase < 2; ++phase) {
-        for (int64_t g = 0; g < n_tensors || g == 0; g += GROUP) {
+        const int64_t count = n_tensors < 1 ? 1 : ceil_div(n_tensors, GROUP);
+        for (int64_t q = 0; q < count; ++q) {
+            const int64_t g = (phase ? count - 1 - q : q) * GROUP;
             Table t;
             t.tensors = (int32_t)(n_tensors - g < GROUP ? n_tensors - g : GROUP);
             t.first_piece[0] = 0;

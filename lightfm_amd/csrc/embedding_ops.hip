@@ -27,41 +27,46 @@ __global__ __launch_bounds__(256) void lookup_kernel(lfm_lookup_args a, int lane
         lo = l < 0 ? 0 : (l > a.nnz ? a.nnz : l);
         hi = h > a.nnz ? a.nnz : h;
     }
-    for (int c = lane * VEC; c < a.d; c += lanes * VEC) {
+    const int base = (int)(threadIdx.x & 63) & ~(lanes - 1);  // the group's first lane in its wave
+    for (int c0 = 0; c0 < a.d; c0 += lanes * VEC) {
+        const int c = c0 + lane * VEC;
         float acc[VEC];
 #pragma unroll
         for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
-        int64_t j = lo;
-        if (BAGS) {
-            for (; j + 4 <= hi; j += 4) {  // four rows in flight
-                V r[4];
-                float w[4];
+        // a bag's ids are read `lanes` at a time and handed round, rows UP at a time: the loads do not wait for each other
+        constexpr int UP = BAGS ? 8 : 1;
+        for (int64_t j0 = lo; j0 < hi; j0 += lanes) {
+            int32_t mine = -1;
+            float weight = 0.0f;
+            if (j0 + lane < hi) {
+                const int64_t id = (int64_t)ids[j0 + lane];
+                if ((uint64_t)id < (uint64_t)a.vocab) {
+                    mine = (int32_t)id;
+                    weight = BAGS && a.values ? a.values[j0 + lane] : 1.0f;
+                }
+            }
+            const int count = hi - j0 < lanes ? (int)(hi - j0) : lanes;
+            for (int q0 = 0; q0 < count; q0 += UP) {
+                V r[UP];
+                float w[UP];
+                int32_t id[UP];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int64_t id = (int64_t)ids[j + q];
-                    const bool ok = (uint64_t)id < (uint64_t)a.vocab;
-                    w[q] = a.values ? a.values[j + q] : 1.0f;
-                    if (ok) r[q] = *(const V *)((const T *)a.table + id * a.table_stride + c);
-                    else {
-                        w[q] = 0.0f;
+                for (int q = 0; q < UP; ++q) {
+                    id[q] = __shfl(mine, base + (q0 + q < count ? q0 + q : 0));
+                    w[q] = __shfl(weight, base + (q0 + q < count ? q0 + q : 0));
+                    if (q0 + q >= count) id[q] = -1;
 #pragma unroll
-                        for (int k = 0; k < VEC; ++k) r[q].v[k] = (T)0.0f;
-                    }
+                    for (int k = 0; k < VEC; ++k) r[q].v[k] = (T)0.0f;
+                    if (id[q] >= 0 && c < a.d) r[q] = *(const V *)((const T *)a.table + id[q] * a.table_stride + c);
                 }
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
+                for (int q = 0; q < UP; ++q)
+                    if (id[q] >= 0)
 #pragma unroll
-                    for (int k = 0; k < VEC; ++k) acc[k] = fmaf(w[q], (float)r[q].v[k], acc[k]);
+                        for (int k = 0; k < VEC; ++k) acc[k] = fmaf(w[q], (float)r[q].v[k], acc[k]);
             }
         }
-        for (; j < hi; ++j) {
-            const int64_t id = (int64_t)ids[j];
-            if ((uint64_t)id >= (uint64_t)a.vocab) continue;
-            const float w = BAGS && a.values ? a.values[j] : 1.0f;
-            const V r = *(const V *)((const T *)a.table + id * a.table_stride + c);
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) acc[k] = fmaf(w, (float)r.v[k], acc[k]);
-        }
+        if (c >= a.d) continue;
         V o;
 #pragma unroll
         for (int k = 0; k < VEC; ++k) o.v[k] = (T)(acc[k] * a.scale);
@@ -130,7 +135,7 @@ SortPlan sort_plan(int64_t vocab, int64_t nnz)
     p.passes = (all + 10) / 11;
     p.bits = (all + p.passes - 1) / p.passes;
     p.bins = 1 << p.bits;
-    int64_t want = ceil_div(nnz, 4096);
+    int64_t want = ceil_div(nnz, 2048);
     if (want < 1) want = 1;
     if (want > MAX_BLOCKS) want = MAX_BLOCKS;
     p.items = ceil_div(ceil_div(nnz, want), SORT_THREADS) * SORT_THREADS;
@@ -186,7 +191,8 @@ __global__ __launch_bounds__(SORT_THREADS) void count_kernel(const I *ids, const
     for (int b = threadIdx.x; b < bins; b += SORT_THREADS) hist[(int64_t)blockIdx.x * bins + b] = count[b];
 }
 
-template <typename I, bool FIRST>
+// PER: neighbouring digits whose counts one thread adds up
+template <typename I, bool FIRST, int PER>
 __global__ __launch_bounds__(SORT_THREADS) void scatter_kernel(const I *ids, const uint32_t *keys, const uint32_t *pos,
                                                               int64_t n, int64_t vocab, int shift, int bits,
                                                               int64_t items, const uint32_t *hist, int blocks,
@@ -204,21 +210,22 @@ __global__ __launch_bounds__(SORT_THREADS) void scatter_kernel(const I *ids, con
         const uint32_t k = FIRST ? key_of(ids, j, vocab) : keys[j];
         atomicAdd(&count[wave][(k >> shift) & (uint32_t)(bins - 1)], 1u);
     }
-    // a thread's bins: `per` neighbouring ones
-    const int per = bins > SORT_THREADS ? bins / SORT_THREADS : 1;
-    uint32_t before[4] = {0, 0, 0, 0}, total[4] = {0, 0, 0, 0}, sum = 0;
-    const int first = threadIdx.x * per;
+    uint32_t before[PER], total[PER], sum = 0;
+#pragma unroll
+    for (int q = 0; q < PER; ++q) before[q] = total[q] = 0;
+    const int first = threadIdx.x * PER;
     if (first < bins) {
-        for (int b = 0; b < blocks; ++b)
+#pragma unroll 16
+        for (int b = 0; b < blocks; ++b) {
+            const Vec<uint32_t, PER> h = *(const Vec<uint32_t, PER> *)(hist + (int64_t)b * bins + first);
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (q < per) {
-                    const uint32_t h = hist[(int64_t)b * bins + first + q];
-                    total[q] += h;
-                    if (b < (int)blockIdx.x) before[q] += h;
-                }
+            for (int q = 0; q < PER; ++q) {
+                total[q] += h.v[q];
+                before[q] += b < (int)blockIdx.x ? h.v[q] : 0u;
+            }
+        }
 #pragma unroll
-        for (int q = 0; q < 4; ++q) sum += total[q];
+        for (int q = 0; q < PER; ++q) sum += total[q];
     }
     uint32_t scan = sum;  // inclusive scan over the threads
     for (int o = 1; o < 64; o <<= 1) {
@@ -231,16 +238,16 @@ __global__ __launch_bounds__(SORT_THREADS) void scatter_kernel(const I *ids, con
     for (int w = 0; w < wave; ++w) at += wave_sum[w];
     if (first < bins) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-            if (q < per) {
-                uint32_t next = at + before[q];
-                for (int w = 0; w < SORT_WAVES; ++w) {
-                    const uint32_t c = count[w][first + q];
-                    count[w][first + q] = next;
-                    next += c;
-                }
-                at += total[q];
+        for (int q = 0; q < PER; ++q) {
+            uint32_t next = at + before[q];
+#pragma unroll
+            for (int w = 0; w < SORT_WAVES; ++w) {
+                const uint32_t c = count[w][first + q];
+                count[w][first + q] = next;
+                next += c;
             }
+            at += total[q];
+        }
     }
     __syncthreads();
     for (int64_t j0 = lo; j0 < hi; j0 += 64) {
@@ -289,61 +296,73 @@ __device__ inline void store_row(const SumArgs &a, uint32_t key, int c, const fl
     *(Vec<T, VEC> *)((T *)a.out + (int64_t)key * a.d + c) = o;
 }
 
+// A block reads the ids, rows and values of its lane groups' chunks at once (they are pointers to pointers: position, bag,
+// row), then each group walks its own.
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void chunk_sum_kernel(SumArgs a, int lanes_log2)
 {
-    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t chunk = t >> lanes_log2, lo = chunk * CHUNK;
-    if (lo >= a.n) return;
-    const int lanes = 1 << lanes_log2, lane = (int)(t & (lanes - 1));
-    const int64_t hi = lo + CHUNK < a.n ? lo + CHUNK : a.n;
+    constexpr int MOST = 64 * CHUNK;  // 4 lanes to a group at least
+    __shared__ uint32_t keys[MOST + 1];
+    __shared__ int32_t rows[MOST];
+    __shared__ float values[MOST];
+    const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> lanes_log2, groups = 256 >> lanes_log2;
+    const int64_t first = (int64_t)blockIdx.x * groups * CHUNK;
     const uint32_t none = (uint32_t)a.vocab;
-    const uint32_t earlier = lo ? a.keys[lo - 1] : none, later = hi < a.n ? a.keys[hi] : none;
+    for (int i = threadIdx.x; i <= groups * CHUNK; i += 256) {
+        const int64_t j = first + i;
+        const uint32_t key = j < a.n ? a.keys[j] : none;
+        keys[i] = key;
+        if (i == groups * CHUNK) continue;
+        int32_t row = -1;
+        float value = 0.0f;
+        if (key != none) {
+            const uint32_t p = a.pos[j];
+            row = a.bag_of ? a.bag_of[p] : (int32_t)p;
+            if ((uint64_t)row < (uint64_t)a.rows) value = a.values ? a.values[p] : 1.0f;
+            else row = -1;
+        }
+        rows[i] = row;
+        values[i] = value;
+    }
+    __syncthreads();
+    const int lo = group * CHUNK;
+    const int64_t chunk = (int64_t)blockIdx.x * groups + group;
+    if (first + lo >= a.n) return;
+    const int hi = a.n - first < lo + CHUNK ? (int)(a.n - first) : lo + CHUNK;
+    const uint32_t earlier = lo ? keys[lo - 1] : first ? a.keys[first - 1] : none, later = keys[hi];
     typedef Vec<T, VEC> V;
     for (int c = lane * VEC; c < a.d; c += lanes * VEC) {
         float acc[VEC];
 #pragma unroll
         for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
-        uint32_t run = a.keys[lo];
-        bool began = lo == 0 || earlier != run;  // the run's first id is in this chunk
-        for (int64_t j0 = lo; j0 < hi; j0 += 8) {
+        uint32_t run = keys[lo];
+        bool began = earlier != run || (first == 0 && lo == 0);  // the run's first id is in this chunk
+        for (int j0 = lo; j0 < hi; j0 += 8) {
             V r[8];
-            float w[8];
-            uint32_t key[8];
-            const int m = hi - j0 < 8 ? (int)(hi - j0) : 8;
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
-                key[q] = none;
-                w[q] = 0.0f;
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) r[q].v[k] = (T)0.0f;
-                if (q < m) {
-                    key[q] = a.keys[j0 + q];
-                    const uint32_t p = a.pos[j0 + q];
-                    const int64_t row = a.bag_of ? (int64_t)a.bag_of[p] : (int64_t)p;
-                    if (key[q] != none && (uint64_t)row < (uint64_t)a.rows) {
-                        w[q] = a.values ? a.values[p] : 1.0f;
-                        r[q] = *(const V *)((const T *)a.d_out + row * a.stride + c);
-                    }
-                }
+                if (j0 + q < hi && rows[j0 + q] >= 0) r[q] = *(const V *)((const T *)a.d_out + rows[j0 + q] * a.stride + c);
             }
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
-                if (q >= m) break;
-                if (key[q] != run) {  // the run ends here
+                if (j0 + q >= hi) break;
+                if (keys[j0 + q] != run) {  // the run ends here
                     if (began) {
                         if (run != none) store_row<T, VEC>(a, run, c, acc);
                     } else {
 #pragma unroll
                         for (int k = 0; k < VEC; ++k) a.head[chunk * a.d + c + k] = acc[k];
                     }
-                    run = key[q];
+                    run = keys[j0 + q];
                     began = true;
 #pragma unroll
                     for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
                 }
+                if (rows[j0 + q] >= 0)
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) acc[k] = fmaf(w[q], (float)r[q].v[k], acc[k]);
+                    for (int k = 0; k < VEC; ++k) acc[k] = fmaf(values[j0 + q], (float)r[q].v[k], acc[k]);
             }
         }
         if (run == none) continue;
@@ -356,51 +375,72 @@ __global__ __launch_bounds__(256) void chunk_sum_kernel(SumArgs a, int lanes_log
     }
 }
 
-// One block per chunk; only those whose last run starts there and goes on have work: the run's chunks are shared by the
-// block's lane groups (contiguous shares), whose sums are added in order.
+// A run that goes on behind its first chunk: its parts are shared by a wave's lane groups, or by a block's where the run is
+// long (a popular id), and added in a fixed order.  A block looks at one chunk per wave.
+constexpr int LONG_RUN = 64;
+
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void join_kernel(SumArgs a, int lanes_log2)
 {
-    const int64_t chunk = blockIdx.x, end = (chunk + 1) * CHUNK;
-    if (end >= a.n) return;
-    const uint32_t key = a.keys[end - 1];
-    if (key == (uint32_t)a.vocab || a.keys[end] != key) return;
-    if (chunk && a.keys[end - CHUNK] == key && a.keys[end - CHUNK - 1] == key) return;  // began earlier
-    int64_t lo = end, hi = a.n;  // the first position behind the run
-    while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (a.keys[mid] <= key) lo = mid + 1;
-        else hi = mid;
-    }
-    const int64_t parts = (lo - 1) / CHUNK - chunk;  // the chunks behind this one that the run reaches
-    const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> lanes_log2,
-              groups = 256 >> lanes_log2;
     __shared__ float sums[256 * VEC];
-    const int64_t share = ceil_div(parts, groups);
-    const int64_t p0 = group * share < parts ? group * share : parts, p1 = p0 + share < parts ? p0 + share : parts;
-    for (int c0 = 0; c0 < a.d; c0 += lanes * VEC) {
-        const int c = c0 + lane * VEC;
-        float acc[VEC];
+    __shared__ int64_t parts_of[4];
+    const int wave = threadIdx.x >> 6, in_wave = threadIdx.x & 63;
+    const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1);
+    const int64_t chunk0 = (int64_t)blockIdx.x * 4;
+    // the parts behind a chunk whose last run starts there and goes on: chunks that begin with the run's id
+    int64_t parts = 0;
+    const int64_t end = (chunk0 + wave + 1) * CHUNK;
+    if (end < a.n) {
+        const uint32_t key = a.keys[end - 1];
+        const bool earlier = end > CHUNK && a.keys[end - CHUNK] == key && a.keys[end - CHUNK - 1] == key;
+        if (key != (uint32_t)a.vocab && !earlier)
+            for (int64_t p = 0;; p += 64) {
+                const int64_t at = end + (p + in_wave) * CHUNK;
+                const uint64_t same = __ballot(at < a.n && a.keys[at] == key);
+                parts += __popcll(same);
+                if (~same) break;
+            }
+    }
+    if (in_wave == 0) parts_of[wave] = parts;
+    __syncthreads();
+    for (int w = 0; w < 4; ++w) {
+        const int64_t n = parts_of[w], chunk = chunk0 + w;
+        const bool together = n > LONG_RUN;
+        if (n == 0 || (!together && w != wave)) continue;
+        const int groups = (together ? 256 : 64) >> lanes_log2, group = (together ? (int)threadIdx.x : in_wave) >> lanes_log2;
+        float *mine = sums + (together ? 0 : wave * 64 * VEC);
+        const uint32_t key = a.keys[(chunk + 1) * CHUNK];
+        const int64_t share = ceil_div(n, groups);
+        const int64_t p0 = group * share < n ? group * share : n, p1 = p0 + share < n ? p0 + share : n;
+        const int used = (int)ceil_div(n, share);
+        for (int c0 = 0; c0 < a.d; c0 += lanes * VEC) {
+            const int c = c0 + lane * VEC;
+            float acc[VEC];
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
-        if (c < a.d) {
-            for (int64_t p = p0; p < p1; ++p)
+            for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
+            if (c < a.d) {
+#pragma unroll 8
+                for (int64_t p = p0; p < p1; ++p) {
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) acc[k] += a.head[(chunk + 1 + p) * a.d + c + k];
+                    for (int k = 0; k < VEC; ++k) acc[k] += a.head[(chunk + 1 + p) * a.d + c + k];
+                }
+            }
+            if (together) __syncthreads();
+            else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) mine[(group * lanes + lane) * VEC + k] = acc[k];
+            if (together) __syncthreads();
+            else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            if (group == 0 && c < a.d) {
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) acc[k] = a.tail[chunk * a.d + c + k];
+                for (int g = 0; g < used; ++g)
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) acc[k] += mine[(g * lanes + lane) * VEC + k];
+                store_row<T, VEC>(a, key, c, acc);
+            }
         }
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) sums[threadIdx.x * VEC + k] = acc[k];
-        __syncthreads();
-        if (group == 0 && c < a.d) {
-            const int used = share ? (int)ceil_div(parts, share) : 0;
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) acc[k] = a.tail[chunk * a.d + c + k];
-            for (int g = 0; g < used; ++g)
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) acc[k] += sums[(g * lanes + lane) * VEC + k];
-            store_row<T, VEC>(a, key, c, acc);
-        }
-        __syncthreads();
+        if (together) __syncthreads();  // (a wave's own sums use the same places)
     }
 }
 
@@ -432,12 +472,13 @@ GradSpace grad_space(int64_t vocab, int64_t nnz, int d, bool bags, void *ws)
 template <typename T, int VEC>
 hipError_t launch_sums(const SumArgs &s, hipStream_t st)
 {
-    const int ll = lanes_for(s.d, VEC);
+    int ll = lanes_for(s.d, VEC);
+    if (ll < 2) ll = 2;
     const int64_t chunks = ceil_div(s.n, CHUNK);
-    chunk_sum_kernel<T, VEC><<<dim3((unsigned)ceil_div(chunks << ll, 256)), 256, 0, st>>>(s, ll);
+    chunk_sum_kernel<T, VEC><<<dim3((unsigned)ceil_div(chunks, 256 >> ll)), 256, 0, st>>>(s, ll);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || chunks < 2) return e;
-    join_kernel<T, VEC><<<dim3((unsigned)chunks), 256, 0, st>>>(s, ll);
+    join_kernel<T, VEC><<<dim3((unsigned)ceil_div(chunks, 4)), 256, 0, st>>>(s, ll);
     return hipGetLastError();
 }
 
@@ -478,12 +519,20 @@ hipError_t grad_typed(const lfm_lookup_args &a, void *ws, hipStream_t st)
                 nullptr);
         if ((e = hipGetLastError()) != hipSuccess) return e;
         if (a.nnz == 0) return hipSuccess;
-        if (pass == 0)
-            scatter_kernel<I, true><<<dim3((unsigned)p.blocks), SORT_THREADS, 0, st>>>(
-                ids, nullptr, nullptr, a.nnz, a.vocab, shift, p.bits, p.items, s.hist, p.blocks, s.keys[at], s.pos[at]);
-        else
-            scatter_kernel<I, false><<<dim3((unsigned)p.blocks), SORT_THREADS, 0, st>>>(
-                ids, keys, pos, a.nnz, a.vocab, shift, p.bits, p.items, s.hist, p.blocks, s.keys[at], s.pos[at]);
+        const int per = p.bins / SORT_THREADS;
+#define SCATTER(FIRST, PER)                                                                                               \
+    scatter_kernel<I, FIRST, PER><<<dim3((unsigned)p.blocks), SORT_THREADS, 0, st>>>(                                         \
+        ids, keys, pos, a.nnz, a.vocab, shift, p.bits, p.items, s.hist, p.blocks, s.keys[at], s.pos[at])
+        if (pass == 0) {
+            if (per <= 1) SCATTER(true, 1);
+            else if (per == 2) SCATTER(true, 2);
+            else SCATTER(true, 4);
+        } else {
+            if (per <= 1) SCATTER(false, 1);
+            else if (per == 2) SCATTER(false, 2);
+            else SCATTER(false, 4);
+        }
+#undef SCATTER
         if ((e = hipGetLastError()) != hipSuccess) return e;
         keys = s.keys[at];
         pos = s.pos[at];

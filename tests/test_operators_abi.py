@@ -10,6 +10,19 @@ import pytest
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
+class LfmSoftmaxArgs(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("hidden", "table", "targets", "bias", "weights", "loss", "lse", "d_hidden",
+                                           "d_table", "d_bias")]
+                + [(n, C.c_int64) for n in ("rows", "vocab", "hidden_stride", "table_stride")]
+                + [(n, C.c_int32) for n in ("d", "dtype", "id_bytes", "reserved")])
+
+
+class LfmLookupArgs(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("table", "ids", "indptr", "values", "out", "d_out")]
+                + [(n, C.c_int64) for n in ("rows", "vocab", "nnz", "table_stride", "d_out_stride")]
+                + [(n, C.c_int32) for n in ("d", "dtype", "id_bytes")] + [("scale", C.c_float)])
+
+
 @pytest.fixture(scope="module")
 def ops():
     from lightfm_amd import build
@@ -32,7 +45,7 @@ def test_library_exports_every_declared_symbol(ops):
 
 
 def test_struct_layouts_match_header(ops, tmp_path):
-    mirror = {"lfm_softmax_args": ops.LfmSoftmaxArgs, "lfm_lookup_args": ops.LfmLookupArgs}
+    mirror = {"lfm_softmax_args": LfmSoftmaxArgs, "lfm_lookup_args": LfmLookupArgs}
     lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "lfm_ops.h"', "int main(void) {"]
     for struct, t in mirror.items():
         lines.append('printf("%s %%zu\\n", sizeof(%s));' % (struct, struct))
@@ -57,7 +70,7 @@ def _softmax_args(ops, **kw):
                   d_table=fake, d_bias=None, rows=4, vocab=8, hidden_stride=16, table_stride=16, d=16, dtype=0,
                   id_bytes=4, reserved=0)
     values.update(kw)
-    return ops.LfmSoftmaxArgs(*[values[n] for n, _ in ops.LfmSoftmaxArgs._fields_])
+    return LfmSoftmaxArgs(*[values[n] for n, _ in LfmSoftmaxArgs._fields_])
 
 
 @pytest.mark.parametrize("wrong, code", [
@@ -102,7 +115,7 @@ def _lookup_args(ops, **kw):
     values = dict(table=fake, ids=fake, indptr=None, values=None, out=fake, d_out=fake, rows=4, vocab=8, nnz=4,
                   table_stride=16, d_out_stride=16, d=16, dtype=0, id_bytes=4, scale=1.0)
     values.update(kw)
-    return ops.LfmLookupArgs(*[values[n] for n, _ in ops.LfmLookupArgs._fields_])
+    return LfmLookupArgs(*[values[n] for n, _ in LfmLookupArgs._fields_])
 
 
 @pytest.mark.parametrize("wrong", [
