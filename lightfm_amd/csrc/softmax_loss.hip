@@ -64,6 +64,15 @@ __device__ inline float half_wave_sum(float v)
     return __uint_as_float(low) + __uint_as_float(high);
 }
 
+// in pairs: long sums of these are then as many times shorter
+__device__ inline float sum16(const float (&q)[16])
+{
+    float a[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a[j] = q[2 * j] + q[2 * j + 1];
+    return ((a[0] + a[1]) + (a[2] + a[3])) + ((a[4] + a[5]) + (a[6] + a[7]));
+}
+
 __device__ inline float exp2_fast(float v) { return __builtin_amdgcn_exp2f(v); }
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
@@ -420,10 +429,17 @@ __device__ inline void accumulate(f32x16 (&out)[DP / 32], const Values<E, NS> &p
 struct Pieces {
     uint32_t owners, tiles, blocks;  // owners * tiles units, dealt to `blocks` blocks
 
-    __host__ __device__ inline uint64_t begin(uint32_t block) const { return (uint64_t)owners * tiles * block / blocks; }
+    __host__ __device__ inline uint64_t begin(uint32_t block) const
+    {
+        const uint64_t units = (uint64_t)owners * tiles;
+        if ((units * (blocks + 1)) >> 32 == 0) return (uint32_t)(units * block) / blocks;
+        return units * block / blocks;
+    }
     __host__ __device__ inline uint32_t block_of(uint64_t unit) const
     {
-        return (uint32_t)(((unit + 1) * blocks - 1) / ((uint64_t)owners * tiles));
+        const uint64_t units = (uint64_t)owners * tiles, at = (unit + 1) * blocks - 1;
+        if ((units * blocks) >> 32 == 0) return (uint32_t)at / (uint32_t)units;  // (a 64-bit division takes microseconds)
+        return (uint32_t)(at / units);
     }
     __host__ __device__ inline uint32_t first_block(uint32_t owner) const { return block_of((uint64_t)owner * tiles); }
     __host__ __device__ inline uint32_t last_block(uint32_t owner) const { return block_of((uint64_t)owner * tiles + tiles - 1); }
@@ -579,10 +595,8 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, GRAD)) void rows_
                 }
                 float q[16];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    q[j] = exp2_fast(__builtin_fmaf(s[j], dv.c, base));
-                    l += q[j];
-                }
+                for (int j = 0; j < 16; ++j) q[j] = exp2_fast(__builtin_fmaf(s[j], dv.c, base));
+                l += sum16(q);
                 if (GRAD) {
                     Values<E, NS> p;
                     p.pack(q);
@@ -751,8 +765,7 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, true)) void table
                         for (int j = 0; j < 4; ++j) q[4 * g + j] = (hits >> (4 * h)) & (1u << (8 * g + j)) ? -ws[j] : q[4 * g + j];
                     }
                 }
-#pragma unroll
-                for (int j = 0; j < 16; ++j) db += q[j];
+                db += sum16(q);
                 Values<E, NS> p;
                 p.pack(q);
                 accumulate<E, NS, DP>(out, p, to);
