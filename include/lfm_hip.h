@@ -305,6 +305,23 @@ int lfm_session_download_shuffle(lfm_session *s, int32_t slot, int32_t *out, int
 int lfm_session_epoch(lfm_session *s, int32_t loss, int32_t slot, double item_alpha,
                       double user_alpha, int32_t k, int32_t n_positives, const uint32_t *seeds,
                       int32_t n_seeds, lfm_opts *opts);
+/* One epoch of the softmax loss: every positive interaction (Y > 0) against ALL items,
+ *   loss = weight * (log sum_v exp s(u, v) - s(u, i)),  s(u, v) = <user representation, item representation v> + item bias v
+ * (the user bias shifts every score of a user alike and is left as it is).  The shuffled positions are taken in batches;
+ * a batch's gradients are summed and one adagrad / adadelta step is made with them: there are no concurrent updates, the same input gives
+ * the same bits.  alpha adds alpha * (interactions of the batch) * W to a table's gradient, after the clipping.  Both feature
+ * matrices may be anything lfm_session_create takes.  No reference counterpart (its losses sample their negatives). */
+typedef struct lfm_softmax_epoch {
+    int32_t batch;        /* in: interactions per step; 0 = auto (interactions / 64, a multiple of 32, 256 ... 8192) */
+    float max_norm;       /* in: a batch's gradients are scaled down to this global norm; 0 = never, the norm is not computed */
+    double loss;          /* out: summed loss of the epoch, each batch before its step */
+    int64_t targets;      /* out: interactions that were trained on */
+    int32_t steps;        /* out */
+    float grad_norm;      /* out: global norm of the last batch's gradients before the clipping (max_norm > 0) */
+    float kernel_ms;      /* out: device time of the epoch */
+    int32_t reserved;
+} lfm_softmax_epoch;
+int lfm_session_epoch_softmax(lfm_session *s, int32_t slot, double item_alpha, double user_alpha, lfm_softmax_epoch *opts);
 /* 1 if every item/user embedding and bias is finite (LFM:447-464), else 0. */
 int lfm_session_check_finite(lfm_session *s);
 /* Pairwise predictions with the resident weights (ids are host arrays). */

@@ -56,6 +56,11 @@ class LfmOpts(C.Structure):
                 ("plan_flags", C.c_int32)]
 
 
+class LfmSoftmaxEpoch(C.Structure):
+    _fields_ = [("batch", C.c_int32), ("max_norm", C.c_float), ("loss", C.c_double), ("targets", C.c_int64),
+                ("steps", C.c_int32), ("grad_norm", C.c_float), ("kernel_ms", C.c_float), ("reserved", C.c_int32)]
+
+
 class LfmItemExport(C.Structure):
     """include/lfm_hip.h: lfm_item_export -- the HIP IPC handles of a session's item-side allocations."""
     _fields_ = [("handle", (C.c_char * 64) * 4), ("offset", C.c_int64 * 4), ("bytes", C.c_int64 * 4),
@@ -70,7 +75,7 @@ EXPORTS = (
     "lfm_predict", "lfm_predict_ranks", "lfm_auc_from_rank", "lfm_in_positives",
     "lfm_session_create", "lfm_session_create_scoring", "lfm_session_set_features", "lfm_session_set_interactions", "lfm_session_upload_shuffle",
     "lfm_session_device_shuffle", "lfm_session_device_shuffle_ahead", "lfm_shuffle_permutation", "lfm_session_download_shuffle",
-    "lfm_session_epoch", "lfm_session_check_finite", "lfm_session_predict",
+    "lfm_session_epoch", "lfm_session_epoch_softmax", "lfm_session_check_finite", "lfm_session_predict",
     "lfm_session_predict_ranks", "lfm_session_sync_to_host", "lfm_session_load_model",
     "lfm_session_build_positives", "lfm_session_download_positives", "lfm_session_representations",
     "lfm_session_destroy",

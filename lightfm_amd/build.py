@@ -17,8 +17,8 @@ OUT_DIR = os.path.join(HERE, "_lib")
 LIB = os.path.join(OUT_DIR, "liblfm_hip.so")
 OPS_LIB = os.path.join(OUT_DIR, "liblfm_ops.so")
 SOURCES = ["fit_kernels.hip", "fit_kernels_wide.hip", "warp_tile.hip", "warp_tile_lpr16.hip", "warp_tile_lpr32.hip",
-           "warp_tile_lpr64.hip", "warp_tile_ahead.hip", "warp_tile_bpr.hip", "logistic_tile.hip", "feat_kernels.hip", "feat_kernels_wide.hip", "feat_kernels_hot.hip", "feat_kernels_ada.hip", "hot_slices.hip", "predict_kernels.hip", "csr_build.hip", "session.hip"]
-# the device-memory operators: in liblfm_ops.so with their C ABI
+           "warp_tile_lpr64.hip", "warp_tile_ahead.hip", "warp_tile_bpr.hip", "logistic_tile.hip", "feat_kernels.hip", "feat_kernels_wide.hip", "feat_kernels_hot.hip", "feat_kernels_ada.hip", "hot_slices.hip", "predict_kernels.hip", "csr_build.hip", "softmax_epoch.hip", "session.hip"]
+# the device-memory operators: in liblfm_ops.so with their C ABI, in liblfm_hip.so for the softmax epochs
 OPS_SOURCES = ["softmax_loss.hip", "embedding_ops.hip", "clip_norm.hip"]
 OPS_API = ["lfm_ops.hip"]
 TORCH_OPS = "torch_ops.cpp"  # their binding for torch tensors (host code)
@@ -61,9 +61,9 @@ def build(force=False, verbose=False):
         subprocess.check_call(cmd)
     with ThreadPoolExecutor(max_workers=len(objs)) as ex:
         list(ex.map(run, jobs))
-    mine = [objs[s] for s in SOURCES]
+    mine = [objs[s] for s in SOURCES + OPS_SOURCES]
     if force or _stale(LIB, mine):
-        run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + mine + ["-ldl"])
+        run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-Wl,-Bsymbolic", "-o", LIB] + mine + ["-ldl"])
     mine = [objs[s] for s in OPS_SOURCES + OPS_API]
     if force or _stale(OPS_LIB, mine):
         # liblfm_ops.so works on torch's memory and streams, so it has to bind to the HIP runtime torch has loaded --
@@ -72,7 +72,7 @@ def build(force=False, verbose=False):
         stand_in = os.path.join(OUT_DIR, "link", "libamdhip64.so")
         os.makedirs(os.path.dirname(stand_in), exist_ok=True)
         run(["gcc", "-shared", "-fPIC", "-x", "c", os.devnull, "-Wl,-soname,libamdhip64.so", "-o", stand_in])
-        run([HIPCC, "--offload-arch=gfx950", "-no-hip-rt", "-shared", "-fPIC", "-o", OPS_LIB] + mine
+        run([HIPCC, "--offload-arch=gfx950", "-no-hip-rt", "-shared", "-fPIC", "-Wl,-Bsymbolic", "-o", OPS_LIB] + mine
             + ["-Wl,--no-as-needed", stand_in])
         os.remove(stand_in)
     binding, src = os.path.join(OUT_DIR, "_torch_ops.so"), os.path.join(CSRC, TORCH_OPS)

@@ -35,6 +35,34 @@ struct PredictArgs {
     int32_t tile_rows, tile_stride;
 };
 
+// softmax_epoch.hip
+struct SoftmaxBatch {
+    const int32_t *shuffle, *user_ids, *item_ids;
+    const float *Y, *weight;
+    int32_t *users, *targets;
+    float *weights;
+    unsigned long long *counters;
+    int64_t begin, n;
+    int32_t len;
+};
+struct SoftmaxTable {
+    float *W, *G, *M;
+    const float *g;   // summed gradients of the batch, shaped like W
+    int64_t cells;    // cells of W that g covers
+    float l2;         // alpha x interactions of the batch: the gradient of the L2 term is l2 * W
+};
+struct SoftmaxUpdate {
+    SoftmaxTable table[3];  // user embeddings, item embeddings, item biases
+    const float *norm;      // global norm of the gradients, or nullptr = not clipped
+    float max_norm, lr, rho, eps;
+    int32_t adadelta, len, items;
+    const float *loss;      // [len]
+    const int32_t *targets;
+    double *stats;          // [2] += summed loss, interactions that had a target
+};
+hipError_t launch_softmax_batch(const SoftmaxBatch &b, hipStream_t st);
+hipError_t launch_softmax_update(const SoftmaxUpdate &u, int cus, hipStream_t st);
+
 struct RanksArgs {
     const float *user_rep;  // [n_test_users_rows, rs] dense representations (bias at [d])
     const float *item_rep;  // [rs, n_items] component-major (coalesced across items)

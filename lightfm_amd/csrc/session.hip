@@ -24,6 +24,7 @@
 #include "../../include/lfm_hip.h"
 #include "device.hpp"
 #include "kernels.hpp"
+#include "ops_common.hpp"
 #include "pool.hpp"
 
 using namespace lfm;
@@ -3046,6 +3047,219 @@ extern "C" int lfm_session_epoch(lfm_session *s, int32_t loss, int32_t slot, dou
     if (c[FAULT_SLOT])  // device.hpp: guard_row
         return fail(LFM_ECORRUPT, "a shuffle entry outside [0, n) was read on the device: the shuffle slot is not a permutation "
                                   "(lfm_session_upload_shuffle input) or device memory is corrupted; the epoch's updates are unreliable");
+    return LFM_OK;
+}
+
+// The softmax loss (include/lfm_hip.h): the operators of ops_common.hpp on the session's tables and stream, a batch at a time.
+//   representations   embedding_lookup over the feature matrices (identity features: the tables themselves)
+//   loss, gradients   softmax_loss of the batch's users against all items
+//   tables' gradients embedding_grad of the same lookups: sorted sums, dense -- the item side has a gradient in every row anyway
+//   clipping          clip_global_norm's norm; the factor is applied by the update, which reads the gradients in any case
+extern "C" int lfm_session_epoch_softmax(lfm_session *s, int32_t slot, double item_alpha, double user_alpha, lfm_softmax_epoch *opts)
+{
+    if (!s || !opts) return fail(LFM_EINVAL, "null pointer");
+    if (s->scoring_only) return fail(LFM_EINVAL, "a scoring session (lfm_session_create_scoring) cannot train");
+    if (s->shards.n > 0 || s->share) return fail(LFM_EUNSUPPORTED, "the softmax loss needs the whole item tables in the session: they are owner-sharded");
+    if (s->comm) return fail(LFM_EUNSUPPORTED, "the softmax loss trains on one device");
+    if (slot < 0 || slot >= (int)s->shuffles.size() || s->shuffles[slot]->n != (size_t)s->n)
+        return fail(LFM_EINVAL, "shuffle slot not uploaded");
+    if (s->n && (!s->item_ids.p || !s->Y.p)) return fail(LFM_EINVAL, "item_ids / Y not uploaded");
+    if (s->n && !s->weight_aliases_Y && !s->weight.p) return fail(LFM_EINVAL, "sample_weight not uploaded");
+    if (opts->batch < 0 || opts->batch > (1 << 20)) return fail(LFM_EINVAL, "batch must lie in [0, 2^20]");
+    if (!(opts->max_norm >= 0.0f)) return fail(LFM_EINVAL, "max_norm must not be negative");
+    if (!(item_alpha >= 0.0) || !(user_alpha >= 0.0)) return fail(LFM_EINVAL, "alpha must not be negative");
+    opts->loss = 0.0;
+    opts->targets = 0;
+    opts->steps = 0;
+    opts->grad_norm = opts->kernel_ms = 0.0f;
+    if (!s->n) return LFM_OK;
+    if (s->itf.rows < 1) return fail(LFM_EINVAL, "the model has no items");
+    if (std::max(s->itf.nnz, s->usf.nnz) > INT32_MAX - 4096) return fail(LFM_EUNSUPPORTED, "a feature matrix with 2^31 - 4096 entries or more");
+    HIP_TRY(hipSetDevice(s->device));
+    if (s->stream2) (void)hipStreamSynchronize(s->stream2);  // (left running only by an epoch that failed half-way)
+    if (s->pairs_live) LFM_TRY(bias_pairs_unpack(s, s->stream));
+    if (s->rows_live) LFM_TRY(row_pairs_unpack(s, s->stream));
+    if (slot < (int)s->shuffle_ready.size() && s->shuffle_ready[slot])
+        HIP_TRY(hipStreamWaitEvent(s->stream, s->shuffle_ready[slot], 0));
+
+    const int64_t n = s->n, items = s->itf.rows, users = s->usf.rows;
+    const int d = s->d;  // padded components are zeros: their products and gradients vanish
+    const bool item_ids_only = s->itf.identity, user_ids_only = s->usf.identity;
+    int64_t batch = opts->batch ? opts->batch : std::min<int64_t>(8192, std::max<int64_t>(256, n / 64 / 32 * 32));
+    batch = std::max<int64_t>(1, std::min(batch, n));
+    const int64_t item_rows = item_ids_only ? items : s->n_feat[0], user_rows = user_ids_only ? users : s->n_feat[1];
+
+    DBuf<int32_t> b_users, b_targets;
+    DBuf<float> b_weights, loss, lse, hidden, d_hidden, user_rep, d_user_rep, item_rep, item_bias, d_item_rep, d_item_bias;
+    DBuf<float> dW_user, dW_item, db_item, norm;
+    DBuf<double> stats;
+    DBuf<char> ws;
+    DrainOnExit drain{s->stream};
+    LFM_TRY(b_users.alloc(batch));
+    LFM_TRY(b_targets.alloc(batch));
+    LFM_TRY(b_weights.alloc(batch));
+    LFM_TRY(loss.alloc(batch));
+    LFM_TRY(lse.alloc(batch));
+    LFM_TRY(hidden.alloc((size_t)batch * d));
+    LFM_TRY(d_hidden.alloc((size_t)batch * d));
+    LFM_TRY(dW_user.alloc((size_t)user_rows * d));
+    LFM_TRY(dW_item.alloc((size_t)item_rows * d));
+    LFM_TRY(db_item.alloc(item_rows));
+    LFM_TRY(norm.alloc(1));
+    LFM_TRY(stats.alloc(2));
+    if (!user_ids_only) {
+        LFM_TRY(user_rep.alloc((size_t)users * d));
+        LFM_TRY(d_user_rep.alloc((size_t)users * d));
+    }
+    if (!item_ids_only) {
+        LFM_TRY(item_rep.alloc((size_t)items * d));
+        LFM_TRY(item_bias.alloc(items));
+        LFM_TRY(d_item_rep.alloc((size_t)items * d));
+        LFM_TRY(d_item_bias.alloc(items));
+    }
+
+    // the representations of one side: bags of its feature matrix
+    auto features = [&](const DevCsr &f, int side, int width) {
+        lfm_lookup_args a = {};
+        a.ids = f.indices.p;
+        a.indptr = f.indptr.p;
+        a.values = f.data.p;
+        a.rows = f.rows;
+        a.vocab = s->n_feat[side];
+        a.nnz = f.nnz;
+        a.d = width;
+        a.table_stride = a.d_out_stride = width;
+        a.dtype = LFM_F32;
+        a.id_bytes = 4;
+        a.scale = 1.0f;
+        return a;
+    };
+    auto user_bags = features(s->usf, 1, d), item_bags = features(s->itf, 0, d), bias_bags = features(s->itf, 0, 1);
+    user_bags.table = s->tab[1][0].p;
+    user_bags.out = user_rep.p;
+    item_bags.table = s->tab[0][0].p;
+    item_bags.out = item_rep.p;
+    bias_bags.table = s->tab[0][3].p;
+    bias_bags.out = item_bias.p;
+    lfm_lookup_args pick = {};  // the batch's users
+    pick.table = user_ids_only ? s->tab[1][0].p : user_rep.p;
+    pick.ids = b_users.p;
+    pick.out = hidden.p;
+    pick.vocab = users;
+    pick.d = d;
+    pick.table_stride = pick.d_out_stride = d;
+    pick.dtype = LFM_F32;
+    pick.id_bytes = 4;
+    pick.scale = 1.0f;
+    lfm_softmax_args sm = {};
+    sm.hidden = hidden.p;
+    sm.table = item_ids_only ? s->tab[0][0].p : item_rep.p;
+    sm.targets = b_targets.p;
+    sm.bias = item_ids_only ? s->tab[0][3].p : item_bias.p;
+    sm.weights = b_weights.p;
+    sm.loss = loss.p;
+    sm.lse = lse.p;
+    sm.d_hidden = d_hidden.p;
+    sm.d_table = item_ids_only ? dW_item.p : d_item_rep.p;
+    sm.d_bias = item_ids_only ? db_item.p : d_item_bias.p;
+    sm.vocab = items;
+    sm.hidden_stride = sm.table_stride = d;
+    sm.d = d;
+    sm.dtype = LFM_F32;
+    sm.id_bytes = 4;
+    const void *grads[3] = {dW_user.p, dW_item.p, db_item.p};
+    const int64_t counts[3] = {user_rows * d, item_rows * d, item_rows};
+    const int32_t types[3] = {LFM_F32, LFM_F32, LFM_F32};
+
+    int64_t need = ops::clip_workspace(3, counts);
+    for (int64_t rows : {batch, n % batch}) {
+        if (!rows) continue;
+        need = std::max(need, ops::softmax_workspace(rows, items, d, LFM_F32, true));
+        need = std::max(need, ops::embedding_grad_workspace(rows, users, rows, d, false));
+    }
+    if (!user_ids_only) need = std::max(need, ops::embedding_grad_workspace(users, s->n_feat[1], s->usf.nnz, d, true));
+    if (!item_ids_only) {
+        need = std::max(need, ops::embedding_grad_workspace(items, s->n_feat[0], s->itf.nnz, d, true));
+        need = std::max(need, ops::embedding_grad_workspace(items, s->n_feat[0], s->itf.nnz, 1, true));
+    }
+    LFM_TRY(ws.alloc((size_t)need));
+
+    SoftmaxBatch gather = {s->shuffles[slot]->p, s->user_ids.p, s->item_ids.p, s->Y.p, s->weight_aliases_Y ? s->Y.p : s->weight.p,
+                           b_users.p, b_targets.p, b_weights.p, s->counters.p, 0, n, 0};
+    SoftmaxUpdate update = {};
+    update.table[0] = {s->tab[1][0].p, s->tab[1][1].p, s->tab[1][2].p, dW_user.p, counts[0], 0.0f};
+    update.table[1] = {s->tab[0][0].p, s->tab[0][1].p, s->tab[0][2].p, dW_item.p, counts[1], 0.0f};
+    update.table[2] = {s->tab[0][3].p, s->tab[0][4].p, s->tab[0][5].p, db_item.p, counts[2], 0.0f};
+    update.norm = opts->max_norm > 0.0f ? norm.p : nullptr;
+    update.max_norm = opts->max_norm;
+    update.lr = s->lr;
+    update.rho = s->rho;
+    update.eps = s->eps;
+    update.adadelta = s->adadelta;
+    update.items = (int32_t)items;
+    update.loss = loss.p;
+    update.targets = b_targets.p;
+    update.stats = stats.p;
+
+    HIP_TRY(hipMemsetAsync(s->counters.p, 0, 13 * sizeof(unsigned long long), s->stream));
+    HIP_TRY(hipMemsetAsync(stats.p, 0, 2 * sizeof(double), s->stream));
+    HIP_TRY(hipMemsetAsync(norm.p, 0, sizeof(float), s->stream));
+    HIP_TRY(hipEventRecord(s->ev0, s->stream));
+    int32_t steps = 0;
+    for (int64_t begin = 0; begin < n; begin += batch, ++steps) {
+        const int64_t rows = std::min(batch, n - begin);
+        gather.begin = begin;
+        gather.len = update.len = (int32_t)rows;
+        pick.rows = pick.nnz = sm.rows = rows;
+        HIP_TRY(launch_softmax_batch(gather, s->stream));
+        if (!user_ids_only) HIP_TRY(ops::embedding_lookup(user_bags, s->stream));
+        if (!item_ids_only) {
+            HIP_TRY(ops::embedding_lookup(item_bags, s->stream));
+            HIP_TRY(ops::embedding_lookup(bias_bags, s->stream));
+        }
+        HIP_TRY(ops::embedding_lookup(pick, s->stream));
+        HIP_TRY(ops::softmax_loss(sm, true, ws.p, s->stream));
+        lfm_lookup_args back = pick;
+        back.d_out = d_hidden.p;
+        back.out = user_ids_only ? dW_user.p : d_user_rep.p;
+        HIP_TRY(ops::embedding_grad(back, ws.p, s->stream));
+        if (!user_ids_only) {
+            back = user_bags;
+            back.d_out = d_user_rep.p;
+            back.out = dW_user.p;
+            HIP_TRY(ops::embedding_grad(back, ws.p, s->stream));
+        }
+        if (!item_ids_only) {
+            back = item_bags;
+            back.d_out = d_item_rep.p;
+            back.out = dW_item.p;
+            HIP_TRY(ops::embedding_grad(back, ws.p, s->stream));
+            back = bias_bags;
+            back.d_out = d_item_bias.p;
+            back.out = db_item.p;
+            HIP_TRY(ops::embedding_grad(back, ws.p, s->stream));
+        }
+        if (update.norm)
+            HIP_TRY(ops::clip_global_norm(3, grads, nullptr, counts, types, opts->max_norm, norm.p, ws.p, s->stream));
+        update.table[0].l2 = (float)(user_alpha * (double)rows);
+        update.table[1].l2 = update.table[2].l2 = (float)(item_alpha * (double)rows);
+        HIP_TRY(launch_softmax_update(update, s->cus, s->stream));
+    }
+    HIP_TRY(hipEventRecord(s->ev1, s->stream));
+    HIP_TRY(hipStreamSynchronize(s->stream));
+    HIP_TRY(hipEventElapsedTime(&opts->kernel_ms, s->ev0, s->ev1));
+    double sums[2];
+    LFM_TRY(stats.download(sums));
+    LFM_TRY(norm.download(&opts->grad_norm));
+    opts->loss = sums[0];
+    opts->targets = (int64_t)sums[1];
+    opts->steps = steps;
+    unsigned long long c[13];
+    LFM_TRY(s->counters.download(c));
+    ++s->epochs_run;
+    if (c[FAULT_SLOT])
+        return fail(LFM_ECORRUPT, "a shuffle entry outside [0, n) was read on the device: the shuffle slot is not a permutation; "
+                                  "the epoch's updates are unreliable");
     return LFM_OK;
 }
 

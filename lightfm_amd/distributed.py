@@ -221,6 +221,8 @@ class DistributedFit(object):
         self.host_shuffle = host_shuffle
         if item_tables not in ("replicated", "owner"):
             raise ValueError("item_tables must be 'replicated' or 'owner'")
+        if model.loss == "softmax":
+            raise NotImplementedError("the softmax loss trains on one device (LightFM.fit)")
         self.owner_sharded = item_tables == "owner" and world > 1
         if self.owner_sharded and (item_features is not None or user_features is not None or model.loss != "warp"
                                    or model.learning_schedule != "adagrad" or model.item_alpha or model.user_alpha

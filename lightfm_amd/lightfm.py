@@ -159,6 +159,15 @@ class _Session(object):
             C.c_int32(k), C.c_int32(n), N.u32p(seeds), 0 if seeds is None else len(seeds),
             C.byref(opts)))
 
+    def epoch_softmax(self, item_alpha, user_alpha, slot=0):
+        """One epoch of the softmax loss (lfm_session_epoch_softmax) with options.softmax_batch / softmax_max_norm;
+        returns what it did as a dict: kernel_ms, loss (mean per target), targets, steps, grad_norm."""
+        o = N.LfmSoftmaxEpoch(batch=int(options.softmax_batch), max_norm=float(options.softmax_max_norm))
+        N.check(N.lib().lfm_session_epoch_softmax(self.handle, slot, C.c_double(item_alpha), C.c_double(user_alpha),
+                                                  C.byref(o)))
+        return {"kernel_ms": float(o.kernel_ms), "loss": float(o.loss) / max(1, int(o.targets)),
+                "targets": int(o.targets), "steps": int(o.steps), "grad_norm": float(o.grad_norm)}
+
     def check_finite(self):
         return bool(N.check(N.lib().lfm_session_check_finite(self.handle)))
 
@@ -294,6 +303,12 @@ class LightFM(object):
     Parameters are those of the reference: no_components, k, n, learning_schedule
     ('adagrad' | 'adadelta'), loss ('logistic' | 'bpr' | 'warp' | 'warp-kos'),
     learning_rate, rho, epsilon, item_alpha, user_alpha, max_sampled, random_state.
+
+    One loss more than the reference's: 'softmax', the cross entropy of every positive interaction
+    against ALL items instead of sampled negatives.  It trains in batches, one optimizer step each
+    (options.softmax_batch, options.softmax_max_norm; include/lfm_hip.h: lfm_session_epoch_softmax),
+    so the same random_state gives the same model bit for bit; k, n, max_sampled and num_threads have
+    no meaning for it, and user biases keep their initial zeros (they shift all scores of a user alike).
     """
 
     def __init__(self, no_components=10, k=5, n=10, learning_schedule="adagrad", loss="logistic",
@@ -308,7 +323,7 @@ class LightFM(object):
         assert 0 < rho < 1
         assert epsilon >= 0
         assert learning_schedule in ("adagrad", "adadelta")
-        assert loss in ("logistic", "warp", "bpr", "warp-kos")
+        assert loss in ("logistic", "warp", "bpr", "warp-kos", "softmax")
         if max_sampled < 1:
             raise ValueError("max_sampled must be a positive integer")
 
@@ -675,7 +690,7 @@ class LightFM(object):
                     self.random_state.shuffle(shuffle_indices)
                     session.upload_shuffle(shuffle_indices)
                 seeds = None
-                if loss != "logistic":  # _lightfm_fast.pyx.template:812-814
+                if loss not in ("logistic", "softmax"):  # _lightfm_fast.pyx.template:812-814
                     seeds = np.ascontiguousarray(self.random_state.randint(
                         0, np.iinfo(np.int32).max, size=num_threads).astype(np.uint32))
                 next_keys = None
@@ -684,20 +699,24 @@ class LightFM(object):
                     # trains (the draws keep their order: keys, seeds, keys, seeds, ...)
                     next_keys = self.random_state.randint(0, np.iinfo(np.int32).max, size=624)
                     session.device_shuffle_ahead(int(next_keys[0]), int(next_keys[1]), slot=1 - slot)
-                opts, _ = make_opts()
-                opts.history = int(getattr(self, "_trained_interactions", 0))
-                session.epoch(loss, self.item_alpha, self.user_alpha, self.k, self.n, seeds, opts, slot=slot)
+                if loss == "softmax":
+                    stats = session.epoch_softmax(self.item_alpha, self.user_alpha, slot=slot)
+                else:
+                    opts, _ = make_opts()
+                    opts.history = int(getattr(self, "_trained_interactions", 0))
+                    session.epoch(loss, self.item_alpha, self.user_alpha, self.k, self.n, seeds, opts, slot=slot)
+                    stats = {"kernel_ms": float(opts.kernel_ms),
+                             "counters": list(opts.counters),
+                             "kernel_used": int(opts.kernel_used),
+                             "tile_ng": int(opts.tile_ng),
+                             "in_flight": int(opts.in_flight),
+                             "launches": int(opts.launches),
+                             "user_store": int(opts.user_store),
+                             "plan_flags": int(opts.plan_flags)}
                 if next_keys is not None:
                     slot = 1 - slot
                 self._trained_interactions = getattr(self, "_trained_interactions", 0) + n
-                self._last_epoch_stats.append({"kernel_ms": float(opts.kernel_ms),
-                                               "counters": list(opts.counters),
-                                               "kernel_used": int(opts.kernel_used),
-                                               "tile_ng": int(opts.tile_ng),
-                                               "in_flight": int(opts.in_flight),
-                                               "launches": int(opts.launches),
-                                               "user_store": int(opts.user_store),
-                                               "plan_flags": int(opts.plan_flags)})
+                self._last_epoch_stats.append(stats)
                 if not session.check_finite():  # LFM:664
                     session.sync_to_host(model)
                     raise ValueError(_NOT_FINITE)

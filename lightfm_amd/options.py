@@ -40,11 +40,14 @@ shuffle_ahead      with device_shuffle: the permutation of epoch e + 1 is writte
 trim_after_fit     True: LightFM.fit_partial hands the device memory its session used back to the HIP runtime when it returns
                    (lfm_device_trim; for processes that share the GPU with other code).  Off by default: the pool that keeps
                    released blocks is what fixed the stale-memory fault of round 2, and the next fit reuses them.
+softmax_batch      LightFM(loss="softmax"): interactions per optimizer step; 0 (default) = a 64th of the interactions, a
+                   multiple of 32 between 256 and 8192.
+softmax_max_norm   ... the global norm that a batch's gradients are scaled down to; 0 = no clipping.
 host_positives     True: the positives lookup is built on the host (interactions.tocsr(), LFM:365-372)
                    and uploaded; False (default): built on the device from the uploaded COO.
 
 Environment: LIGHTFM_AMD_MODE, _LAUNCHES, _FIRST_BATCH, _MAX_WAVES, _RAMP_K, _UPDATE_MODE,
-_WARP_KERNEL, _FEAT_KERNEL, _DEBUG, _DEVICE_SHUFFLE, _DEVICE; LIGHTFM_AMD_TABLE_ALLOC / _TABLE_ALLOC_MASK select the
+_WARP_KERNEL, _FEAT_KERNEL, _DEBUG, _DEVICE_SHUFFLE, _DEVICE, _SOFTMAX_BATCH, _SOFTMAX_MAX_NORM; LIGHTFM_AMD_TABLE_ALLOC / _TABLE_ALLOC_MASK select the
 allocation flavour of the weight tables (csrc/session.hip).
 """
 import os
@@ -69,6 +72,8 @@ class _Options(object):
         self.shuffle_ahead = os.environ.get("LIGHTFM_AMD_SHUFFLE_AHEAD", "0") != "0"
         self.trim_after_fit = os.environ.get("LIGHTFM_AMD_TRIM_AFTER_FIT", "0") != "0"
         self.cache_scoring_session = os.environ.get("LIGHTFM_AMD_CACHE_SCORING", "1") != "0"
+        self.softmax_batch = int(os.environ.get("LIGHTFM_AMD_SOFTMAX_BATCH", "0"))
+        self.softmax_max_norm = float(os.environ.get("LIGHTFM_AMD_SOFTMAX_MAX_NORM", "0"))
         self.log_samples = False
         self.last_counters = None
         self.last_kernel_ms = None
