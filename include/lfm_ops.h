@@ -39,7 +39,10 @@ const char *lfm_ops_last_error(void);
  *   q[n, v] = weights[n] * (exp(s[n, v] - lse[n]) - [v == targets[n]])     (0 for a row without a target),
  *   d_hidden = q table,  d_table = q^T hidden,  d_bias[v] = sum_n q[n, v].
  * The logits are never written to memory.  bias / weights may be NULL (0 / 1); d_bias may be NULL.  A bias of -inf
- * removes an item.  Rows of hidden and table are contiguous, `*_stride` elements apart; the gradients are dense. */
+ * removes an item: its row of the table is not looked at, whatever it holds, and has a zero gradient (as a target, its loss is
+ * infinite).  Rows of hidden and table are contiguous, `*_stride` elements apart; the gradients are dense.
+ * float32 operands keep 22 bits and a floor of 2^-39 of the largest magnitude of hidden (rows with a target) or table (items not
+ * removed).  At most 2^27 rows and 2^30 items. */
 typedef struct lfm_softmax_args {
     const void *hidden, *table; /* [rows, d], [vocab, d] of `dtype` */
     const void *targets;        /* [rows] int32 or int64 */
@@ -81,8 +84,8 @@ int lfm_ops_embedding_grad_workspace(int64_t rows, int64_t vocab, int64_t nnz, i
 int lfm_ops_embedding_lookup_grad(const lfm_lookup_args *args, void *workspace, int64_t workspace_bytes, void *stream);
 
 /* norm = sqrt(sum of squares over all tensors), summed in float64; out[i] = x[i] * min(1, max_norm / norm).
- * `x`, `out`, `counts`, `dtypes` are HOST arrays of n_tensors entries; out[i] may be x[i]; out NULL computes the
- * norm alone.  A norm that is not finite is reported in `norm` and leaves the values unscaled. */
+ * `x`, `out`, `counts`, `dtypes` are HOST arrays of n_tensors entries; out[i] may be x[i] and overlaps nothing else (a
+ * tensor that is listed twice cannot be scaled: LFM_EINVAL); out NULL computes the norm alone.  A norm that is not finite is reported in `norm` and leaves the values unscaled. */
 int lfm_ops_clip_workspace(int64_t n_tensors, const int64_t *counts, int64_t *bytes);
 int lfm_ops_clip_global_norm(int64_t n_tensors, const void *const *x, void *const *out, const int64_t *counts,
                              const int32_t *dtypes, double max_norm, float *norm, void *workspace,

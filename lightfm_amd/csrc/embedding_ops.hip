@@ -15,7 +15,7 @@ namespace {
 template <typename T, typename I, int VEC, bool BAGS>
 __global__ __launch_bounds__(256) void lookup_kernel(lfm_lookup_args a, int lanes_log2)
 {
-    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t t = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x;
     const int64_t row = t >> lanes_log2;
     if (row >= a.rows) return;
     const int lanes = 1 << lanes_log2, lane = (int)(t & (lanes - 1));
@@ -90,9 +90,10 @@ template <typename T, typename I, int VEC>
 hipError_t launch_lookup(const lfm_lookup_args &a, hipStream_t st)
 {
     const int ll = lanes_for(a.d, VEC);
-    const int64_t blocks = ceil_div(a.rows << ll, 256);
-    if (a.indptr) lookup_kernel<T, I, VEC, true><<<dim3((unsigned)blocks), 256, 0, st>>>(a, ll);
-    else lookup_kernel<T, I, VEC, false><<<dim3((unsigned)blocks), 256, 0, st>>>(a, ll);
+    const int64_t blocks = ceil_div(a.rows << ll, 256), most = 1 << 22;  // (a dimension of a launch has fewer than 2^32 threads)
+    const dim3 grid((unsigned)(blocks < most ? blocks : most), (unsigned)ceil_div(blocks, most));
+    if (a.indptr) lookup_kernel<T, I, VEC, true><<<grid, 256, 0, st>>>(a, ll);
+    else lookup_kernel<T, I, VEC, false><<<grid, 256, 0, st>>>(a, ll);
     return hipGetLastError();
 }
 

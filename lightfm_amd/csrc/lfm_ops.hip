@@ -1,7 +1,9 @@
 // lfm_ops.hip -- the C ABI of include/lfm_ops.h: argument checks on the host, then the launchers of ops_common.hpp.
 #include <math.h>
 
+#include <algorithm>
 #include <string>
+#include <vector>
 
 #include "ops_common.hpp"
 
@@ -27,6 +29,7 @@ static int finish(hipError_t e)
 extern "C" const char *lfm_ops_last_error(void) { return g_ops_err.c_str(); }
 
 static const int64_t MOST_ROWS = 2147483647;
+static const int64_t MOST_SOFTMAX_ROWS = 1 << 27, MOST_SOFTMAX_ITEMS = 1 << 30;  // (launches stay below 2^32 threads)
 
 static int check_type(int32_t dtype, int32_t id_bytes)
 {
@@ -51,8 +54,8 @@ static int check_space(const void *ws, int64_t have, int64_t need)
 static int check_softmax_sizes(int64_t rows, int64_t vocab, int32_t d, int32_t dtype)
 {
     OPS_TRY(check_type(dtype, 4));
-    if (rows < 0 || rows > MOST_ROWS) return refuse(LFM_EINVAL, "rows out of range");
-    if (vocab < 1 || vocab > MOST_ROWS) return refuse(LFM_EINVAL, "the vocabulary is empty or too large");
+    if (rows < 0 || rows > MOST_SOFTMAX_ROWS) return refuse(LFM_EINVAL, "rows out of range");
+    if (vocab < 1 || vocab > MOST_SOFTMAX_ITEMS) return refuse(LFM_EINVAL, "the vocabulary is empty or too large");
     if (d < 1) return refuse(LFM_EINVAL, "d must be positive");
     if (d > LFM_MAX_COMPONENTS) return refuse(LFM_EUNSUPPORTED, "d is beyond LFM_MAX_COMPONENTS");
     return LFM_OK;
@@ -137,6 +140,35 @@ static int check_clip(int64_t n, const int64_t *counts)
     return LFM_OK;
 }
 
+// Tensors are read and written at the same time by many blocks: an output may be its own input and nothing else.
+static int check_overlap(int64_t n, const void *const *x, void *const *out, const int64_t *counts, const int32_t *dtypes)
+{
+    struct Span {
+        uintptr_t begin, end;
+        bool written;
+    };
+    try {
+        std::vector<Span> spans;
+        spans.reserve((size_t)n * 2);
+        for (int64_t i = 0; i < n; ++i) {
+            if (!counts[i]) continue;
+            const uintptr_t bytes = (uintptr_t)counts[i] * (uintptr_t)dtype_bytes(dtypes[i]), to = (uintptr_t)out[i], from = (uintptr_t)x[i];
+            spans.push_back({to, to + bytes, true});
+            if (from != to) spans.push_back({from, from + bytes, false});
+        }
+        std::sort(spans.begin(), spans.end(), [](const Span &a, const Span &b) { return a.begin < b.begin; });
+        uintptr_t any = 0, written = 0;  // where the spans so far end
+        for (const Span &s : spans) {
+            if (s.begin < written || (s.written && s.begin < any)) return refuse(LFM_EINVAL, "a tensor that is written overlaps another one");
+            any = std::max(any, s.end);
+            if (s.written) written = std::max(written, s.end);
+        }
+    } catch (...) {
+        return refuse(LFM_ENOMEM, "out of host memory");
+    }
+    return LFM_OK;
+}
+
 extern "C" int lfm_ops_clip_workspace(int64_t n_tensors, const int64_t *counts, int64_t *bytes)
 {
     if (!bytes) return refuse(LFM_EINVAL, "null pointer");
@@ -156,6 +188,7 @@ extern "C" int lfm_ops_clip_global_norm(int64_t n_tensors, const void *const *x,
         OPS_TRY(check_type(dtypes[i], 4));
         if (counts[i] && (!x[i] || (out && !out[i]))) return refuse(LFM_EINVAL, "null tensor");
     }
+    if (out) OPS_TRY(check_overlap(n_tensors, x, out, counts, dtypes));
     OPS_TRY(check_space(ws, ws_bytes, clip_workspace(n_tensors, counts)));
     return finish(clip_global_norm(n_tensors, x, out, counts, dtypes, max_norm, norm, ws, (hipStream_t)stream));
 }

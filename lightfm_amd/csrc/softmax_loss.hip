@@ -5,10 +5,10 @@
 //
 // Two sweeps over the [rows, vocab] plane, each of which makes the scores in registers on the matrix cores and drops them:
 //
-//   rows_kernel   a wave owns 32 CW rows x (in registers) and streams the table through LDS.  dx needs no second look at
+//   rows_kernel   a wave owns 32 rows x (in registers) and streams the table through LDS.  dx needs no second look at
 //                 the scores: sum_v p w is a mean weighted by the softmax, accumulated beside the running maximum and sum
 //                 (rescaled when the maximum grows), so ONE sweep gives lse and dx -- 4 rows vocab d operations.
-//   table_kernel  a wave owns 32 CW rows of the table and streams x; with lse known it forms q and accumulates dw and db.
+//   table_kernel  a wave owns 32 rows of the table and streams x; with lse known it forms q and accumulates dw and db.
 //
 // Both sweeps compute the score tile transposed to what they own: S = streamed tile (rows of the result) x owned rows
 // (columns = lanes).  A lane then holds 16 scores of ONE owned row, the softmax statistics stay in the lane (one exchange
@@ -117,6 +117,9 @@ __device__ inline float bias_units(float b, const Derived &d)
     return fabsf(b) < INFINITY ? fminf(fmaxf(ldexpf(b, d.k), d.low), -d.low) : b;
 }
 
+// An item whose bias is -inf is not there: its row is not looked at, whatever it holds.
+__device__ inline bool removed(const float *bias, int64_t v) { return bias && bias[v] == -INFINITY; }
+
 __device__ inline int64_t target_of(const lfm_softmax_args &a, int64_t n)
 {
     const int64_t t = a.id_bytes == 8 ? ((const int64_t *)a.targets)[n] : (int64_t)((const int32_t *)a.targets)[n];
@@ -144,7 +147,8 @@ __global__ __launch_bounds__(256) void largest_kernel(lfm_softmax_args a, int pa
                 if (!which) {
                     if (c == 0) outlier[r] = 0;
                     if (target_of(a, r) < 0) continue;
-                }
+                } else if (removed(a.bias, r))
+                    continue;
                 const T *q = p + r * stride + c;
                 if (WIDE_LOADS) {
                     const Vec<T, 4> v = *(const Vec<T, 4> *)q;
@@ -218,11 +222,13 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs p, int dp, int width
         const int64_t r = is_x ? i : i - xr;
         const T *src = is_x ? (const T *)p.a.hidden + r * p.a.hidden_stride : (const T *)p.a.table + r * p.a.table_stride;
         E *dst = (E *)(is_x ? p.x : p.w) + r * (NS * dp) + at;
+        const bool gone = !is_x && removed(p.a.bias, r);
         Vec<T, 4> v[2];
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
             const int cq = c + 4 * q;
-            if (WIDE_LOADS && cq + 4 <= p.a.d) v[q] = *(const Vec<T, 4> *)(src + cq);
+            if (gone) v[q] = {};
+            else if (WIDE_LOADS && cq + 4 <= p.a.d) v[q] = *(const Vec<T, 4> *)(src + cq);
             else
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[q].v[j] = cq + j < p.a.d ? src[cq + j] : (T)0.0f;
@@ -483,13 +489,13 @@ struct Stream {
 };
 
 // registers: two waves per SIMD while the operands leave room for it, one beyond
-#ifndef W1
 constexpr int waves_for(int ns, int dp, bool sums) { return ns * dp > (sums ? 192 : 256) ? 1 : 2; }
-#else
-constexpr int waves_for(int ns, int dp, bool sums) { return W1; }
-#endif
 
-
+// Bound by the matrix pipe and the exponentials together: a block of 32 x 32 scores costs 4 DP matrix cycles per product and
+// about as many for its 16 exponentials, maxima, sums and roundings at DP = 128, which overlap only across the two waves of a
+// SIMD (one wave: 1.5 times the time; three: the operands spill).  8192 x 200003 x 128 bfloat16: 0.90 - 0.94 ms with the
+// gradient, 890 - 930 TFLOP/s, where a product of 8192^3 by the library reaches 1137; 8192 x 26744 x 64 float32: 0.187 ms (300
+// TFLOP/s, each of them three float16 products; the float32 pipe reaches 150).
 template <typename E, int NS, int DP, bool GRAD, bool WIDE>
 __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, GRAD)) void rows_kernel(SweepArgs a)
 {
@@ -498,6 +504,7 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, GRAD)) void rows_
     static_assert(!WIDE || St::BLOCKS == 1, "a chunk per tile");
     __shared__ __attribute__((aligned(16))) E tile[2][Tl::SIZE];
     __shared__ __attribute__((aligned(16))) float sb[2][Tl::BV];
+    __shared__ uint64_t gone[2];  // removed items of a tile
     const Derived dv = derive(NS == 2 ? a.scales : nullptr);
     const St sm(a.chunks);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
@@ -521,19 +528,38 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, GRAD)) void rows_
 
         Tl t;
         float next_bias = 0.0f;
+        bool next_gone = false;
         auto fetch = [&](int i, int j) {
             const int64_t r = (int64_t)(t0 + i) * Tl::BV, v = r + threadIdx.x;
             t.fetch((const E *)a.w + sm.offset(j), a.ldw, r, a.vocab);
-            if (j == 0 && threadIdx.x < Tl::BV) next_bias = v >= a.vocab ? -INFINITY : a.bias ? bias_units(a.bias[v], dv) : 0.0f;
+            if (j == 0 && threadIdx.x < Tl::BV) {
+                next_bias = v >= a.vocab ? -INFINITY : a.bias ? bias_units(a.bias[v], dv) : 0.0f;
+                next_gone = v < a.vocab && next_bias == -INFINITY;
+            }
         };
         auto store = [&](int i, int j, int buf) {
             t.store(tile[buf]);
-            if (j == 0 && threadIdx.x < Tl::BV) sb[i & 1][threadIdx.x] = next_bias;
+            if (j == 0 && threadIdx.x < Tl::BV) {
+                sb[i & 1][threadIdx.x] = next_bias;
+                const uint64_t mask = __ballot(next_gone);
+                if (threadIdx.x == 0) gone[i & 1] = mask;
+            }
+        };
+        // the rows of removed items, where the tile has any (split operands: pack_kernel has seen to it)
+        auto clear_removed = [&](int i, int buf) {
+            if (NS == 2) return;
+            const uint64_t mask = gone[i & 1];
+            if (mask == 0) return;
+#pragma unroll
+            for (int q = 0; q < Tl::PER; ++q)
+                if ((mask >> Tl::row_of(q)) & 1u) *(uint4 *)(tile[buf] + slot_of(Tl::row_of(q)) * Tl::ROW + (q * 256 + (int)threadIdx.x) % Tl::CHUNKS * 8) = make_uint4(0, 0, 0, 0);
+            __syncthreads();
         };
         __syncthreads();  // (the owner before is done with the tiles)
         fetch(0, 0);
         store(0, 0, 0);
         __syncthreads();
+        clear_removed(0, 0);
         int buf = 0;
         for (int i = 0; i < nt; ++i) {
             if (!WIDE && i + 1 < nt) fetch(i + 1, 0);
@@ -561,6 +587,7 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, GRAD)) void rows_
                         store(i, j + 1, buf ^ 1);
                         __syncthreads();
                         buf ^= 1;
+                        clear_removed(i, buf);
                     }
                     if (GRAD) to.read(tile[buf], 0);
                 } else {
@@ -606,6 +633,7 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, GRAD)) void rows_
             if (i + 1 < nt) store(i + 1, 0, buf ^ 1);
             __syncthreads();
             buf ^= 1;
+            if (i + 1 < nt) clear_removed(i + 1, buf);
         }
         const float sum = half_wave_sum(l);
         if (n >= a.rows) continue;
@@ -635,6 +663,8 @@ struct RowFacts {
     int32_t target[BV];
 };
 
+// Bound like rows_kernel, with more to do per score: maximum, rate and target of a score's row come from LDS.  8192 x 200003 x
+// 128 bfloat16: 1.13 ms, 740 TFLOP/s; 8192 x 26744 x 64 float32: 0.220 ms.
 template <typename T, typename E, int NS, int DP, bool WIDE>
 __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, true)) void table_kernel(SweepArgs a)
 {
@@ -658,8 +688,9 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, true)) void table
         const int32_t w0 = (int32_t)(owner * 128 + wave * 32);
         const int64_t v = (int64_t)w0 + (lane & 31);
         typename Half<E>::x8 own[NS][DP / 16];
-        if (!WIDE) load_owned<E, NS, DP>(own, (const E *)a.w, a.ldw, v, a.vocab, dv.owned);
         const float bias = a.bias && v < a.vocab ? bias_units(a.bias[v], dv) : 0.0f;
+        const int64_t have = NS == 1 && bias == -INFINITY ? 0 : a.vocab;  // a removed item's row: zeros
+        if (!WIDE) load_owned<E, NS, DP>(own, (const E *)a.w, a.ldw, v, have, dv.owned);
         float db = 0.0f;
         f32x16 out[DP / 32];
 #pragma unroll
@@ -674,7 +705,7 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, true)) void table
             t.fetch((const E *)a.x + sm.offset(j), a.ldx, r, a.rows);
 #pragma unroll
             for (int k = 0; k < Tl::PER; ++k) {
-                const int64_t n = r + (k * 256 + (int)threadIdx.x) / Tl::CHUNKS;
+                const int64_t n = r + Tl::row_of(k);
                 keep[k] = n < a.rows && a.row_target[n] >= 0;
             }
             if (j == 0 && threadIdx.x < Tl::BV) {
@@ -719,7 +750,7 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, true)) void table
                 const float fars = f.far[r0 + (lane & 31)];
                 if (WIDE) {
                     for (int j = 0; j < sm.chunks; ++j) {
-                        load_owned<E, NS, DP>(own, (const E *)a.w + sm.offset(j), a.ldw, v, a.vocab, dv.owned);
+                        load_owned<E, NS, DP>(own, (const E *)a.w + sm.offset(j), a.ldw, v, have, dv.owned);
                         const bool last = j + 1 == sm.chunks;
                         if (!last || i + 1 < nt) fetch(last ? i + 1 : i, last ? 0 : j + 1);
                         so.read(tile[buf], 0);
@@ -859,6 +890,7 @@ __global__ __launch_bounds__(256) void few_rows_kernel(SweepArgs a, const float 
             for (int u = 0; u < U; ++u) {
                 const int64_t v = v0 + (int64_t)u * groups;
                 w[u] = *(const Vec<float, VEC> *)(table + (v < hi ? v : v0) * a.ldw + c);
+                if (b[u] == -INFINITY) w[u] = {};  // a removed item, or none
             }
 #pragma unroll
             for (int r = 0; r < ROWS; ++r)
@@ -1007,6 +1039,7 @@ __global__ __launch_bounds__(256) void join_rows_kernel(JoinArgs j)
         if (row_max<LANES>(finite, shared) == 0.0f) {
             float top = -INFINITY, mass = 0.0f;
             for (int64_t v = lane; v < a.vocab; v += LANES) {
+                if (removed(a.bias, v)) continue;
                 const float s = dot_lane(x, (const T *)a.table + v * a.table_stride, a.d) + (a.bias ? a.bias[v] : 0.0f);
                 const float up = fmaxf(top, s);
                 if (up > -INFINITY) mass = mass * expf(top - up) + expf(s - up);
@@ -1127,13 +1160,13 @@ __global__ __launch_bounds__(256) void join_table_kernel(SweepArgs a, int ns)
 template <typename T>
 __global__ __launch_bounds__(256) void clear_kernel(T *p, int64_t n, float *q, int64_t m)
 {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < n) p[i] = (T)0.0f;
-    if (q && i < m) q[i] = 0.0f;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        p[i] = (T)0.0f;
+        if (q && i < m) q[i] = 0.0f;  // (m <= n)
+    }
 }
 
 // -------------------------------------------------------------------- host ---
-
 
 struct Plan {
     int dp, ns;
@@ -1274,12 +1307,15 @@ hipError_t run(const lfm_softmax_args &a, bool grad, void *ws, hipStream_t st)
     hipError_t e;
     if (a.rows == 0) {
         if (!grad) return hipSuccess;
-        clear_kernel<T><<<dim3((unsigned)ceil_div(a.vocab * a.d, 256)), 256, 0, st>>>((T *)a.d_table, a.vocab * a.d, a.d_bias, a.vocab);
+        const int64_t blocks = ceil_div(a.vocab * a.d, 256);
+        clear_kernel<T><<<dim3((unsigned)(blocks < 8192 ? blocks : 8192)), 256, 0, st>>>((T *)a.d_table, a.vocab * a.d, a.d_bias, a.vocab);
         return hipGetLastError();
     }
     // scales are wanted for float32 operands, and of the weights for float16 gradients
     const bool scales = NS == 2 || (a.dtype == LFM_F16 && a.weights && grad);
-    auto in_place = [&](const void *q, int64_t stride) { return NS == 1 && a.d == p.dp && stride % 8 == 0 && ((uintptr_t)q & 15) == 0; };
+    auto in_place = [&](const void *q, int64_t stride) {  // (offsets inside a tile are 32-bit)
+        return NS == 1 && a.d == p.dp && stride % 8 == 0 && stride < (1 << 24) && ((uintptr_t)q & 15) == 0;
+    };
     const bool x_there = in_place(a.hidden, a.hidden_stride), w_there = in_place(a.table, a.table_stride);
     // both operands can be read four elements at a time
     const bool wide = a.d % 4 == 0 && a.hidden_stride % 4 == 0 && a.table_stride % 4 == 0 &&

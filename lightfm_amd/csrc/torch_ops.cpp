@@ -57,7 +57,9 @@ const char *type_name(const at::Tensor &t) { return c10::toString(t.scalar_type(
 const at::Tensor &tensor(PyObject *o, const char *name)
 {
     if (!THPVariable_Check(o)) refuse(PyExc_TypeError, "%s must be a torch tensor", name);
-    return THPVariable_Unpack(o);
+    const at::Tensor &t = THPVariable_Unpack(o);
+    if (t.is_neg()) refuse(PyExc_ValueError, "%s is a lazily negated view: call resolve_neg() first", name);
+    return t;
 }
 
 void shape(const at::Tensor &t, const char *name, int64_t dims)
@@ -323,6 +325,8 @@ PyObject *clip(PyObject *, PyObject *const *args, Py_ssize_t n)
         const at::Tensor norm = on.make({}, at::kFloat), ws = on.scratch(need);
         check(lfm_ops_clip_global_norm((int64_t)xs.size(), x.data(), scale ? y.data() : nullptr, counts.data(), kinds.data(), top,
                                        (float *)norm.data_ptr(), ws.data_ptr(), need, on.stream()));
+        for (const at::Tensor *t : ys)  // written in place: autograd has to notice
+            if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
         return THPVariable_Wrap(norm);
     });
 }

@@ -1,8 +1,8 @@
 """Operators of a full-softmax training step on tensors that live on the GPU (include/lfm_ops.h).
 
-`LightFM` trains with sampled ranking losses from host arrays; a model that is trained with the softmax over the whole
-catalogue -- a session or sequence recommender on top of the same item tables -- needs three operators more, and needs
-them on device memory, between the layers of its own program.  They take and return torch tensors of one GPU:
+`LightFM(loss="softmax")` runs these kernels on its own tables; a model of the caller's that is trained with the softmax
+over the whole catalogue -- a session or sequence recommender on top of the same item tables -- needs them on device
+memory, between the layers of its own program.  They take and return torch tensors of one GPU:
 
     softmax_loss(hidden, table, targets, bias=, weights=)       -> loss, lse
     softmax_loss_grad(hidden, table, targets, bias=, weights=)  -> loss, lse, d_hidden, d_table, d_bias
@@ -80,7 +80,8 @@ def softmax_loss(hidden, table, targets, bias=None, weights=None):
     """Cross entropy of every row of `hidden` [rows, d] against all rows of `table` [vocab, d]: scores
     s = hidden table^T + bias, lse = log sum exp s, loss = weights * (lse - s[target]).  Returns (loss, lse), float32
     [rows]; a row whose target is not in [0, vocab) has loss 0.  bias [vocab] / weights [rows] are float32; a bias of
-    -inf takes an item out of the softmax.  The scores are never kept."""
+    -inf takes an item out of the softmax, whatever its row holds.  The scores are never kept.  float32 operands are
+    multiplied with 22 bits and a floor of 2^-39 of the largest magnitude of hidden or table."""
     return _ops.softmax(hidden, table, targets, bias, weights, False)
 
 
@@ -115,7 +116,7 @@ def global_norm(tensors):
 def clip_global_norm(tensors, max_norm, out=None):
     """Scales all tensors (a list or tuple) by min(1, max_norm / norm), norm = global_norm(tensors), in place or into the
     tensors of `out`, and returns the norm.  A norm that is not finite leaves the values unscaled: look at the returned
-    norm."""
+    norm.  A tensor that is written overlaps no other one (ValueError)."""
     if not max_norm >= 0.0:
         raise ValueError("max_norm must not be negative")
     return _ops.clip(tensors, max_norm, tensors if out is None else out)

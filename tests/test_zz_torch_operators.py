@@ -203,6 +203,31 @@ def test_softmax_nothing_left(env, dtype, rows):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows, d", [(2, 64), (70, 64), (70, 50), (33, 300)])
+def test_softmax_removed_items_hold_anything(env, dtype, rows, d):
+    """NaN, infinities and the type's largest values in the rows of removed items: the results are those of zeros there,
+    bit for bit (in place, packed, in chunks of columns, and with few rows)."""
+    torch, ops = env
+    x, w, t, b, k = make(torch, rows, 420, d, dtype, seed=14, ignored=False)
+    gone = torch.zeros(420, dtype=torch.bool, device="cuda")
+    gone[[0, 3, 64, 65, 200, 419]] = True
+    gone[300:390] = True
+    t[gone[t.long()]] = 7
+    b[gone] = -math.inf
+    w[gone] = 0
+    clean = check_softmax(env, x, w, t, b, k)
+    few = ops.softmax_loss(x, w, t, bias=b, weights=k)
+    w[gone] = torch.finfo(w.dtype).max
+    w[3], w[64], w[65, 1], w[320:340] = float("nan"), math.inf, -math.inf, -math.inf
+    got = ops.softmax_loss_grad(x, w, t, bias=b, weights=k)
+    for i in range(5):
+        assert torch.equal(got[i], clean[i]), i
+    for one, other in zip(ops.softmax_loss(x, w, t, bias=b, weights=k), few):
+        assert torch.equal(one, other)
+    assert (got[3][gone] == 0).all() and (got[4][gone] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("rows", [12, 100])
 def test_softmax_rows_without_target_are_not_read(env, dtype, rows):
     """NaN and infinities in rows without a target touch nothing but their own lse."""
@@ -509,6 +534,17 @@ def test_lookup_offsets_past_32_bits(env):
     assert not g.view(torch.int32).any()
 
 
+def test_lookup_of_more_lanes_than_one_dimension_of_a_launch(env):
+    """2^30 + 80 lanes: a launch of two rows of blocks."""
+    torch, ops = env
+    rows, d = (1 << 26) + 5, 128
+    w = torch.randn(1009, d, device="cuda").to(torch.bfloat16)
+    ids = (torch.arange(rows, device="cuda") % 1009).int()
+    out = ops.embedding_lookup(w, ids)
+    for lo in range(0, rows, 1 << 22):
+        assert torch.equal(out[lo:lo + (1 << 22)], w[ids[lo:lo + (1 << 22)].long()]), lo
+
+
 # -------------------------------------------------------------------- clip ---
 
 def check_clip(env, tensors, max_norm, out=None):
@@ -675,6 +711,28 @@ def test_after_a_session_in_the_same_process(env):
     t = torch.arange(60, device="cuda") % 50
     check_softmax(env, h, w, t, b, None)
     assert np.isfinite(m.predict(np.zeros(50, np.int32), np.arange(50, dtype=np.int32))).all()
+
+
+def test_clip_refuses_overlaps_and_tells_autograd(env):
+    torch, ops = env
+    a = torch.ones(1000, device="cuda")
+    b = torch.ones(1000, device="cuda")
+    for wrong in (lambda: ops.clip_global_norm([a, a], 1.0), lambda: ops.clip_global_norm([a, a[100:200]], 1.0),
+                  lambda: ops.clip_global_norm([a, b], 1.0, out=[b, a]), lambda: ops.clip_global_norm([a[:900], b], 1.0, out=[a[100:], b]),
+                  lambda: ops.clip_global_norm([a, b], 1.0, out=[torch.empty_like(a), a]),
+                  lambda: ops.clip_global_norm([a, b], 1.0, out=[torch.ones(1000, device="cuda")] * 2)):
+        with pytest.raises(ValueError, match="overlaps"):
+            wrong()
+    assert (a == 1).all() and (b == 1).all()
+    assert abs(float(ops.global_norm([a, a])) - math.sqrt(2000.0)) < 1e-4  # (reading twice is no conflict)
+    out = torch.empty(2, 1000, device="cuda")
+    ops.clip_global_norm([a, a], 1.0, out=[out[0], out[1]])
+    assert torch.equal(out[0], out[1])
+    before = a._version
+    ops.clip_global_norm([a[:500], a[500:]], 1.0)
+    assert a._version > before
+    with pytest.raises(ValueError, match="negated"):
+        ops.global_norm([torch.ones(4, dtype=torch.complex64, device="cuda")[:1].conj().imag])
 
 
 def test_python_refusals_on_the_gpu(env):
