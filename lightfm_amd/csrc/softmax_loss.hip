@@ -82,7 +82,7 @@ constexpr float P_SHIFT = 7.0f, LAG = 8.0f;
 // exp2(s c - m c) as one multiply-add is off by the rounding of m c: with |m c| up to this, as much as s itself
 constexpr float FAR = 512.0f;
 constexpr int K_MOST = 60;  // see Scales
-constexpr int MAX_PARTS = 128;
+constexpr int MAX_PARTS = 512;  // of an operand in largest_kernel (128: 24380 x 169 float32 takes 100 us instead of 82)
 
 // Powers of two that bring the operands into float16's range (all 0 for half-precision operands).
 struct Scales {
@@ -1183,13 +1183,22 @@ int width_for(int d)
     return (d + 255) / 256 * 256;
 }
 
+// As many blocks as run at once, with two exceptions.  A block of a single tile is mostly prologue and parts to join: up to
+// twice as many tiles as the card has compute units are dealt two to a block (gradients of 5276 rows x 712 items x 16 float32: 69 ->
+// 55 us, 3660 x 806 x 188 float16: 115 -> 100).  And where there are nearly as many owners as blocks would be, each has a block
+// to itself and nothing is joined (1003 x 50021 x 100 float16, 391 owners for 512 blocks: 120 -> 106 us; with 301 owners,
+// 2228 x 38507 x 19 float32, the idle slots cost more than the join: 125 -> 145).
 Pieces pieces_for(int64_t owned, int64_t streamed, int bv, int64_t slots)
 {
     Pieces p;
     p.owners = (uint32_t)ceil_div(owned < 1 ? 1 : owned, 128);
     p.tiles = (uint32_t)ceil_div(streamed < 1 ? 1 : streamed, bv);
     const uint64_t units = (uint64_t)p.owners * p.tiles;
-    p.blocks = (uint32_t)(units < (uint64_t)slots ? units : (uint64_t)slots);
+    uint64_t blocks = units / 2 > p.owners ? units / 2 : p.owners;
+    if (blocks < 256) blocks = units < 256 ? units : 256;
+    if (blocks > (uint64_t)slots) blocks = slots;
+    if (p.owners <= blocks && (uint64_t)p.owners * 100 >= blocks * 70) blocks = p.owners;
+    p.blocks = (uint32_t)blocks;
     return p;
 }
 
@@ -1200,7 +1209,7 @@ Plan plan_for(int64_t rows, int64_t vocab, int d, int dtype, bool grad)
     p.ns = dtype == LFM_F32 ? 2 : 1;
     p.chunks = p.dp > 256 ? p.dp / 256 : 1;
     const int w = p.dp > 256 ? 256 : p.dp, bv = p.ns * w <= 128 ? 64 : 32;
-    // as many blocks as run at once on the card's 256 compute units
+    // slots: blocks that run at once on the card's 256 compute units
     p.rows = pieces_for(rows, vocab, bv, 256 * (p.chunks > 1 ? 1 : waves_for(p.ns, w, grad)));
     p.few = 0;
     if (!grad && dtype == LFM_F32 && rows <= FEW) {
