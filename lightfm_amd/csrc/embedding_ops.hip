@@ -105,6 +105,8 @@ hipError_t lookup_typed(const lfm_lookup_args &a, hipStream_t st)
         return launch_lookup<T, I, W>(a, st);
     if (aligned(a.table, a.table_stride, a.d, sizeof(T), W / 2) && aligned(a.out, a.d, a.d, sizeof(T), W / 2))
         return launch_lookup<T, I, W / 2>(a, st);
+    if constexpr (W > 4)
+        if (aligned(a.table, a.table_stride, a.d, sizeof(T), 2) && aligned(a.out, a.d, a.d, sizeof(T), 2)) return launch_lookup<T, I, 2>(a, st);
     return launch_lookup<T, I, 1>(a, st);
 }
 
@@ -115,12 +117,11 @@ hipError_t lookup_typed(const lfm_lookup_args &a, hipStream_t st)
 //    eight waves one contiguous part of the piece each, so "earlier block, earlier wave, earlier lane" is the order of
 //    the positions.  The scatter kernel sums the blocks' digit counts itself (at most 128 blocks): a digit takes two
 //    launches, and no count depends on the order in which atomics land.
-// 2. the sorted list is cut into chunks of CHUNK ids; a lane group sums a chunk's runs of equal ids in float32, in
-//    order.  A run inside one chunk is written to its row at once, a run that crosses chunks leaves partial sums.
+// 2. the sorted list is cut into chunks of 8 to 32 ids (chunk_for); a lane group sums a chunk's runs of equal ids in float32, in order.  A run inside one chunk is written to its row at once, a run that crosses chunks leaves partial sums.
 // 3. the block of the chunk where a crossing run starts adds the run's partial sums, in a fixed order.
 // Rows without ids are zero: the first launch fills the output.
 
-constexpr int SORT_WAVES = 8, SORT_THREADS = 64 * SORT_WAVES, MAX_BINS = 2048, MAX_BLOCKS = 128, CHUNK = 32;
+constexpr int SORT_WAVES = 8, SORT_THREADS = 64 * SORT_WAVES, MAX_BINS = 2048, MAX_BLOCKS = 128;
 
 struct SortPlan {
     int passes, bits, bins;  // digits, bits of a digit, 1 << bits
@@ -176,9 +177,15 @@ __device__ inline void fill_and_bags(int first, uint4 *fill, int64_t fill_words,
 
 // Short lists are sorted in one launch: an id's place is the number of ids before it (smaller, or equal and earlier), which
 // a block counts for 32 ids over the whole list in LDS, eight threads to an id.  n^2 comparisons, but no passes that wait for
-// each other: 3 launches for the whole gradient instead of 6.  On the GPU alone (26744 x 64) 1000 ids take 21.9 us against 28, 2000
-// 25.8 against 31.6, 4000 32.5 against 33.9; a caller that is bound by its launches saves three of them.
-constexpr int SHORT = 2048, RANKED = 32, RANK_PARTS = 256 / RANKED;
+// each other: 3 launches for the whole gradient instead of 6.  On the GPU alone (26744 x 64 float32) 2000 ids take 19.8 us, 3000 21.7
+// against 27, 4000 26.1 against 28; from 6000 on (31 against 28) the digits are faster.
+constexpr int SHORT = 4096, RANKED = 32, RANK_PARTS = 256 / RANKED;
+
+// Ids that a lane group sums one after the other, eight rows in flight: small chunks while there are lanes enough, large ones
+// where the parts of runs that cross chunks would cost more than the waiting (26744 x 64 float32 / 400000 x 128 bfloat16, us, 8 | 16 |
+// 32 to a chunk: 8000 ids 29 | 31 | 36 / 48 | 53 | 64; 60000 35 | 36 | 40 / 59 | 62 | 72; 180000 48 | 48 | 48 / 92 | 86 | 92; 600000 32
+// alone 85 / 144, 16 90 / 158).
+int chunk_for(int64_t nnz) { return nnz <= 65536 ? 8 : nnz <= 200000 ? 16 : 32; }
 
 template <typename I>
 __global__ __launch_bounds__(256) void rank_kernel(const I *ids, int n, int64_t vocab, int sort_blocks, uint4 *fill, int64_t fill_words,
@@ -367,8 +374,8 @@ __device__ inline void store_row(const SumArgs &a, uint32_t key, int c, const fl
 }
 
 // A block reads the ids, rows and values of its lane groups' chunks at once (they are pointers to pointers: position, bag,
-// row), then each group walks its own.
-template <typename T, int VEC>
+// row), then each group walks its own.  blockIdx.y: the columns, as many at a time as a group has lanes for.
+template <typename T, int VEC, int CHUNK>
 __global__ __launch_bounds__(256) void chunk_sum_kernel(SumArgs a, int lanes_log2)
 {
     constexpr int MOST = 64 * CHUNK;  // 4 lanes to a group at least
@@ -401,7 +408,8 @@ __global__ __launch_bounds__(256) void chunk_sum_kernel(SumArgs a, int lanes_log
     const int hi = a.n - first < lo + CHUNK ? (int)(a.n - first) : lo + CHUNK;
     const uint32_t earlier = lo ? keys[lo - 1] : first ? a.keys[first - 1] : none, later = keys[hi];
     typedef Vec<T, VEC> V;
-    for (int c = lane * VEC; c < a.d; c += lanes * VEC) {
+    const int c = ((int)blockIdx.y * lanes + lane) * VEC;
+    if (c < a.d) {
         float acc[VEC];
 #pragma unroll
         for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
@@ -435,7 +443,7 @@ __global__ __launch_bounds__(256) void chunk_sum_kernel(SumArgs a, int lanes_log
                     for (int k = 0; k < VEC; ++k) acc[k] = fmaf(values[j0 + q], (float)r[q].v[k], acc[k]);
             }
         }
-        if (run == none) continue;
+        if (run == none) return;
         if (began && later != run) store_row<T, VEC>(a, run, c, acc);
         else {
             float *to = (began ? a.tail : a.head) + chunk * a.d + c;
@@ -449,7 +457,7 @@ __global__ __launch_bounds__(256) void chunk_sum_kernel(SumArgs a, int lanes_log
 // long (a popular id), and added in a fixed order.  A block looks at one chunk per wave.
 constexpr int LONG_RUN = 64;
 
-template <typename T, int VEC>
+template <typename T, int VEC, int CHUNK>
 __global__ __launch_bounds__(256) void join_kernel(SumArgs a, int lanes_log2)
 {
     __shared__ float sums[256 * VEC];
@@ -483,32 +491,29 @@ __global__ __launch_bounds__(256) void join_kernel(SumArgs a, int lanes_log2)
         const int64_t share = ceil_div(n, groups);
         const int64_t p0 = group * share < n ? group * share : n, p1 = p0 + share < n ? p0 + share : n;
         const int used = (int)ceil_div(n, share);
-        for (int c0 = 0; c0 < a.d; c0 += lanes * VEC) {
-            const int c = c0 + lane * VEC;
-            float acc[VEC];
+        const int c = ((int)blockIdx.y * lanes + lane) * VEC;
+        float acc[VEC];
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
-            if (c < a.d) {
+        for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
+        if (c < a.d) {
 #pragma unroll 8
-                for (int64_t p = p0; p < p1; ++p) {
+            for (int64_t p = p0; p < p1; ++p) {
 #pragma unroll
-                    for (int k = 0; k < VEC; ++k) acc[k] += a.head[(chunk + 1 + p) * a.d + c + k];
-                }
+                for (int k = 0; k < VEC; ++k) acc[k] += a.head[(chunk + 1 + p) * a.d + c + k];
             }
-            if (together) __syncthreads();
-            else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+        if (together) __syncthreads();
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) mine[(group * lanes + lane) * VEC + k] = acc[k];
-            if (together) __syncthreads();
-            else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            if (group == 0 && c < a.d) {
+        for (int k = 0; k < VEC; ++k) mine[(group * lanes + lane) * VEC + k] = acc[k];
+        if (together) __syncthreads();
+        else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (group == 0 && c < a.d) {
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) acc[k] = a.tail[chunk * a.d + c + k];
-                for (int g = 0; g < used; ++g)
+            for (int k = 0; k < VEC; ++k) acc[k] = a.tail[chunk * a.d + c + k];
+            for (int g = 0; g < used; ++g)
 #pragma unroll
-                    for (int k = 0; k < VEC; ++k) acc[k] += mine[(g * lanes + lane) * VEC + k];
-                store_row<T, VEC>(a, key, c, acc);
-            }
+                for (int k = 0; k < VEC; ++k) acc[k] += mine[(g * lanes + lane) * VEC + k];
+            store_row<T, VEC>(a, key, c, acc);
         }
         if (together) __syncthreads();  // (a wave's own sums use the same places)
     }
@@ -526,7 +531,7 @@ GradSpace grad_space(int64_t vocab, int64_t nnz, int d, bool bags, void *ws)
     Carver c(ws);
     GradSpace s;
     const SortPlan p = sort_plan(vocab, nnz);
-    const int64_t chunks = ceil_div(nnz, CHUNK);
+    const int64_t chunks = ceil_div(nnz, chunk_for(nnz));
     for (int i = 0; i < 2; ++i) {
         s.keys[i] = c.take<uint32_t>(nnz);
         s.pos[i] = c.take<uint32_t>(nnz);
@@ -539,17 +544,28 @@ GradSpace grad_space(int64_t vocab, int64_t nnz, int d, bool bags, void *ws)
     return s;
 }
 
-template <typename T, int VEC>
-hipError_t launch_sums(const SumArgs &s, hipStream_t st)
+template <typename T, int VEC, int CHUNK>
+hipError_t launch_chunks(const SumArgs &s, hipStream_t st)
 {
     int ll = lanes_for(s.d, VEC);
     if (ll < 2) ll = 2;
     const int64_t chunks = ceil_div(s.n, CHUNK);
-    chunk_sum_kernel<T, VEC><<<dim3((unsigned)ceil_div(chunks, 256 >> ll)), 256, 0, st>>>(s, ll);
+    const unsigned slices = (unsigned)ceil_div(s.d, (int64_t)VEC << ll);  // (at most 1024)
+    chunk_sum_kernel<T, VEC, CHUNK><<<dim3((unsigned)ceil_div(chunks, 256 >> ll), slices), 256, 0, st>>>(s, ll);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || chunks < 2) return e;
-    join_kernel<T, VEC><<<dim3((unsigned)ceil_div(chunks, 4)), 256, 0, st>>>(s, ll);
+    join_kernel<T, VEC, CHUNK><<<dim3((unsigned)ceil_div(chunks, 4), slices), 256, 0, st>>>(s, ll);
     return hipGetLastError();
+}
+
+template <typename T, int VEC>
+hipError_t launch_sums(const SumArgs &s, hipStream_t st)
+{
+    switch (chunk_for(s.n)) {
+    case 8: return launch_chunks<T, VEC, 8>(s, st);
+    case 16: return launch_chunks<T, VEC, 16>(s, st);
+    default: return launch_chunks<T, VEC, 32>(s, st);
+    }
 }
 
 template <typename T>
@@ -560,6 +576,8 @@ hipError_t sums_typed(const SumArgs &s, hipStream_t st)
         return launch_sums<T, W>(s, st);
     if (aligned(s.d_out, s.stride, s.d, sizeof(T), W / 2) && aligned(s.out, s.d, s.d, sizeof(T), W / 2))
         return launch_sums<T, W / 2>(s, st);
+    if constexpr (W > 4)
+        if (aligned(s.d_out, s.stride, s.d, sizeof(T), 2) && aligned(s.out, s.d, s.d, sizeof(T), 2)) return launch_sums<T, 2>(s, st);
     return launch_sums<T, 1>(s, st);
 }
 

@@ -462,6 +462,16 @@ def test_lookup_long_lists(env):
         assert torch.equal(first, ops.embedding_lookup_grad(x, ids, vocab))
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows, vocab, d", [(4096, 3, 70), (4097, 3, 70), (65536, 900, 131), (65537, 7, 34), (150001, 20011, 6), (200001, 40, 257)])
+def test_lookup_gradient_at_the_lengths_where_the_form_changes(env, rows, vocab, d, dtype):
+    torch, ops = env
+    ids, _, _ = bags(torch, rows, vocab, 0, seed=rows + d, skew=True)
+    x = torch.randn(rows, d, device="cuda").to(getattr(torch, DTYPE[dtype]))
+    first = check_lookup_grad(env, x, ids, vocab, None, None, 1.25)
+    assert torch.equal(first, ops.embedding_lookup_grad(x, ids, vocab, scale=1.25))
+
+
 def test_lookup_one_id_only_and_all_out_of_range(env):
     torch, ops = env
     x = torch.randn(5000, 24, device="cuda")
