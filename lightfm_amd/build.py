@@ -6,9 +6,11 @@ hipcc cross-compiles without a GPU.  -ffp-contract=off keeps the reference's
 separate float32 multiply/add roundings (no FMA contraction);
 -munsafe-fp-atomics selects the hardware global_atomic_add_f32.
 """
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -76,9 +78,7 @@ def build(force=False, verbose=False):
             + ["-Wl,--no-as-needed", stand_in])
         os.remove(stand_in)
     binding, src = os.path.join(OUT_DIR, "_torch_ops.so"), os.path.join(CSRC, TORCH_OPS)
-    if force or _stale(binding, [src, OPS_LIB, hdrs[1]]):
-        import sysconfig
-
+    if importlib.util.find_spec("torch") and (force or _stale(binding, [src, OPS_LIB, hdrs[1]])):
         import torch
         root = os.path.dirname(torch.__file__)
         run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-w", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",

@@ -164,8 +164,25 @@ __device__ inline void fill_and_bags(int first, uint4 *fill, int64_t fill_words,
     for (int64_t i = t; i < fill_words; i += step) fill[i] = make_uint4(0, 0, 0, 0);
     if (t < fill_tail_bytes) fill_tail[t] = 0;
     if (!indptr) return;
-    for (int64_t j = t; j < n; j += step) {  // the last row whose bag starts at or before j
-        int64_t lo = 0, hi = rows - 1;
+    const double per_id = (double)rows / (double)n;
+    for (int64_t j = t; j < n; j += step) {  // the last row whose bag starts at or before j, looked for around where even bags have it
+        int64_t lo = 0, hi = rows - 1, at = (int64_t)((double)j * per_id), gap = 1;
+        if (at > hi) at = hi;
+        if ((int64_t)indptr[at] <= j) {
+            lo = at;
+            while (lo + gap <= hi && (int64_t)indptr[lo + gap] <= j) {
+                lo += gap;
+                gap *= 2;
+            }
+            if (lo + gap - 1 < hi) hi = lo + gap - 1;
+        } else {
+            hi = at > 0 ? at - 1 : 0;
+            while (hi - gap >= 0 && (int64_t)indptr[hi - gap + 1] > j) {
+                hi -= gap;
+                gap *= 2;
+            }
+            if (hi - gap + 1 > 0) lo = hi - gap + 1;
+        }
         while (lo < hi) {
             const int64_t mid = (lo + hi + 1) >> 1;
             if ((int64_t)indptr[mid] <= j) lo = mid;
