@@ -42,7 +42,7 @@ const char *lfm_ops_last_error(void);
  * removes an item: its row of the table is not looked at, whatever it holds, and has a zero gradient (as a target, its loss is
  * infinite).  Rows of hidden and table are contiguous, `*_stride` elements apart; the gradients are dense.
  * float32 operands keep 22 bits and a floor of 2^-39 of the largest magnitude of hidden (rows with a target) or table (items not
- * removed).  At most 2^27 rows and 2^30 items. */
+ * removed); the terms q of d_table keep 22 bits and an absolute error of 2^-38 of the largest weight.  At most 2^27 rows and 2^30 items. */
 typedef struct lfm_softmax_args {
     const void *hidden, *table; /* [rows, d], [vocab, d] of `dtype` */
     const void *targets;        /* [rows] int32 or int64 */

@@ -19,7 +19,8 @@
 // float32 operands: x = 2^-k (hi + lo) with hi, lo in float16 and k from the largest magnitude, a product is hi hi + hi lo +
 // lo hi on the float16 matrix pipe.  An operand keeps 22 bits (and a floor of 2^-39 of the largest magnitude), the product
 // left out is 2^-22 of the term: the size of float32's own rounding over a sum, at a third of the float16 rate instead of the
-// float32 pipe's 1/16.  The probabilities that enter the second product are split the same way.  Half-precision operands
+// float32 pipe's 1/16.  The probabilities that enter the second product are split the same way: those of dw, scaled so that the
+// largest weight is 2^14, are off by 2^-38 of it at most, so a probability below 2^-17 or so has fewer bits than float32's.  Half-precision operands
 // are multiplied as they are; their probabilities are rounded once to the operands' type (to nearest: 2^-9 / 2^-12
 // relative, below the rounding of the result).  All sums, maxima and statistics are float32.
 #include "ops_common.hpp"
@@ -366,7 +367,7 @@ __device__ inline void scores(f32x16 &acc, const typename Half<E>::x8 (&own)[NS]
 }
 
 // Eight float32 values to a matrix operand: rounded to nearest (bf16, f16), or split into two float16 (hi towards zero, two
-// values per instruction; the remainder is exact and keeps 11 bits more).
+// values per instruction; the remainder is exact and keeps 11 bits more, to nearest).
 __device__ inline Half<bf16_t>::x8 round_values(const float (&v)[8], Half<bf16_t>::x8)
 {
     Half<bf16_t>::x8 r;
@@ -407,7 +408,7 @@ struct Values {  // the probabilities of 32 streamed rows as matrix operands
                 v[0][k] = cut_values(part);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) rest[j] = __builtin_fmaf((float)v[0][k][j], -1.0f, part[j]);
-                v[NS - 1][k] = cut_values(rest);
+                v[NS - 1][k] = round_values(rest, typename Half<E>::x8());
             } else
                 v[0][k] = round_values(part, typename Half<E>::x8());
         }

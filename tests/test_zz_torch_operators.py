@@ -202,6 +202,43 @@ def test_softmax_nothing_left(env, dtype, rows):
     near(torch, lse, torch.full_like(lse, torch.finfo(torch.float32).min).double(), torch.tensor(2.0 ** 105, device="cuda").double(), "lse")
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_softmax_offsets_past_32_bits(env, dtype):
+    """A table of more than 2^32 elements: scores, gradients and targets at both ends of it."""
+    torch, ops = env
+    vocab, d, rows, step = 67500001, 64, 9, 1 << 22
+    x, _, _, _, k = make(torch, rows, 8, d, dtype, seed=15, ignored=False)
+    w = torch.empty(vocab, d, dtype=x.dtype, device="cuda").normal_(0.0, 0.3)
+    t = torch.tensor([0, 1, 33554432, 67108863, 67108864, vocab - 1, vocab - 2, vocab, -1], device="cuda")
+    has = (t >= 0) & (t < vocab)
+    g = torch.where(has, k, torch.zeros_like(k)).double()
+    xx = x.double()
+    lse = torch.full((rows,), -math.inf, dtype=torch.float64, device="cuda")
+    for lo in range(0, vocab, step):
+        lse = torch.logaddexp(lse, torch.logsumexp(xx @ w[lo:lo + step].double().t(), 1))
+    dx = torch.zeros(rows, d, dtype=torch.float64, device="cuda")
+    for lo in range(0, vocab, step):
+        ww = w[lo:lo + step].double()
+        dx += torch.exp(xx @ ww.t() - lse[:, None]) @ ww
+    wt = w[t.clamp(0, vocab - 1)].double()
+    loss = torch.where(has, g * (lse - (xx * wt).sum(1)), torch.zeros_like(lse))
+    dx = g[:, None] * (dx - wt)
+    got = ops.softmax_loss_grad(x, w, t, weights=k)
+    # scores are good to 2^-18 (2^-20 of |x||w| < 3 and less); the float32 sums over 2^26 items are joined from some hundred parts
+    # of tiles that are added in pairs: 2^-14 is far above their rounding and far below a row that is read in a wrong place
+    near(torch, got[1], lse, 2.0 ** -14 * lse.abs(), "lse")
+    near(torch, got[0], loss, 2.0 ** -14 * (lse.abs() + 1), "loss")
+    near(torch, got[2], dx, (2 * unit(torch, x.dtype) + 2.0 ** -14) * (dx.abs() + g[:, None]), "d_hidden")
+    at = torch.cat([t[has], torch.tensor([2, 33554431, 33554433, 50000000, 67108865, vocab - 3], device="cuda")])
+    q = torch.exp(xx @ w[at].double().t() - lse[:, None])
+    q = g[:, None] * (q - (t[:, None] == at[None, :]).double())
+    dw = q.t() @ torch.where(has[:, None], xx, torch.zeros_like(xx))
+    # float32: q is multiplied by 2^(14 - e), 2^e >= the largest weight > 2^(e - 1), and cut into two float16, the second to
+    # nearest: where that is subnormal (steps of 2^-24) q is off by 2^-25 2^(e - 14) <= 2^-38 of the largest weight
+    floor = 2.0 ** -38 * float(g.max()) if dtype == "f32" else 0.0
+    near(torch, got[3][at], dw, (4 * unit(torch, x.dtype) + 2.0 ** -14) * (q.abs().t() @ xx.abs()) + floor * torch.where(has[:, None], xx.abs(), torch.zeros_like(xx)).sum(0) + 1e-30, "d_table")
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("rows, d", [(2, 64), (70, 64), (70, 50), (33, 300)])
 def test_softmax_removed_items_hold_anything(env, dtype, rows, d):
@@ -646,7 +683,7 @@ def test_training_step_together(env):
     norm = math.sqrt(sum(float(t.grad.square().sum()) for t in (u, i, b)))
     loss, got_norm, grads = training_step(torch, ops, users, items, bias, ids, targets, weights)
     # 300 rows x 1203 scores of size < 10 in 32 bits: a probability is off by < 2^-16 relatively, every sum by < 2^-15 of its mass
-    assert abs(float(loss.double().sum()) - float(total)) <= 2.0 ** -16 * float((each * weights.double() * has).abs().sum())
+    assert abs(float(loss.double().sum()) - float(total.detach())) <= 2.0 ** -16 * float((each * weights.double() * has).abs().sum())
     factor = min(1.0, 0.05 / norm)
     mass = weights.double().sum() * float(items.abs().max()) * 2
     assert abs(float(got_norm) - norm) <= 2.0 ** -14 * norm
@@ -721,6 +758,61 @@ def test_after_a_session_in_the_same_process(env):
     t = torch.arange(60, device="cuda") % 50
     check_softmax(env, h, w, t, b, None)
     assert np.isfinite(m.predict(np.zeros(50, np.int32), np.arange(50, dtype=np.int32))).all()
+
+
+@pytest.mark.parametrize("max_norm", [0.0, 0.7])
+def test_softmax_epochs_are_these_operators(env, max_norm):
+    """An epoch of LightFM(loss="softmax") over feature matrices against the same steps made of the operators on torch
+    tensors, batch by batch."""
+    torch, ops = env
+    import numpy as np
+    import scipy.sparse as sp
+    from lightfm_amd import LightFM
+    from lightfm_amd.options import options
+    rs = np.random.RandomState(8)
+    n_users, n_items, n, d, batch, lr = 90, 130, 1000, 24, 300, 0.05
+    coo = sp.coo_matrix((np.ones(n, np.float32), (rs.randint(0, n_users, n), rs.randint(0, n_items, n))), shape=(n_users, n_items))
+    fu = sp.random(n_users, 40, 0.1, format="csr", dtype=np.float32, random_state=rs)
+    fi = sp.random(n_items, 30, 0.1, format="csr", dtype=np.float32, random_state=rs)
+    before = {k: getattr(options, k) for k in ("softmax_batch", "softmax_max_norm", "device_shuffle")}
+    m = LightFM(no_components=d, loss="softmax", learning_rate=lr, random_state=4)
+    m._initialize(d, 30, 40)
+    tables = [torch.from_numpy(getattr(m, name).copy()).cuda() for name in ("user_embeddings", "item_embeddings")]
+    bias = torch.zeros(30, 1, device="cuda")
+    order = np.arange(n, dtype=np.int32)
+    state = np.random.RandomState()
+    state.set_state(m.random_state.get_state())
+    state.shuffle(order)
+    try:
+        options.set(softmax_batch=batch, softmax_max_norm=max_norm, device_shuffle=False)
+        m.fit_partial(coo, user_features=fu, item_features=fi, epochs=1)
+    finally:
+        options.set(**before)
+    csr = [[torch.from_numpy(v).cuda() for v in (f.indices.astype(np.int32), f.indptr.astype(np.int32), f.data)] for f in (fu, fi)]
+    u = torch.from_numpy(coo.row.astype(np.int32)).cuda()
+    t = torch.from_numpy(coo.col.astype(np.int32)).cuda()
+    weights = tables + [bias]
+    accumulators = [torch.ones_like(x) for x in weights]
+    for lo in range(0, n, batch):
+        pos = torch.from_numpy(order[lo:lo + batch]).cuda().long()
+        user, item = (ops.embedding_lookup(tables[s], csr[s][0], indptr=csr[s][1], values=csr[s][2]) for s in (0, 1))
+        b = ops.embedding_lookup(bias, csr[1][0], indptr=csr[1][1], values=csr[1][2]).view(-1)
+        h = ops.embedding_lookup(user, u[pos])
+        _, _, dh, di, db = ops.softmax_loss_grad(h, item, t[pos], bias=b, weights=torch.ones(len(pos), device="cuda"))
+        du = ops.embedding_lookup_grad(dh, u[pos], n_users)
+        grads = [ops.embedding_lookup_grad(g, csr[s][0], rows, indptr=csr[s][1], values=csr[s][2])
+                 for g, s, rows in ((du, 0, 40), (di, 1, 30), (db.view(-1, 1), 1, 30))]
+        if max_norm:
+            norm = ops.clip_global_norm(grads, max_norm)
+        for x, acc, g in zip(weights, accumulators, grads):
+            acc.add_(g * g)
+            x.sub_(lr * g / acc.sqrt())
+    if max_norm:
+        assert abs(float(norm) - m._last_epoch_stats[-1]["grad_norm"]) <= 8 * U32 * float(norm)
+    # the same kernels in the same order: what may differ is a rounding in each of the four steps' scaling and update
+    for x, name in zip(weights, ("user_embeddings", "item_embeddings", "item_biases")):
+        want = torch.from_numpy(getattr(m, name)).cuda().view_as(x)
+        assert (x - want).abs().max() <= 4 * 8 * U32 * lr + 4 * U32 * want.abs().max(), name
 
 
 def test_clip_refuses_overlaps_and_tells_autograd(env):
