@@ -448,6 +448,10 @@ struct Pieces {
         if ((units * blocks) >> 32 == 0) return (uint32_t)at / (uint32_t)units;  // (a 64-bit division takes microseconds)
         return (uint32_t)(at / units);
     }
+    __host__ __device__ inline uint32_t owner_of(uint64_t unit) const
+    {
+        return unit >> 32 == 0 ? (uint32_t)unit / tiles : (uint32_t)(unit / tiles);
+    }
     __host__ __device__ inline uint32_t first_block(uint32_t owner) const { return block_of((uint64_t)owner * tiles); }
     __host__ __device__ inline uint32_t last_block(uint32_t owner) const { return block_of((uint64_t)owner * tiles + tiles - 1); }
     // most blocks that one owner is spread over
@@ -512,7 +516,7 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, GRAD)) void rows_
     uint64_t unit = a.pieces.begin(blockIdx.x);
     const uint64_t end = a.pieces.begin(blockIdx.x + 1);
     while (unit < end) {
-        const uint32_t owner = (uint32_t)(unit / a.pieces.tiles), t0 = (uint32_t)(unit - (uint64_t)owner * a.pieces.tiles);
+        const uint32_t owner = a.pieces.owner_of(unit), t0 = (uint32_t)(unit - (uint64_t)owner * a.pieces.tiles);
         const uint64_t left = end - unit;
         const int nt = (int)(a.pieces.tiles - t0 < left ? a.pieces.tiles - t0 : left);
         unit += nt;
@@ -682,7 +686,7 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, true)) void table
     const uint64_t begin = a.pieces.begin(blockIdx.x), end = a.pieces.begin(blockIdx.x + 1);
     uint64_t unit = begin;
     while (unit < end) {
-        const uint32_t owner = (uint32_t)(unit / a.pieces.tiles), t0 = (uint32_t)(unit - (uint64_t)owner * a.pieces.tiles);
+        const uint32_t owner = a.pieces.owner_of(unit), t0 = (uint32_t)(unit - (uint64_t)owner * a.pieces.tiles);
         const uint64_t left = end - unit;
         const int nt = (int)(a.pieces.tiles - t0 < left ? a.pieces.tiles - t0 : left);
         unit += nt;
@@ -733,10 +737,13 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, true)) void table
                 f.target[threadIdx.x] = next_t;
             }
         };
-        __syncthreads();  // (the owner before is done with the tiles)
-        fetch(0, 0);
-        store(0, 0, 0);
-        __syncthreads();
+        // where all rows are one tile it is still there from the owner before
+        if (WIDE || a.pieces.tiles > 1 || unit == begin + 1) {
+            __syncthreads();  // (the owner before is done with the tiles)
+            fetch(0, 0);
+            store(0, 0, 0);
+            __syncthreads();
+        }
         int buf = 0;
         for (int i = 0; i < nt; ++i) {
             if (!WIDE && i + 1 < nt) fetch(i + 1, 0);
@@ -989,7 +996,8 @@ __device__ inline float row_max(float v, float *shared)
 }
 
 // Joins the parts of the table, finishes lse, loss, dx, and leaves table_kernel what it needs.  LANES lanes per row: 16 where
-// there are rows enough to fill the card, a block's 256 (which share the parts, too) where there are few.
+// there are rows enough to fill the card, a block's 256 (which share the parts, too) where there are few; with very few the
+// columns of dx are dealt to blockIdx.y, each of which makes the row's statistics for itself.
 template <typename T, int LANES>
 __global__ __launch_bounds__(256) void join_rows_kernel(JoinArgs j)
 {
@@ -1053,13 +1061,13 @@ __global__ __launch_bounds__(256) void join_rows_kernel(JoinArgs j)
     }
     if (odd && t >= 0) loss = NAN;
     loss = t < 0 ? 0.0f : g * loss;
-    if (lane == 0) {
+    if (lane == 0 && blockIdx.y == 0) {
         a.lse[n] = lse;
         a.loss[n] = loss;
     }
     if (!j.grad) return;
     const bool lost = odd && t >= 0;  // not finite: its gradients are not either
-    if (lane == 0) {
+    if (lane == 0 && blockIdx.y == 0) {
         const int shift = j.shifted == 2 ? 14 - j.scales->eg : j.shifted ? 14 : 0;
         const float gs = ldexpf(g, shift);
         j.row_target[n] = (int32_t)t;
@@ -1069,9 +1077,10 @@ __global__ __launch_bounds__(256) void join_rows_kernel(JoinArgs j)
     }
     const int kw = j.ns == 2 ? j.scales->kw : 0;
     // four columns per lane; with 256 lanes `groups` of them share a column's parts
-    const int columns = j.dp / 4, groups = LANES == 256 ? 256 / columns : 1, group = LANES == 256 ? lane / columns : 0;
-    const int c_first = LANES == 256 ? (lane - group * columns) * 4 : lane * 4;
-    for (int c = c_first; c < j.dp; c += (LANES == 256 ? columns : LANES) * 4) {
+    const int span = LANES == 256 ? j.dp / (int)gridDim.y : j.dp, c_begin = LANES == 256 ? (int)blockIdx.y * span : 0;
+    const int columns = span / 4, groups = LANES == 256 ? 256 / columns : 1, group = LANES == 256 ? lane / columns : 0;
+    const int c_first = c_begin + (LANES == 256 ? lane - group * columns : lane) * 4;
+    for (int c = c_first; c < c_begin + span; c += (LANES == 256 ? columns : LANES) * 4) {
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (t >= 0 && c < a.d && group < groups) {
             const float *pm = j.pm + (int64_t)(c >> 8) * j.parts * a.rows;  // the maxima that chunk c / 256 went by
@@ -1118,15 +1127,22 @@ __global__ __launch_bounds__(256) void join_rows_kernel(JoinArgs j)
     }
 }
 
-// dw and db of the table rows that several blocks share, added in the order of the blocks: block (owner, 32 columns, 32 rows)
+// dw and db of the table rows that several blocks share, added in the order of the blocks: block (owner, 32 columns, 32 rows), or,
+// where there are more owners than blocks, (boundary between two blocks, ...): the others have a block to themselves.
 template <typename T>
 __global__ __launch_bounds__(256) void join_table_kernel(SweepArgs a, int ns)
 {
-    const uint32_t owner = blockIdx.x, b0 = a.pieces.first_block(owner), b1 = a.pieces.last_block(owner);
+    uint32_t owner = blockIdx.x, b0 = blockIdx.x;
+    if (a.pieces.owners > a.pieces.blocks) {  // (an owner lies in two blocks at most)
+        const uint64_t boundary = a.pieces.begin(b0 + 1);
+        owner = a.pieces.owner_of(boundary);
+        if (boundary == (uint64_t)owner * a.pieces.tiles) return;
+    } else
+        b0 = a.pieces.first_block(owner);
+    const uint32_t b1 = a.pieces.last_block(owner);
     if (b0 == b1) return;
     const int shift = a.shifted == 2 ? a.scales->eg - 14 : a.shifted ? -14 : 0, kx = ns == 2 ? a.scales->kx : 0;
-    // only the first of the blocks may have begun with an earlier owner
-    const int64_t first = 2 * (int64_t)b0 + (a.pieces.begin(b0) > (uint64_t)owner * a.pieces.tiles ? 0 : 1);
+    const int64_t first = 2 * (int64_t)b0 + 1;  // the others began inside the owner
     auto part = [&](uint32_t b) { return b == b0 ? first : 2 * (int64_t)b; };
     const int c = (int)blockIdx.y * 32 + (threadIdx.x & 7) * 4;
     const int r = (int)blockIdx.z * 32 + (threadIdx.x >> 3);
@@ -1304,7 +1320,11 @@ template <typename T>
 hipError_t join_rows(JoinArgs j, int64_t parts, hipStream_t st)
 {
     j.aligned = j.a.d % 4 == 0 && ((uintptr_t)j.a.d_hidden & (4 * sizeof(T) - 1)) == 0;
-    if (j.a.rows <= 2048 && parts > 4) join_rows_kernel<T, 256><<<dim3((unsigned)j.a.rows), 256, 0, st>>>(j);
+    if (j.a.rows <= 2048 && parts > 4) {
+        int slices = j.grad ? j.dp / 32 : 1;  // (with every row's dx in one block 32 rows x 200003 x 128: 14.7 us)
+        while (slices > 1 && (j.a.rows * slices > 1024 || j.dp / 32 % slices)) --slices;
+        join_rows_kernel<T, 256><<<dim3((unsigned)j.a.rows, (unsigned)slices), 256, 0, st>>>(j);
+    }
     else join_rows_kernel<T, 16><<<dim3((unsigned)ceil_div(j.a.rows, 16)), 256, 0, st>>>(j);
     return hipGetLastError();
 }
@@ -1418,8 +1438,9 @@ hipError_t run(const lfm_softmax_args &a, bool grad, void *ws, hipStream_t st)
     w.pieces = p.table;
 #define TABLE(DP, WIDE) sweep_table<T, E, NS, DP, WIDE>(w, st)
     BY_WIDTH(p.dp, TABLE)
-    if (e != hipSuccess || p.table.owners % p.table.blocks == 0) return e;  // (no block shares an owner)
-    join_table_kernel<T><<<dim3(p.table.owners, (unsigned)(p.dp / 32), 4), 256, 0, st>>>(w, NS);
+    if (e != hipSuccess || p.table.owners % p.table.blocks == 0 || p.table.tiles == 1) return e;  // (no block shares an owner)
+    const uint32_t shared = p.table.owners > p.table.blocks ? p.table.blocks - 1 : p.table.owners;
+    join_table_kernel<T><<<dim3(shared, (unsigned)(p.dp / 32), 4), 256, 0, st>>>(w, NS);
     return hipGetLastError();
 }
 
