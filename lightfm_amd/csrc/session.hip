@@ -3074,6 +3074,7 @@ extern "C" int lfm_session_epoch_softmax(lfm_session *s, int32_t slot, double it
     opts->grad_norm = opts->kernel_ms = 0.0f;
     if (!s->n) return LFM_OK;
     if (s->itf.rows < 1) return fail(LFM_EINVAL, "the model has no items");
+    if (s->itf.rows > (1 << 30)) return fail(LFM_EUNSUPPORTED, "more than 2^30 items");
     if (std::max(s->itf.nnz, s->usf.nnz) > INT32_MAX - 4096) return fail(LFM_EUNSUPPORTED, "a feature matrix with 2^31 - 4096 entries or more");
     HIP_TRY(hipSetDevice(s->device));
     if (s->stream2) (void)hipStreamSynchronize(s->stream2);  // (left running only by an epoch that failed half-way)

@@ -496,6 +496,28 @@ struct Stream {
 // registers: two waves per SIMD while the operands leave room for it, one beyond
 constexpr int waves_for(int ns, int dp, bool sums) { return ns * dp > (sums ? 192 : 256) ? 1 : 2; }
 
+// A wave's 32 rows x 32 columns of a result on their way to memory: the products leave a lane 4 neighbouring columns of its row,
+// which written as they are make 16-byte pieces (2-byte ones where rows are not aligned); by way of LDS a row's 32 columns
+// are written by neighbouring lanes.
+struct Strip {
+    float v[32][36];
+
+    __device__ inline void write(const f32x16 &out)
+    {
+        const int lane = threadIdx.x & 63;
+        settle();  // (what was read before)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *(float4 *)&v[lane & 31][8 * g + 4 * (lane >> 5)] = make_float4(out[4 * g], out[4 * g + 1], out[4 * g + 2], out[4 * g + 3]);
+        settle();
+    }
+    // the order of a wave's own accesses
+    __device__ static inline void settle() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+    __device__ static inline int row4(int i) { return i * 8 + ((threadIdx.x & 63) >> 3); }
+    __device__ static inline int column4() { return (threadIdx.x & 7) * 4; }
+    __device__ inline float4 read4(int i) const { return *(const float4 *)&v[row4(i)][column4()]; }
+};
+
 // Bound by the matrix pipe and the exponentials together: a block of 32 x 32 scores costs 4 DP matrix cycles per product and
 // about as many for its 16 exponentials, maxima, sums and roundings at DP = 128, which overlap only across the two waves of a
 // SIMD (one wave: 1.5 times the time; three: the operands spill).  8192 x 200003 x 128 bfloat16: 0.90 - 0.94 ms with the
@@ -510,6 +532,7 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, GRAD)) void rows_
     __shared__ __attribute__((aligned(16))) E tile[2][Tl::SIZE];
     __shared__ __attribute__((aligned(16))) float sb[2][Tl::BV];
     __shared__ uint64_t gone[2];  // removed items of a tile
+    __shared__ __attribute__((aligned(16))) Strip strips[GRAD ? 4 : 1];
     const Derived dv = derive(NS == 2 ? a.scales : nullptr);
     const St sm(a.chunks);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
@@ -641,20 +664,23 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, GRAD)) void rows_
             if (i + 1 < nt) clear_removed(i + 1, buf);
         }
         const float sum = half_wave_sum(l);
-        if (n >= a.rows) continue;
-        const int64_t part = (int64_t)(blockIdx.x - a.pieces.first_block(owner)) * a.rows + n;
-        if (h == 0) {
-            const int64_t to = part + (WIDE ? (int64_t)blockIdx.y * a.parts * a.rows : 0);
+        const int64_t part = (int64_t)(blockIdx.x - a.pieces.first_block(owner)) * a.rows;
+        if (h == 0 && n < a.rows) {
+            const int64_t to = part + n + (WIDE ? (int64_t)blockIdx.y * a.parts * a.rows : 0);
             a.pm[to] = m;
             a.pl[to] = sum;
         }
         if (GRAD)
 #pragma unroll
-            for (int b = 0; b < DP / 32; ++b)
+            for (int b = 0; b < DP / 32; ++b) {
+                Strip *strip = &strips[wave];
+                strip->write(out[b]);
 #pragma unroll
-                for (int g = 0; g < 4; ++g)
-                    *(float4 *)(a.po + part * a.dp + (WIDE ? (int)blockIdx.y * DP : 0) + b * 32 + 8 * g + 4 * h) =
-                        make_float4(out[b][4 * g], out[b][4 * g + 1], out[b][4 * g + 2], out[b][4 * g + 3]);
+                for (int i = 0; i < 4; ++i) {
+                    const int64_t r = (int64_t)owner * 128 + wave * 32 + strip->row4(i);
+                    if (r < a.rows) *(float4 *)(a.po + (part + r) * a.dp + (WIDE ? (int)blockIdx.y * DP : 0) + b * 32 + strip->column4()) = strip->read4(i);
+                }
+            }
     }
 }
 
@@ -670,14 +696,18 @@ struct RowFacts {
 
 // Bound like rows_kernel, with more to do per score: maximum, rate and target of a score's row come from LDS.  8192 x 200003 x
 // 128 bfloat16: 1.13 ms, 740 TFLOP/s; 8192 x 26744 x 64 float32: 0.220 ms.
-template <typename T, typename E, int NS, int DP, bool WIDE>
+// ONE: all rows are one tile, which stays in LDS over the owners: few rows, and what counts is how the table is read and dw written
+// (whole calls in us, the general form and this one: 2 x 178913 x 98 bfloat16 110 and 78, 24 x 211856 x 65 float16 100 and 76, 1 x
+// 24380 x 169 float32 77 and 68).  With more tiles the detour by LDS costs registers in the sweep and gains nothing.
+template <typename T, typename E, int NS, int DP, bool WIDE, bool ONE>
 __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, true)) void table_kernel(SweepArgs a)
 {
     typedef Tile<E, NS, DP> Tl;
     typedef Stream<E, NS, DP, WIDE> St;
-    static_assert(!WIDE || St::BLOCKS == 1, "a chunk per tile");
-    __shared__ __attribute__((aligned(16))) E tile[2][Tl::SIZE];
-    __shared__ __attribute__((aligned(16))) RowFacts<Tl::BV> facts[2];
+    static_assert(!WIDE || (St::BLOCKS == 1 && !ONE), "a chunk per tile");
+    __shared__ __attribute__((aligned(16))) E tile[ONE ? 1 : 2][Tl::SIZE];
+    __shared__ __attribute__((aligned(16))) RowFacts<Tl::BV> facts[ONE ? 1 : 2];
+    __shared__ __attribute__((aligned(16))) Strip strips[ONE ? 4 : 1];
     const Derived dv = derive(NS == 2 ? a.scales : nullptr);
     const St sm(a.chunks);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
@@ -737,8 +767,7 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, true)) void table
                 f.target[threadIdx.x] = next_t;
             }
         };
-        // where all rows are one tile it is still there from the owner before
-        if (WIDE || a.pieces.tiles > 1 || unit == begin + 1) {
+        if (!ONE || unit == begin + 1) {
             __syncthreads();  // (the owner before is done with the tiles)
             fetch(0, 0);
             store(0, 0, 0);
@@ -746,7 +775,7 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, true)) void table
         }
         int buf = 0;
         for (int i = 0; i < nt; ++i) {
-            if (!WIDE && i + 1 < nt) fetch(i + 1, 0);
+            if (!WIDE && !ONE && i + 1 < nt) fetch(i + 1, 0);
             const RowFacts<Tl::BV> &f = facts[i & 1];
 #pragma unroll
             for (int blk = 0; blk < St::BLOCKS; ++blk) {
@@ -809,11 +838,42 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, true)) void table
                 p.pack(q);
                 accumulate<E, NS, DP>(out, p, to);
             }
+            if (ONE) break;
             if (i + 1 < nt) store(i + 1, 0, buf ^ 1);
             __syncthreads();
             buf ^= 1;
         }
         const float total = half_wave_sum(db);
+        if constexpr (ONE) {
+            if (a.db && h == 0 && v < a.vocab) a.db[v] = ldexpf(total, shift);
+            Strip *strip = &strips[wave];
+#pragma unroll
+            for (int b = 0; b < DP / 32; ++b) {
+                strip->write(out[b]);
+                if (a.aligned) {
+                    const int c = b * 32 + strip->column4();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int64_t to = (int64_t)w0 + strip->row4(i);
+                        const float4 f = strip->read4(i);
+                        const float o[4] = {f.x, f.y, f.z, f.w};
+                        Vec<T, 4> r;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) r.v[k] = (T)ldexpf(o[k], shift - kx);
+                        if (to < a.vocab && c < a.d) *(Vec<T, 4> *)((T *)a.dw + to * a.d + c) = r;
+                    }
+                } else {
+                    const int c = b * 32 + (lane & 31);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int64_t to = (int64_t)w0 + 2 * i + h;
+                        const float f = strip->v[2 * i + h][lane & 31];
+                        if (to < a.vocab && c < a.d) ((T *)a.dw)[to * a.d + c] = (T)ldexpf(f, shift - kx);
+                    }
+                }
+            }
+            continue;
+        }
         const uint32_t b0 = a.pieces.first_block(owner), b1 = a.pieces.last_block(owner);
         if (b0 != b1) {  // shared with other blocks: the block's first owner, or its last
             const int64_t part = 2 * (int64_t)blockIdx.x + (begin > (uint64_t)owner * a.pieces.tiles ? 0 : 1);
@@ -1290,7 +1350,8 @@ hipError_t sweep_rows(const SweepArgs &s, bool grad, hipStream_t st)
 template <typename T, typename E, int NS, int DP, bool WIDE>
 hipError_t sweep_table(const SweepArgs &s, hipStream_t st)
 {
-    table_kernel<T, E, NS, DP, WIDE><<<dim3(s.pieces.blocks, (unsigned)s.chunks), 256, 0, st>>>(s);
+    if (!WIDE && s.pieces.tiles == 1) table_kernel<T, E, NS, DP, WIDE, !WIDE><<<dim3(s.pieces.blocks), 256, 0, st>>>(s);
+    else table_kernel<T, E, NS, DP, WIDE, false><<<dim3(s.pieces.blocks, (unsigned)s.chunks), 256, 0, st>>>(s);
     return hipGetLastError();
 }
 

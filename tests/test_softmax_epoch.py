@@ -242,6 +242,19 @@ def test_epochs_without_targets_leave_the_model():
 
 
 @pytest.mark.gpu
+def test_feature_matrices_without_entries():
+    """Every representation is zero: a uniform softmax, log(items) per target, and nothing to learn from."""
+    coo, _ = make_data(4, 30, 20, 64)
+    m = LightFM(no_components=8, loss="softmax", random_state=1)
+    m._initialize(8, 5, 6)
+    before = m.item_embeddings.copy(), m.user_embeddings.copy()
+    m.fit_partial(coo, user_features=sp.csr_matrix((30, 6), dtype=np.float32), item_features=sp.csr_matrix((20, 5), dtype=np.float32))
+    assert abs(m._last_epoch_stats[-1]["loss"] - np.log(20)) <= 2.0 ** -20 * np.log(20)
+    assert np.array_equal(before[0], m.item_embeddings) and np.array_equal(before[1], m.user_embeddings)
+    assert not m.item_biases.any()
+
+
+@pytest.mark.gpu
 def test_refused_options_and_divergence():
     coo, _ = make_data(3, 30, 20, 50)
     m = LightFM(no_components=8, loss="softmax", random_state=1)

@@ -683,7 +683,7 @@ def test_training_step_together(env):
     norm = math.sqrt(sum(float(t.grad.square().sum()) for t in (u, i, b)))
     loss, got_norm, grads = training_step(torch, ops, users, items, bias, ids, targets, weights)
     # 300 rows x 1203 scores of size < 10 in 32 bits: a probability is off by < 2^-16 relatively, every sum by < 2^-15 of its mass
-    assert abs(float(loss.double().sum()) - float(total.detach())) <= 2.0 ** -16 * float((each * weights.double() * has).abs().sum())
+    assert abs(float(loss.double().sum()) - float(total.detach())) <= 2.0 ** -16 * float((each * weights.double() * has).abs().sum().detach())
     factor = min(1.0, 0.05 / norm)
     mass = weights.double().sum() * float(items.abs().max()) * 2
     assert abs(float(got_norm) - norm) <= 2.0 ** -14 * norm
