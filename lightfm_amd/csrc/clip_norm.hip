@@ -148,7 +148,9 @@ __global__ __launch_bounds__(256) void scale_kernel(Table t, const double *parti
     // a norm that is not finite (an element was not) scales nothing
     const float f = norm > max_norm && norm < HUGE_VAL ? (float)(max_norm / norm) : 1.0f;
     const int pieces = t.first_piece[t.tensors];
-    // from the last piece to the first: what the norm read last is still in the 256 MB cache
+    // From the last piece to the first: what the norm read last is still in the 256 MB cache, and the results, stored past it
+    // (piece_scale), do not push the first ones out before the next call: 320 M elements of two types 209 + 396 us before, 177 + 408
+    // with both, the order alone gains nothing.
     for (int back = blockIdx.x; back < pieces; back += gridDim.x) {
         const int p = pieces - 1 - back;
         const int i = tensor_of(t, p);
