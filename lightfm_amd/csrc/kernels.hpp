@@ -42,9 +42,12 @@ struct SoftmaxBatch {
     int32_t *users, *targets;
     float *weights;
     unsigned long long *counters;
+    int32_t *first;   // [n_users], SOFTMAX_NOBODY: gets the first position of the batch that is a user's; nullptr = not wanted
+    int32_t *slots;   // [len] that position for every position
     int64_t begin, n;
-    int32_t len;
+    int32_t len, n_users;
 };
+constexpr int32_t SOFTMAX_NOBODY = 0x7f7f7f7f;
 struct SoftmaxTable {
     float *W, *G, *M;
     const float *g;   // summed gradients of the batch, shaped like W
@@ -53,6 +56,11 @@ struct SoftmaxTable {
 };
 struct SoftmaxUpdate {
     SoftmaxTable table[3];  // user embeddings, item embeddings, item biases
+    // user embeddings whose gradient has a row per position instead of one per user (SoftmaxBatch::slots; then table[0].cells is 0):
+    // position i's row is the sum of its user's where slots[i] == i.  `first` is left as it was before the batch.
+    const int32_t *users, *slots;
+    int32_t *first;
+    int32_t d;
     const float *norm;      // global norm of the gradients, or nullptr = not clipped
     float max_norm, lr, rho, eps;
     int32_t adadelta, len, items;

@@ -3053,7 +3053,9 @@ extern "C" int lfm_session_epoch(lfm_session *s, int32_t loss, int32_t slot, dou
 // The softmax loss (include/lfm_hip.h): the operators of ops_common.hpp on the session's tables and stream, a batch at a time.
 //   representations   embedding_lookup over the feature matrices (identity features: the tables themselves)
 //   loss, gradients   softmax_loss of the batch's users against all items
-//   tables' gradients embedding_grad of the same lookups: sorted sums, dense -- the item side has a gradient in every row anyway
+//   tables' gradients embedding_grad of the same lookups: sorted sums, dense -- the item side has a gradient in every row anyway.
+//                     Of users with identity features only those of the batch have one: their rows are summed at the user's first
+//                     position in the batch, so that a step does not touch the whole table (unless an L2 penalty does)
 //   clipping          clip_global_norm's norm; the factor is applied by the update, which reads the gradients in any case
 extern "C" int lfm_session_epoch_softmax(lfm_session *s, int32_t slot, double item_alpha, double user_alpha, lfm_softmax_epoch *opts)
 {
@@ -3088,9 +3090,11 @@ extern "C" int lfm_session_epoch_softmax(lfm_session *s, int32_t slot, double it
     const bool item_ids_only = s->itf.identity, user_ids_only = s->usf.identity;
     int64_t batch = opts->batch ? opts->batch : std::min<int64_t>(8192, std::max<int64_t>(256, n / 64 / 32 * 32));
     batch = std::max<int64_t>(1, std::min(batch, n));
-    const int64_t item_rows = item_ids_only ? items : s->n_feat[0], user_rows = user_ids_only ? users : s->n_feat[1];
+    const bool by_position = user_ids_only && user_alpha == 0.0;
+    const int64_t item_rows = item_ids_only ? items : s->n_feat[0];
+    const int64_t user_rows = by_position ? batch : user_ids_only ? users : s->n_feat[1];
 
-    DBuf<int32_t> b_users, b_targets;
+    DBuf<int32_t> b_users, b_targets, first, slots;
     DBuf<float> b_weights, loss, lse, hidden, d_hidden, user_rep, d_user_rep, item_rep, item_bias, d_item_rep, d_item_bias;
     DBuf<float> dW_user, dW_item, db_item, norm;
     DBuf<double> stats;
@@ -3104,6 +3108,11 @@ extern "C" int lfm_session_epoch_softmax(lfm_session *s, int32_t slot, double it
     LFM_TRY(hidden.alloc((size_t)batch * d));
     LFM_TRY(d_hidden.alloc((size_t)batch * d));
     LFM_TRY(dW_user.alloc((size_t)user_rows * d));
+    if (by_position) {
+        LFM_TRY(first.alloc((size_t)users));
+        LFM_TRY(slots.alloc(batch));
+        HIP_TRY(hipMemsetAsync(first.p, 0x7f, (size_t)users * sizeof(int32_t), s->stream));  // SOFTMAX_NOBODY
+    }
     LFM_TRY(dW_item.alloc((size_t)item_rows * d));
     LFM_TRY(db_item.alloc(item_rows));
     LFM_TRY(norm.alloc(1));
@@ -3169,14 +3178,14 @@ extern "C" int lfm_session_epoch_softmax(lfm_session *s, int32_t slot, double it
     sm.dtype = LFM_F32;
     sm.id_bytes = 4;
     const void *grads[3] = {dW_user.p, dW_item.p, db_item.p};
-    const int64_t counts[3] = {user_rows * d, item_rows * d, item_rows};
+    int64_t counts[3] = {user_rows * d, item_rows * d, item_rows};
     const int32_t types[3] = {LFM_F32, LFM_F32, LFM_F32};
 
     int64_t need = ops::clip_workspace(3, counts);
     for (int64_t rows : {batch, n % batch}) {
         if (!rows) continue;
         need = std::max(need, ops::softmax_workspace(rows, items, d, LFM_F32, true));
-        need = std::max(need, ops::embedding_grad_workspace(rows, users, rows, d, false));
+        need = std::max(need, ops::embedding_grad_workspace(rows, by_position ? rows : users, rows, d, false));
     }
     if (!user_ids_only) need = std::max(need, ops::embedding_grad_workspace(users, s->n_feat[1], s->usf.nnz, d, true));
     if (!item_ids_only) {
@@ -3186,9 +3195,13 @@ extern "C" int lfm_session_epoch_softmax(lfm_session *s, int32_t slot, double it
     LFM_TRY(ws.alloc((size_t)need));
 
     SoftmaxBatch gather = {s->shuffles[slot]->p, s->user_ids.p, s->item_ids.p, s->Y.p, s->weight_aliases_Y ? s->Y.p : s->weight.p,
-                           b_users.p, b_targets.p, b_weights.p, s->counters.p, 0, n, 0};
+                           b_users.p, b_targets.p, b_weights.p, s->counters.p, first.p, slots.p, 0, n, 0, (int32_t)users};
     SoftmaxUpdate update = {};
-    update.table[0] = {s->tab[1][0].p, s->tab[1][1].p, s->tab[1][2].p, dW_user.p, counts[0], 0.0f};
+    update.table[0] = {s->tab[1][0].p, s->tab[1][1].p, s->tab[1][2].p, dW_user.p, by_position ? 0 : counts[0], 0.0f};
+    update.users = b_users.p;
+    update.slots = slots.p;
+    update.first = first.p;
+    update.d = d;
     update.table[1] = {s->tab[0][0].p, s->tab[0][1].p, s->tab[0][2].p, dW_item.p, counts[1], 0.0f};
     update.table[2] = {s->tab[0][3].p, s->tab[0][4].p, s->tab[0][5].p, db_item.p, counts[2], 0.0f};
     update.norm = opts->max_norm > 0.0f ? norm.p : nullptr;
@@ -3223,6 +3236,11 @@ extern "C" int lfm_session_epoch_softmax(lfm_session *s, int32_t slot, double it
         lfm_lookup_args back = pick;
         back.d_out = d_hidden.p;
         back.out = user_ids_only ? dW_user.p : d_user_rep.p;
+        if (by_position) {
+            back.ids = slots.p;
+            back.vocab = rows;
+            counts[0] = rows * d;
+        }
         HIP_TRY(ops::embedding_grad(back, ws.p, s->stream));
         if (!user_ids_only) {
             back = user_bags;

@@ -16,14 +16,26 @@ __global__ __launch_bounds__(256) void softmax_batch_kernel(SoftmaxBatch b)
         b.counters[FAULT_SLOT] = 1ull;
         r = 0;
     }
-    b.users[i] = b.user_ids[r];
+    const int user = b.user_ids[r];
+    b.users[i] = user;
     b.targets[i] = b.Y[r] > 0.0f ? b.item_ids[r] : -1;
     b.weights[i] = b.weight[r];
+    if (b.first && (uint32_t)user < (uint32_t)b.n_users) atomicMin(&b.first[user], i);
+}
+
+__global__ __launch_bounds__(256) void softmax_slots_kernel(SoftmaxBatch b)
+{
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= b.len) return;
+    const int user = b.users[i];
+    b.slots[i] = (uint32_t)user < (uint32_t)b.n_users ? b.first[user] : -1;
 }
 
 hipError_t launch_softmax_batch(const SoftmaxBatch &b, hipStream_t st)
 {
-    softmax_batch_kernel<<<dim3((unsigned)((b.len + 255) / 256)), 256, 0, st>>>(b);
+    const dim3 grid((unsigned)((b.len + 255) / 256));
+    softmax_batch_kernel<<<grid, 256, 0, st>>>(b);
+    if (b.first) softmax_slots_kernel<<<grid, 256, 0, st>>>(b);
     return hipGetLastError();
 }
 
@@ -83,6 +95,27 @@ __global__ __launch_bounds__(256) void softmax_update_kernel(SoftmaxUpdate u)
             if (u.adadelta) tab.M[i] = m;
         }
     }
+    if (u.slots) {  // every user of the batch once, at the user's first position
+        const SoftmaxTable &tab = u.table[0];
+        cell.l2 = 0.0f;
+        const int quads = u.d >> 2;  // (rows are padded to a multiple of four)
+        for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < (int64_t)u.len * quads; q += step) {
+            const int i = (int)(q / quads), c = (int)(q - (int64_t)i * quads);
+            if (u.slots[i] != i) continue;
+            const int64_t at = (int64_t)u.users[i] * quads + c;
+            const float4 g = ((const float4 *)tab.g)[q];
+            float4 w = ((const float4 *)tab.W)[at], a = ((const float4 *)tab.G)[at], m = {};
+            if (u.adadelta) m = ((const float4 *)tab.M)[at];
+            cell(w.x, a.x, m.x, g.x);
+            cell(w.y, a.y, m.y, g.y);
+            cell(w.z, a.z, m.z, g.z);
+            cell(w.w, a.w, m.w, g.w);
+            ((float4 *)tab.W)[at] = w;
+            ((float4 *)tab.G)[at] = a;
+            if (u.adadelta) ((float4 *)tab.M)[at] = m;
+            if (c == 0) u.first[u.users[i]] = SOFTMAX_NOBODY;
+        }
+    }
     if (blockIdx.x == gridDim.x - 1) {  // the batch's loss, in the order of the threads: the same bits every time
         __shared__ double part[256];
         __shared__ int seen[256];
@@ -113,6 +146,7 @@ hipError_t launch_softmax_update(const SoftmaxUpdate &u, int cus, hipStream_t st
 {
     int64_t most = 1;
     for (const SoftmaxTable &t : u.table) most = std::max(most, t.cells);
+    if (u.slots) most = std::max(most, (int64_t)u.len * u.d);
     const int64_t blocks = std::min<int64_t>((most / 4 + 255) / 256 + 1, (int64_t)cus * 8);
     softmax_update_kernel<<<dim3((unsigned)blocks), 256, 0, st>>>(u);
     return hipGetLastError();
