@@ -5,6 +5,7 @@ device is usable, every compute entry point raises.
 """
 import ctypes as C
 import os
+import sys
 
 import numpy as np
 
@@ -102,6 +103,14 @@ def lib():
                 "%s not found: build it with `python -m lightfm_amd.build` "
                 "(the HIP backend has no CPU fallback)" % LIB_PATH)
         l = C.CDLL(LIB_PATH)
+        if "torch" not in sys.modules:
+            # A torch that is imported later brings its own HIP runtime and looks for "libhsa-runtime64.so" below it; two of
+            # THOSE in a process cannot both open the GPU ("No HIP GPUs are available").  Known under that name, too, the one
+            # that this library has loaded serves both.
+            try:
+                C.CDLL("libhsa-runtime64.so")
+            except OSError:
+                pass
         l.lfm_last_error.restype = C.c_char_p
         l.lfm_last_kernel_ms.restype = C.c_float
         for name in EXPORTS:

@@ -5,6 +5,7 @@ import os
 import pickle
 import re
 import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -239,6 +240,27 @@ def test_epochs_without_targets_leave_the_model():
     m.fit_partial(empty, epochs=1)
     assert m._last_epoch_stats[-1]["steps"] == 0
     assert np.array_equal(before[0], m.item_embeddings)
+
+
+@pytest.mark.gpu
+def test_operators_after_a_fit():
+    """A process that has trained before it imports torch can still use torch and the operators on the GPU."""
+    script = """
+import numpy as np, scipy.sparse as sp
+from lightfm_amd import LightFM
+coo = sp.coo_matrix(np.ones((20, 30), np.float32))
+m = LightFM(no_components=8, loss="softmax", random_state=1).fit(coo)
+import torch
+from lightfm_amd import operators
+w = torch.from_numpy(m.item_embeddings).cuda()
+loss, lse = operators.softmax_loss(w, w, torch.arange(30, device="cuda"))
+want = torch.nn.functional.cross_entropy(w.cpu().double() @ w.cpu().double().t(), torch.arange(30), reduction="none")
+assert (loss.cpu().double() - want).abs().max() < 1e-5
+m.fit(coo)
+print("finished")
+"""
+    out = subprocess.run([sys.executable, "-u", "-c", script], cwd=ROOT, capture_output=True, text=True, timeout=110)
+    assert out.returncode == 0 and "finished" in out.stdout, out.stderr[-2000:]
 
 
 @pytest.mark.gpu

@@ -19,6 +19,8 @@ U32 = 2.0 ** -24
 def env():
     import torch
     if not torch.cuda.is_available():
+        from lightfm_amd import _native
+        assert _native.device_count() == 0, "torch does not see the GPU that the library sees"
         pytest.skip("no GPU")
     from lightfm_amd import operators
     return torch, operators
