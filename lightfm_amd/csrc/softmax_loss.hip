@@ -911,11 +911,19 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, true)) void table
 
 // Without the gradient and with up to FEW float32 rows the table is read once, as it is, and multiplied in float32: the
 // matrix form reads it twice and writes it once before it begins.  `lanes` neighbouring lanes own a table row, VEC elements
-// each and step.  Bound by reading the table.  A block leaves the maximum and the sum of its part of the table for each
-// row, like rows_kernel.  Measured (us, with the join; matrix form in brackets): 26744 x 64, one row 14.6 (24), 8 rows 23.8 (24.8), 16 rows
-// 32.5 (24.8); 200003 x 128: 31 (134), 102 (134), 189 (135).  Half-precision tables need no packing where their rows are 16-byte
-// aligned, and the matrix form is then the faster one from one row on (26744 x 64: 10.5).
+// each and step.  Bound by reading the table with one row, by the products and exponentials with more.  A block leaves the
+// maximum and the sum of its part of the table for each row, like rows_kernel.  Measured (us for 1 / 2 / 4 / 8 rows, with the join;
+// matrix form in brackets): 26744 x 64 9.9 / 11.7 / 15.2 / 17.2 (23), 200003 x 128 26 / 36 / 57 / 96 (84), 60000 x 50 12 / 15 / 22 / 35 (31),
+// 59803 x 51 16 / 23 / 37 / 65 (33), 100000 x 301 37 / 48 / 72 / 123 (226): up to four rows, and up to eight where the table is small
+// or wider than a chunk.  Half-precision tables need no packing where their rows are 16-byte aligned, and the matrix form is then the
+// faster one from one row on (26744 x 64: 10.5).
 constexpr int FEW = 8;
+
+bool takes_few(int64_t rows, int64_t vocab, int d, int dtype, bool grad)
+{
+    if (grad || dtype != LFM_F32) return false;
+    return rows <= 4 || (rows <= FEW && (d > 256 || (d % 4 == 0 && vocab * d <= 4000000)));
+}
 
 template <int VEC, int ROWS>
 __global__ __launch_bounds__(256) void few_rows_kernel(SweepArgs a, const float *hidden, const float *table, int lanes_log2)
@@ -1056,7 +1064,7 @@ __device__ inline float row_max(float v, float *shared)
 }
 
 // Joins the parts of the table, finishes lse, loss, dx, and leaves table_kernel what it needs.  LANES lanes per row: 16 where
-// there are rows enough to fill the card, a block's 256 (which share the parts, too) where there are few; with very few the
+// there are rows enough to fill the card or little to join, a block's 256 (which share the parts, too) elsewhere; with very few the
 // columns of dx are dealt to blockIdx.y, each of which makes the row's statistics for itself.
 template <typename T, int LANES>
 __global__ __launch_bounds__(256) void join_rows_kernel(JoinArgs j)
@@ -1289,7 +1297,7 @@ Plan plan_for(int64_t rows, int64_t vocab, int d, int dtype, bool grad)
     // slots: blocks that run at once on the card's 256 compute units
     p.rows = pieces_for(rows, vocab, bv, 256 * (p.chunks > 1 ? 1 : waves_for(p.ns, w, grad)));
     p.few = 0;
-    if (!grad && dtype == LFM_F32 && rows <= FEW) {
+    if (takes_few(rows, vocab, d, dtype, grad)) {
         const int64_t want = ceil_div(vocab, 16);  // (a block's lane groups have a few table rows each)
         p.few = (int)(want < 1024 ? want : 1024);
     }
@@ -1372,8 +1380,11 @@ hipError_t launch_few(const SweepArgs &w, const lfm_softmax_args &a, int blocks,
     int ll = 0;
     while ((1 << ll) * VEC < a.d && ll < 6) ++ll;
     const float *x = (const float *)a.hidden, *t = (const float *)a.table;
-    if (a.rows == 1) few_rows_kernel<VEC, 1><<<dim3((unsigned)blocks), 256, 0, st>>>(w, x, t, ll);
-    else few_rows_kernel<VEC, FEW><<<dim3((unsigned)blocks), 256, 0, st>>>(w, x, t, ll);
+    const dim3 grid((unsigned)blocks);
+    if (a.rows == 1) few_rows_kernel<VEC, 1><<<grid, 256, 0, st>>>(w, x, t, ll);
+    else if (a.rows == 2) few_rows_kernel<VEC, 2><<<grid, 256, 0, st>>>(w, x, t, ll);
+    else if (a.rows <= 4) few_rows_kernel<VEC, 4><<<grid, 256, 0, st>>>(w, x, t, ll);
+    else few_rows_kernel<VEC, FEW><<<grid, 256, 0, st>>>(w, x, t, ll);
     return hipGetLastError();
 }
 
@@ -1381,7 +1392,7 @@ template <typename T>
 hipError_t join_rows(JoinArgs j, int64_t parts, hipStream_t st)
 {
     j.aligned = j.a.d % 4 == 0 && ((uintptr_t)j.a.d_hidden & (4 * sizeof(T) - 1)) == 0;
-    if (j.a.rows <= 2048 && parts > 4) {
+    if (j.a.rows <= 2048 && parts > (j.grad ? 4 : 64)) {
         int slices = j.grad ? j.dp / 32 : 1;  // (with every row's dx in one block 32 rows x 200003 x 128: 14.7 us)
         while (slices > 1 && (j.a.rows * slices > 1024 || j.dp / 32 % slices)) --slices;
         join_rows_kernel<T, 256><<<dim3((unsigned)j.a.rows, (unsigned)slices), 256, 0, st>>>(j);
@@ -1411,6 +1422,9 @@ hipError_t run(const lfm_softmax_args &a, bool grad, void *ws, hipStream_t st)
     // both operands can be read four elements at a time
     const bool wide = a.d % 4 == 0 && a.hidden_stride % 4 == 0 && a.table_stride % 4 == 0 &&
                       (((uintptr_t)a.hidden | (uintptr_t)a.table) & (4 * sizeof(T) - 1)) == 0;
+    // ... or two
+    const bool two = a.d % 2 == 0 && a.hidden_stride % 2 == 0 && a.table_stride % 2 == 0 &&
+                     (((uintptr_t)a.hidden | (uintptr_t)a.table) & (2 * sizeof(T) - 1)) == 0;
     SweepArgs w = {};
     w.rows = a.rows;
     w.vocab = a.vocab;
@@ -1428,7 +1442,7 @@ hipError_t run(const lfm_softmax_args &a, bool grad, void *ws, hipStream_t st)
     if (NS == 2 && p.few) {
         w.ldx = a.hidden_stride;
         w.ldw = a.table_stride;
-        e = wide ? launch_few<4>(w, a, p.few, st) : launch_few<1>(w, a, p.few, st);
+        e = wide ? launch_few<4>(w, a, p.few, st) : two ? launch_few<2>(w, a, p.few, st) : launch_few<1>(w, a, p.few, st);
         if (e != hipSuccess) return e;
         j.ns = 1;
         j.few = 1;
