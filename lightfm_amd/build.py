@@ -80,6 +80,8 @@ def build(force=False, verbose=False):
     binding, src = os.path.join(OUT_DIR, "_torch_ops.so"), os.path.join(CSRC, TORCH_OPS)
     if importlib.util.find_spec("torch") and (force or _stale(binding, [src, OPS_LIB, hdrs[1]])):
         import torch
+        if torch.version.hip is None:
+            return LIB
         root = os.path.dirname(torch.__file__)
         run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-w", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
              "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI), "-I" + os.path.join(root, "include"),

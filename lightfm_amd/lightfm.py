@@ -162,6 +162,8 @@ class _Session(object):
     def epoch_softmax(self, item_alpha, user_alpha, slot=0):
         """One epoch of the softmax loss (lfm_session_epoch_softmax) with options.softmax_batch / softmax_max_norm;
         returns what it did as a dict: kernel_ms, loss (mean per target), targets, steps, grad_norm."""
+        if not 0 <= int(options.softmax_batch) <= 1 << 20:
+            raise ValueError("softmax_batch must lie in [0, 2^20]")
         o = N.LfmSoftmaxEpoch(batch=int(options.softmax_batch), max_norm=float(options.softmax_max_norm))
         N.check(N.lib().lfm_session_epoch_softmax(self.handle, slot, C.c_double(item_alpha), C.c_double(user_alpha),
                                                   C.byref(o)))
@@ -308,7 +310,7 @@ class LightFM(object):
     against ALL items instead of sampled negatives.  It trains in batches, one optimizer step each
     (options.softmax_batch, options.softmax_max_norm; include/lfm_hip.h: lfm_session_epoch_softmax),
     so the same random_state gives the same model bit for bit; k, n, max_sampled and num_threads have
-    no meaning for it, and user biases keep their initial zeros (they shift all scores of a user alike).
+    no meaning for it, and user biases are left as they are (they shift all scores of a user alike).
     """
 
     def __init__(self, no_components=10, k=5, n=10, learning_schedule="adagrad", loss="logistic",

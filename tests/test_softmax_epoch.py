@@ -280,7 +280,7 @@ def test_feature_matrices_without_entries():
 def test_refused_options_and_divergence():
     coo, _ = make_data(3, 30, 20, 50)
     m = LightFM(no_components=8, loss="softmax", random_state=1)
-    for bad in (dict(softmax_batch=-1), dict(softmax_max_norm=-1.0), dict(softmax_max_norm=float("nan"))):
+    for bad in (dict(softmax_batch=-1), dict(softmax_batch=(1 << 32) + 5), dict(softmax_max_norm=-1.0), dict(softmax_max_norm=float("nan"))):
         options.set(softmax_batch=0, softmax_max_norm=0.0)
         options.set(**bad)
         with pytest.raises(ValueError):
