@@ -204,6 +204,20 @@ def test_softmax_nothing_left(env, dtype, rows):
     near(torch, lse, torch.full_like(lse, torch.finfo(torch.float32).min).double(), torch.tensor(2.0 ** 105, device="cuda").double(), "lse")
 
 
+@pytest.mark.parametrize("d", [1, 50, 51, 64, 257, 300])
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 8, 9])
+def test_softmax_few_float32_rows(env, rows, d):
+    check_softmax(env, *make(env[0], rows, 3001, d, "f32", seed=rows, ignored=rows > 4))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows, d", [(2, 98), (31, 128), (32, 65), (33, 200), (64, 96), (65, 128), (64, 32), (20, 256)])
+def test_softmax_one_tile_of_rows(env, rows, d, dtype):
+    """At and around the number of rows that is one tile of the table's sweep (64, or 32 for wide rows); the table ends inside
+    the last owner of 128."""
+    check_softmax(env, *make(env[0], rows, 9011, d, dtype, seed=rows + d))
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_softmax_offsets_past_32_bits(env, dtype):
     """A table of more than 2^32 elements: scores, gradients and targets at both ends of it."""
@@ -724,6 +738,58 @@ def test_captured_step_replays(env):
         for (loss, norm, grads), (l2, n2, g2) in zip(results, want):
             assert torch.equal(loss, l2) and torch.equal(norm, n2)
             assert all(torch.equal(a, b) for a, b in zip(grads, g2))
+
+
+FORMS = [  # what has a form of its own: few rows, one tile of rows, parts to join or none, short and long lists of ids
+    ("loss", 1, 5000, 64, "f32"), ("loss", 2, 3001, 50, "f32"), ("loss", 4, 3001, 51, "f32"), ("loss", 7, 900, 300, "f32"), ("loss", 700, 5000, 64, "f32"),
+    ("grad", 3, 9000, 98, "bf16"), ("grad", 60, 20011, 40, "f16"), ("grad", 1003, 50021, 100, "f16"), ("grad", 500, 400, 20, "f32"),
+    ("grad", 40, 600, 520, "f32"), ("grad", 0, 50, 8, "f32"),
+    ("ids", 300, 1000, 30, "f32"), ("ids", 5000, 90000, 64, "bf16"), ("ids", 80001, 40, 12, "f32"), ("ids", 210001, 300007, 8, "f16"),
+    ("bags", 0, 10, 5, "f32"), ("bags", 800, 3000, 33, "f32")]
+
+
+@pytest.mark.parametrize("kind, rows, vocab, d, dtype", FORMS)
+def test_captured_forms_replay(env, kind, rows, vocab, d, dtype):
+    torch, ops = env
+
+    def inputs(seed):
+        if kind in ("loss", "grad"):
+            return make(torch, rows, vocab, d, dtype, seed=seed)
+        ids, indptr, values = bags(torch, rows, vocab, 4 if kind == "bags" else 0, seed=seed)
+        g = torch.Generator(device="cuda")
+        g.manual_seed(seed)
+        if kind == "bags":  # (as many ids for every seed, so that they can be copied)
+            indptr = torch.arange(0, 4 * rows + 1, 4, device="cuda", dtype=ids.dtype)
+            ids = torch.randint(-1, vocab, (4 * rows,), generator=g, device="cuda").to(ids.dtype)
+            values = torch.rand(4 * rows, generator=g, device="cuda")
+        x = torch.randn(rows, d, generator=g, device="cuda").to(getattr(torch, DTYPE[dtype]))
+        w = torch.randn(vocab, d, generator=g, device="cuda").to(getattr(torch, DTYPE[dtype]))
+        return [t for t in (x, w, ids, indptr, values) if t is not None]
+
+    def call(a):
+        if kind in ("loss", "grad"):
+            return (ops.softmax_loss_grad if kind == "grad" else ops.softmax_loss)(a[0], a[1], a[2], bias=a[3], weights=a[4])
+        more = dict(indptr=a[3], values=a[4]) if kind == "bags" else {}
+        return ops.embedding_lookup(a[1], a[2], **more), ops.embedding_lookup_grad(a[0], a[2], vocab, **more)
+
+    held = inputs(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(held)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        results = call(held)
+    for turn in range(1, 4):
+        fresh = inputs(turn)
+        want = call(fresh)
+        for a, b in zip(held, fresh):
+            a.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, exact in zip(results, want):
+            assert torch.equal(got, exact)
 
 
 def test_two_streams_at_once(env):
