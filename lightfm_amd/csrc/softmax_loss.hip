@@ -130,8 +130,8 @@ __device__ inline int64_t target_of(const lfm_softmax_args &a, int64_t n)
 // -------------------------------------------------------------- operands ---
 
 // Largest finite magnitudes: `parts` blocks for x (rows with a target; their outlier flags are cleared on the way), as many
-// for w (float32 operands alone), as many for g.  Threads take four columns of a row each; WIDE_LOADS: at once.
-template <typename T, bool WIDE_LOADS>
+// for w (float32 operands alone), as many for g.  Threads take four columns of a row each, LOAD (4, 2, 1) of them at once.
+template <typename T, int LOAD>
 __global__ __launch_bounds__(256) void largest_kernel(lfm_softmax_args a, int parts, float *largest, int tensors, uint8_t *outlier)
 {
     const int which = blockIdx.x / parts, part = blockIdx.x % parts;
@@ -151,12 +151,13 @@ __global__ __launch_bounds__(256) void largest_kernel(lfm_softmax_args a, int pa
                 } else if (removed(a.bias, r))
                     continue;
                 const T *q = p + r * stride + c;
-                if (WIDE_LOADS) {
-                    const Vec<T, 4> v = *(const Vec<T, 4> *)q;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) look((float)v.v[j]);
-                } else
-                    for (int j = 0; j < 4 && c + j < a.d; ++j) look((float)q[j]);
+                for (int j = 0; j < 4; j += LOAD) {
+                    if (c + j >= a.d) break;
+                    const Vec<T, LOAD> v = *(const Vec<T, LOAD> *)(q + j);
+#pragma unroll
+                    for (int i = 0; i < LOAD; ++i) look((float)v.v[i]);
+                }
             }
     } else {
         for (int64_t i = (int64_t)part * 256 + threadIdx.x; i < a.rows; i += (int64_t)parts * 256) {
@@ -191,8 +192,8 @@ struct PackArgs {
 };
 
 // Rows of x and w to the padded, split form, zeros behind d: per row and chunk of `width` columns [hi: width | lo: width]
-// (width = dp up to 256 columns, 256 beyond).  A thread makes 8 elements; WIDE_LOADS: reads them 4 at once.
-template <typename T, typename E, int NS, bool WIDE_LOADS>
+// (width = dp up to 256 columns, 256 beyond).  A thread makes 8 elements and reads LOAD (4, 2, 1) of them at once.
+template <typename T, typename E, int NS, int LOAD>
 __global__ __launch_bounds__(256) void pack_kernel(PackArgs p, int dp, int width)
 {
     __shared__ int ks[3];
@@ -224,26 +225,24 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs p, int dp, int width
         const T *src = is_x ? (const T *)p.a.hidden + r * p.a.hidden_stride : (const T *)p.a.table + r * p.a.table_stride;
         E *dst = (E *)(is_x ? p.x : p.w) + r * (NS * dp) + at;
         const bool gone = !is_x && removed(p.a.bias, r);
-        Vec<T, 4> v[2];
+        T v[8];
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            const int cq = c + 4 * q;
-            if (gone) v[q] = {};
-            else if (WIDE_LOADS && cq + 4 <= p.a.d) v[q] = *(const Vec<T, 4> *)(src + cq);
-            else
+        for (int q = 0; q < 8; q += LOAD) {
+            Vec<T, LOAD> part = {};
+            if (!gone && c + q < p.a.d) part = *(const Vec<T, LOAD> *)(src + c + q);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[q].v[j] = cq + j < p.a.d ? src[cq + j] : (T)0.0f;
+            for (int j = 0; j < LOAD; ++j) v[q + j] = part.v[j];
         }
         x8 hi, lo;
         if (NS == 1) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) hi[j] = (E)v[j >> 2].v[j & 3];
+            for (int j = 0; j < 8; ++j) hi[j] = (E)v[j];
         } else {
             const int k = ks[is_x ? 0 : 1];
             bool fits = true;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                float f = ldexpf((float)v[j >> 2].v[j & 3], k);
+                float f = ldexpf((float)v[j], k);
                 if (is_x && !(fabsf(f) < 65504.0f)) { fits = false; f = 0.0f; }
                 hi[j] = (E)f;
                 lo[j] = (E)(f - (float)hi[j]);
@@ -1461,8 +1460,9 @@ hipError_t run(const lfm_softmax_args &a, bool grad, void *ws, hipStream_t st)
     pk.parts = (int)(ceil_div(most, 4096) < MAX_PARTS ? ceil_div(most, 4096) : MAX_PARTS);
     if (scales) {
         const dim3 grid((unsigned)(pk.tensors * pk.parts));
-        if (wide) largest_kernel<T, true><<<grid, 256, 0, st>>>(a, pk.parts, s.largest, pk.tensors, s.outlier);
-        else largest_kernel<T, false><<<grid, 256, 0, st>>>(a, pk.parts, s.largest, pk.tensors, s.outlier);
+        if (wide) largest_kernel<T, 4><<<grid, 256, 0, st>>>(a, pk.parts, s.largest, pk.tensors, s.outlier);
+        else if (two) largest_kernel<T, 2><<<grid, 256, 0, st>>>(a, pk.parts, s.largest, pk.tensors, s.outlier);
+        else largest_kernel<T, 1><<<grid, 256, 0, st>>>(a, pk.parts, s.largest, pk.tensors, s.outlier);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     if (scales || pk.x || pk.w) {
@@ -1470,8 +1470,9 @@ hipError_t run(const lfm_softmax_args &a, bool grad, void *ws, hipStream_t st)
         int64_t blocks = ceil_div((pk.x ? a.rows : 0) + (pk.w ? a.vocab : 0), per);
         blocks = blocks < 1 ? 1 : blocks > 4096 ? 4096 : blocks;
         const int width = p.dp < 256 ? p.dp : 256;
-        if (wide) pack_kernel<T, E, NS, true><<<dim3((unsigned)blocks), 256, 0, st>>>(pk, p.dp, width);
-        else pack_kernel<T, E, NS, false><<<dim3((unsigned)blocks), 256, 0, st>>>(pk, p.dp, width);
+        if (wide) pack_kernel<T, E, NS, 4><<<dim3((unsigned)blocks), 256, 0, st>>>(pk, p.dp, width);
+        else if (two) pack_kernel<T, E, NS, 2><<<dim3((unsigned)blocks), 256, 0, st>>>(pk, p.dp, width);
+        else pack_kernel<T, E, NS, 1><<<dim3((unsigned)blocks), 256, 0, st>>>(pk, p.dp, width);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     w.x = x_there ? a.hidden : s.x;
