@@ -21,8 +21,8 @@
 // left out is 2^-22 of the term: the size of float32's own rounding over a sum, at a third of the float16 rate instead of the
 // float32 pipe's 1/16.  The probabilities that enter the second product are split the same way: those of dw, scaled so that the
 // largest weight is 2^14, are off by 2^-38 of it at most, so a probability below 2^-17 or so has fewer bits than float32's.  Half-precision operands
-// are multiplied as they are; their probabilities are rounded once to the operands' type (to nearest: 2^-9 / 2^-12
-// relative, below the rounding of the result).  All sums, maxima and statistics are float32.
+// are multiplied as they are; their probabilities are rounded once to the operands' type (to nearest: at most 2^-8 / 2^-11
+// relative, as much as the result's own rounding).  All sums, maxima and statistics are float32.
 #include "ops_common.hpp"
 
 #include <math.h>
