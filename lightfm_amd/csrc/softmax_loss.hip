@@ -1105,7 +1105,8 @@ __global__ __launch_bounds__(256) void join_rows_kernel(JoinArgs j)
         loss = st == -INFINITY ? INFINITY : l <= e ? log1pf(l / e) : ldexpf(m - su, -dv.k) + (logf(l + e) - P_SHIFT * LN2);
     }
     const float sum = l + e;
-    float lse = sum == 0.0f ? -INFINITY : m <= dv.low * 0.999f ? -3.402823466e38f : ldexpf(m, -dv.k) + (logf(sum) - P_SHIFT * LN2);
+    // (m says nothing about a row of NaN, which no maximum takes in: its sum does)
+    float lse = sum != sum ? sum : sum == 0.0f ? -INFINITY : m <= dv.low * 0.999f ? -3.402823466e38f : ldexpf(m, -dv.k) + (logf(sum) - P_SHIFT * LN2);
     const float other = sum == 0.0f ? 1.0f : l / sum;  // 1 - p[target]
     const bool odd = j.ns == 2 && j.outlier[n];
     if (odd) {  // a row beyond x's scale: not finite, or without a target and far larger than the others

@@ -1,0 +1,37 @@
+"""The softmax operators where a row, an item or a whole batch is out of the ordinary: values that are not finite, targets
+that are masked, rows without a target that are far larger than the others, batches without any target, probabilities far
+below the others.  Bounds are derived as in test_zz_torch_operators."""
+import math
+
+import pytest
+
+from tests.test_zz_torch_operators import env, make  # noqa: F401  (env is a fixture)
+
+pytestmark = pytest.mark.gpu
+
+FORMS = [(1, 64), (3, 40), (4, 51), (7, 300), (90, 64), (90, 50), (70, 300), (2500, 64)]
+
+
+def both(ops, x, w, t, b, k):
+    """The loss alone and with its gradients (forms of their own where there are few rows)."""
+    return ops.softmax_loss(x, w, t, bias=b, weights=k), ops.softmax_loss_grad(x, w, t, bias=b, weights=k)
+
+
+# ---------------------------------------------------------------- not finite ---
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows, d", FORMS)
+def test_lse_of_rows_that_are_not_numbers(env, rows, d, dtype):
+    """A hidden row of NaN has a lse of NaN, with a target (and then its loss is NaN) and without one (loss 0).  The other
+    rows have the bits that they have beside rows of zeros."""
+    torch, ops = env
+    x, w, t, b, k = make(torch, rows, 333, d, dtype, seed=31, ignored=False)
+    lost = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    lost[[0, rows // 2, rows - 1]] = True
+    t[rows - 1] = -1
+    clean = both(ops, torch.where(lost[:, None], torch.zeros_like(x), x), w, t, b, k)
+    x[lost] = float("nan")
+    for got, want in zip(both(ops, x, w, t, b, k), clean):
+        assert torch.isnan(got[1][lost]).all()
+        assert torch.equal(got[1][~lost], want[1][~lost]) and torch.equal(got[0][~lost], want[0][~lost])
+        assert (got[0][t < 0] == 0).all() and torch.isnan(got[0][lost & (t >= 0)]).all()
