@@ -39,10 +39,13 @@ const char *lfm_ops_last_error(void);
  *   q[n, v] = weights[n] * (exp(s[n, v] - lse[n]) - [v == targets[n]])     (0 for a row without a target),
  *   d_hidden = q table,  d_table = q^T hidden,  d_bias[v] = sum_n q[n, v].
  * The logits are never written to memory.  bias / weights may be NULL (0 / 1); d_bias may be NULL.  A bias of -inf
- * removes an item: its row of the table is not looked at, whatever it holds, and has a zero gradient (as a target, its loss is
- * infinite).  Rows of hidden and table are contiguous, `*_stride` elements apart; the gradients are dense.
+ * removes an item: its row of the table is not looked at, whatever it holds, and has a zero gradient.  As the target of row n
+ * its loss is infinite and the gradients are the formula's with a probability of 0: -weights[n] table[v] in d_hidden[n]
+ * (elements of that row that are not finite count as 0), -weights[n] hidden[n] in d_table[v], -weights[n] in d_bias[v].
+ * Rows of hidden and table are contiguous, `*_stride` elements apart; the gradients are dense.
  * float32 operands keep 22 bits and a floor of 2^-39 of the largest magnitude of hidden (rows with a target) or table (items not
- * removed); the terms q of d_table keep 22 bits and an absolute error of 2^-38 of the largest weight.  At most 2^27 rows and 2^30 items. */
+ * removed); the terms q of d_table keep 22 bits and an absolute error of 2^-38 of the largest weight.  At most 2^27 rows and
+ * 2^30 items. */
 typedef struct lfm_softmax_args {
     const void *hidden, *table; /* [rows, d], [vocab, d] of `dtype` */
     const void *targets;        /* [rows] int32 or int64 */

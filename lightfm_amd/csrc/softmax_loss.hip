@@ -1081,10 +1081,11 @@ __global__ __launch_bounds__(256) void join_rows_kernel(JoinArgs j)
     const float g = t < 0 ? 0.0f : a.weights ? a.weights[n] : 1.0f;
     const T *x = (const T *)a.hidden + n * a.hidden_stride;
     const T *wt = (const T *)a.table + (t < 0 ? 0 : t) * a.table_stride;
+    const bool out = t >= 0 && removed(a.bias, t);  // its score is -inf, whatever its row holds
     float m = -INFINITY, l = 0.0f, st = 0.0f;
 #pragma unroll 4
     for (int s = lane; s < splits; s += LANES) m = fmaxf(m, j.pm[(int64_t)s * a.rows + n]);
-    if (t >= 0)
+    if (t >= 0 && !out)
         for (int c = lane; c < a.d; c += LANES) st = __builtin_fmaf((float)x[c], (float)wt[c], st);
     m = row_max<LANES>(m, shared);
 #pragma unroll 4
@@ -1184,7 +1185,8 @@ __global__ __launch_bounds__(256) void join_rows_kernel(JoinArgs j)
             float v = 0.0f;
             if (t >= 0 && c + k < a.d) {
                 v = sum == 0.0f ? 0.0f : ldexpf(ov[k] / sum, -kw);
-                v = lost ? NAN : g * (v - other * (float)wt[c + k]);
+                const float wv = (float)wt[c + k];
+                v = lost ? NAN : g * (v - other * (out && !(fabsf(wv) < INFINITY) ? 0.0f : wv));
             }
             r.v[k] = (T)v;
         }

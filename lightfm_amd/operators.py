@@ -80,14 +80,16 @@ def softmax_loss(hidden, table, targets, bias=None, weights=None):
     """Cross entropy of every row of `hidden` [rows, d] against all rows of `table` [vocab, d]: scores
     s = hidden table^T + bias, lse = log sum exp s, loss = weights * (lse - s[target]).  Returns (loss, lse), float32
     [rows]; a row whose target is not in [0, vocab) has loss 0.  bias [vocab] / weights [rows] are float32; a bias of
-    -inf takes an item out of the softmax, whatever its row holds.  The scores are never kept.  float32 operands are
-    multiplied with 22 bits and a floor of 2^-39 of the largest magnitude of hidden or table."""
+    -inf takes an item out of the softmax, whatever its row holds (as a target, its loss is infinite).  The scores are never
+    kept.  float32 operands are multiplied with 22 bits and a floor of 2^-39 of the largest magnitude of hidden or table."""
     return _ops.softmax(hidden, table, targets, bias, weights, False)
 
 
 def softmax_loss_grad(hidden, table, targets, bias=None, weights=None):
     """softmax_loss with the gradients of the SUM of the losses: (loss, lse, d_hidden, d_table, d_bias); d_bias is None
-    without a bias.  For the mean, hand in weights of 1 / rows.  Gradients have the type of hidden / table."""
+    without a bias.  For the mean, hand in weights of 1 / rows.  Gradients have the type of hidden / table.  An item that a
+    bias of -inf takes out has a zero gradient but where it is a target: there the probability is 0 and the gradients follow the
+    formula (elements of its row that are not finite count as 0)."""
     return _ops.softmax(hidden, table, targets, bias, weights, True)
 
 

@@ -35,3 +35,32 @@ def test_lse_of_rows_that_are_not_numbers(env, rows, d, dtype):
         assert torch.isnan(got[1][lost]).all()
         assert torch.equal(got[1][~lost], want[1][~lost]) and torch.equal(got[0][~lost], want[0][~lost])
         assert (got[0][t < 0] == 0).all() and torch.isnan(got[0][lost & (t >= 0)]).all()
+
+
+# ------------------------------------------------------------ masked targets ---
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows, d", FORMS)
+@pytest.mark.parametrize("left", [True, False])
+def test_targets_that_are_removed_items(env, rows, d, dtype, left):
+    """A target whose bias is -inf and whose row holds NaN or infinities: its loss is infinite, everything else is what it is
+    with a row of zeros, bit for bit.  left: there are items besides the removed ones."""
+    torch, ops = env
+    x, w, t, b, k = make(torch, rows, 333, d, dtype, seed=32, ignored=False)
+    b[[5, 64, 200, 332]] = -math.inf
+    if not left:
+        b[:] = -math.inf
+    w[[5, 64, 200, 332]] = 0
+    t[0], t[rows // 2], t[rows - 1] = 5, 64, 332
+    if rows > 10:
+        t[3] = 200
+    out = torch.isinf(b[t.long()])
+    clean = both(ops, x, w, t, b, k)
+    w[5], w[64], w[200] = float("nan"), math.inf, -math.inf
+    w[332, d // 2] = float("nan")
+    for got, want in zip(both(ops, x, w, t, b, k), clean):
+        assert (got[0][out] == math.inf).all() and torch.isfinite(got[0][~out]).all()
+        for i, (g, c) in enumerate(zip(got, want)):
+            assert torch.equal(g, c), i
+            if i > 1:
+                assert torch.isfinite(g).all(), i
