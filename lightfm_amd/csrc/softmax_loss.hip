@@ -1103,7 +1103,9 @@ __global__ __launch_bounds__(256) void join_rows_kernel(JoinArgs j)
         e = exp2_fast((su - up) * dv.c + P_SHIFT);
         l *= exp2_fast((m - up) * dv.c);
         m = up;
-        loss = st == -INFINITY ? INFINITY : l <= e ? log1pf(l / e) : ldexpf(m - su, -dv.k) + (logf(l + e) - P_SHIFT * LN2);
+        // a score below the products' range (a mask) is cut there, which a probability of 0 does not show, but the loss would
+        const float behind = su <= dv.low && m > su ? ldexpf(m, -dv.k) - st : ldexpf(m - su, -dv.k);
+        loss = st == -INFINITY ? INFINITY : l <= e ? log1pf(l / e) : behind + (logf(l + e) - P_SHIFT * LN2);
     }
     const float sum = l + e;
     // (m says nothing about a row of NaN, which no maximum takes in: its sum does)

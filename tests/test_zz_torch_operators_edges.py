@@ -5,7 +5,7 @@ import math
 
 import pytest
 
-from tests.test_zz_torch_operators import env, make  # noqa: F401  (env is a fixture)
+from tests.test_zz_torch_operators import U32, env, make  # noqa: F401  (env is a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -64,3 +64,27 @@ def test_targets_that_are_removed_items(env, rows, d, dtype, left):
             assert torch.equal(g, c), i
             if i > 1:
                 assert torch.isfinite(g).all(), i
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("mask", [-1e30, -3.402823466e38])
+@pytest.mark.parametrize("rows, d", [(1, 64), (3, 40), (7, 300), (90, 64), (70, 300), (2500, 64)])
+def test_targets_that_are_masked_items(env, rows, d, dtype, mask):
+    """A target whose bias is a large negative number, as masks are: loss = weight (lse - score).  The score is the mask
+    to within half a step of float32, lse is of the order of 10: two roundings, and one of the product with the weight.  The
+    gradients are those with -inf for a mask, but for what the scores' own rounding does to the others: nothing."""
+    torch, ops = env
+    x, w, t, b, k = make(torch, rows, 333, d, dtype, seed=33, ignored=False, size=0.05)
+    k = k * 0.5
+    t[t < 20] = 77
+    b[5:15] = mask
+    w[5:15] *= 0.5  # (no row's size rests on them)
+    t[0], t[rows // 2] = 7, 9
+    out = b[t.long()] < -1e20
+    inf = torch.where(b < -1e20, torch.full_like(b, -math.inf), b)
+    for got, want in zip(both(ops, x, w, t, b, k), both(ops, x, w, t, inf, k)):
+        exact = k.double() * -b[t.long()].double()
+        assert ((got[0].double() - exact).abs() <= 4 * U32 * exact)[out].all(), (got[0][out][:4].tolist(), exact[out][:4].tolist())
+        assert torch.equal(got[0][~out], want[0][~out])
+        for i in range(1, len(got)):
+            assert torch.equal(got[i], want[i]), i
