@@ -129,25 +129,31 @@ __device__ inline int64_t target_of(const lfm_softmax_args &a, int64_t n)
 
 // -------------------------------------------------------------- operands ---
 
-// Largest finite magnitudes: `parts` blocks for x (rows with a target; their outlier flags are cleared on the way), as many
-// for w (float32 operands alone), as many for g.  Threads take four columns of a row each, LOAD (4, 2, 1) of them at once.
+// Largest finite magnitudes: `parts` blocks for x (rows with a target, and behind the others' the rows without one; their outlier
+// flags are cleared on the way), as many for w (float32 operands alone), as many for g.  Threads take four columns of a row each,
+// LOAD (4, 2, 1) of them at once.
 template <typename T, int LOAD>
 __global__ __launch_bounds__(256) void largest_kernel(lfm_softmax_args a, int parts, float *largest, int tensors, uint8_t *outlier)
 {
     const int which = blockIdx.x / parts, part = blockIdx.x % parts;
-    float m = 0.0f;
+    float m = 0.0f, rest = 0.0f;  // rest: rows of x without a target
     if (which < 2 && tensors == 3) {
         const T *p = (const T *)(which ? a.table : a.hidden);
         const int64_t rows = which ? a.vocab : a.rows, stride = which ? a.table_stride : a.hidden_stride;
         const int groups = (a.d + 3) / 4, per = 256 / groups, tr = (int)threadIdx.x / groups, c = ((int)threadIdx.x - tr * groups) * 4;
-        auto look = [&](float v) { if (fabsf(v) < INFINITY) m = fmaxf(m, fabsf(v)); };
+        auto look = [&](float v, bool counts) {
+            const float s = fabsf(v) < INFINITY ? fabsf(v) : 0.0f;
+            m = fmaxf(m, counts ? s : 0.0f);
+            rest = fmaxf(rest, counts ? 0.0f : s);
+        };
         const int64_t step = (int64_t)parts * per;
         if (tr < per)
 #pragma unroll 4
             for (int64_t r = (int64_t)part * per + tr; r < rows; r += step) {
+                bool counts = true;
                 if (!which) {
                     if (c == 0) outlier[r] = 0;
-                    if (target_of(a, r) < 0) continue;
+                    counts = target_of(a, r) >= 0;
                 } else if (removed(a.bias, r))
                     continue;
                 const T *q = p + r * stride + c;
@@ -156,7 +162,7 @@ __global__ __launch_bounds__(256) void largest_kernel(lfm_softmax_args a, int pa
                     if (c + j >= a.d) break;
                     const Vec<T, LOAD> v = *(const Vec<T, LOAD> *)(q + j);
 #pragma unroll
-                    for (int i = 0; i < LOAD; ++i) look((float)v.v[i]);
+                    for (int i = 0; i < LOAD; ++i) look((float)v.v[i], counts);
                 }
             }
     } else {
@@ -166,11 +172,19 @@ __global__ __launch_bounds__(256) void largest_kernel(lfm_softmax_args a, int pa
             if (v < INFINITY) m = fmaxf(m, v);
         }
     }
-    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-    __shared__ float s[4];
-    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = m;
+    for (int o = 32; o; o >>= 1) {
+        m = fmaxf(m, __shfl_xor(m, o));
+        rest = fmaxf(rest, __shfl_xor(rest, o));
+    }
+    __shared__ float s[2][4];
+    if ((threadIdx.x & 63) == 0) {
+        s[0][threadIdx.x >> 6] = m;
+        s[1][threadIdx.x >> 6] = rest;
+    }
     __syncthreads();
-    if (threadIdx.x == 0) largest[blockIdx.x] = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+    const int i = threadIdx.x;
+    if (i == 0 || (i == 1 && which == 0 && tensors == 3))
+        largest[i ? tensors * parts + part : (int)blockIdx.x] = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
 }
 
 // k with max 2^k in [2^13, 2^14); 0 for an empty or all-zero operand
@@ -184,7 +198,7 @@ __device__ inline int exponent_for(float largest)
 
 struct PackArgs {
     lfm_softmax_args a;
-    const float *largest;  // parts values for x, w and g, or NULL: no scales are wanted
+    const float *largest;  // parts values for x, w, g and x's rows without a target (or for g alone), or NULL: no scales are wanted
     int parts, tensors;
     Scales *scales;
     void *x, *w;           // packed [rows + the outliers' flags], NULL: that operand is used where it is
@@ -196,21 +210,21 @@ struct PackArgs {
 template <typename T, typename E, int NS, int LOAD>
 __global__ __launch_bounds__(256) void pack_kernel(PackArgs p, int dp, int width)
 {
-    __shared__ int ks[3];
+    __shared__ float ms[4];
+    int kx = 0, kw = 0;
     if (p.largest) {
-        if (threadIdx.x < 192) {
-            const int which = threadIdx.x >> 6, lane = threadIdx.x & 63;
-            float m = 0.0f;
-            if (p.tensors == 3 || which == 2)
-                for (int i = lane; i < p.parts; i += 64) m = fmaxf(m, p.largest[(p.tensors == 3 ? which : 0) * p.parts + i]);
-            for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-            int k = which < 2 ? exponent_for(m) : 14 - exponent_for(m);
-            if (which == 2 && !(m > 0.0f)) k = 0;
-            if (lane == 0) ks[which] = k;
-        }
+        const int which = threadIdx.x >> 6, lane = threadIdx.x & 63;
+        float m = 0.0f;
+        if (p.tensors == 3 || which == 2)
+            for (int i = lane; i < p.parts; i += 64) m = fmaxf(m, p.largest[(p.tensors == 3 ? which : 0) * p.parts + i]);
+        for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+        if (lane == 0) ms[which] = m;
         __syncthreads();
+        // the rows with a target set x's scale; where none holds anything, the others do
+        kx = exponent_for(ms[0] > 0.0f ? ms[0] : ms[3]);
+        kw = exponent_for(ms[1]);
         if (blockIdx.x == 0 && threadIdx.x == 0) {
-            Scales s = {ks[0], ks[1], ks[2], 0};
+            Scales s = {kx, kw, ms[2] > 0.0f ? 14 - exponent_for(ms[2]) : 0, 0};
             *p.scales = s;
         }
     }
@@ -238,7 +252,7 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs p, int dp, int width
 #pragma unroll
             for (int j = 0; j < 8; ++j) hi[j] = (E)v[j];
         } else {
-            const int k = ks[is_x ? 0 : 1];
+            const int k = is_x ? kx : kw;
             bool fits = true;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -1332,7 +1346,7 @@ Space space_for(const Plan &p, int64_t rows, int64_t vocab, bool grad, void *ws)
         return s;
     }
     s.scales = c.take<Scales>(1);
-    s.largest = c.take<float>(3 * MAX_PARTS);
+    s.largest = c.take<float>(4 * MAX_PARTS);
     s.outlier = c.take<uint8_t>(rows);
     s.x = c.take<uint16_t>(rows * p.ns * p.dp);
     s.w = c.take<uint16_t>(vocab * p.ns * p.dp);

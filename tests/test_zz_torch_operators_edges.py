@@ -5,7 +5,7 @@ import math
 
 import pytest
 
-from tests.test_zz_torch_operators import U32, env, make  # noqa: F401  (env is a fixture)
+from tests.test_zz_torch_operators import U32, env, make, near, reference  # noqa: F401  (env is a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -88,3 +88,30 @@ def test_targets_that_are_masked_items(env, rows, d, dtype, mask):
         assert torch.equal(got[0][~out], want[0][~out])
         for i in range(1, len(got)):
             assert torch.equal(got[i], want[i]), i
+
+
+# -------------------------------------------------------- rows without target ---
+
+def lse_bound(torch, x, w, b):
+    """(lse, bound) in 64 bits, a piece of the rows at a time."""
+    values, bounds = [], []
+    for lo in range(0, x.shape[0], 256):
+        t = torch.zeros(min(256, x.shape[0] - lo), dtype=torch.int64, device="cuda")
+        value, bound = reference(torch, x[lo:lo + 256], w, t, b, None)
+        values.append(value[1])
+        bounds.append(bound[1])
+    return torch.cat(values), torch.cat(bounds)
+
+
+@pytest.mark.parametrize("rows, vocab, d", [(3, 333, 40), (7, 900, 50), (90, 333, 64), (2500, 400, 40), (60, 300, 300)])
+def test_batches_without_any_target(env, rows, vocab, d):
+    """Tiny rows against a large table with nothing to train on: lse keeps its precision."""
+    torch, ops = env
+    x, w, t, b, k = make(torch, rows, vocab, d, "f32", seed=36)
+    x, w = x * 1e-6, w * 1e6
+    t[:] = -1
+    value, bound = lse_bound(torch, x, w, b)
+    for got in both(ops, x, w, t, b, k):
+        assert (got[0] == 0).all()
+        near(torch, got[1], value, bound, "lse")
+        assert all((g == 0).all() for g in got[2:])
