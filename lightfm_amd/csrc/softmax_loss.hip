@@ -113,6 +113,25 @@ __device__ inline Derived derive(const Scales *s)
     return d;
 }
 
+// A row without a target that does not fit x's scale has one of its own: `code` = OWN_SCALE + k, the score being matrix units 2^-k,
+// and no factor.  Beside 0, x's scale, it can be NOT_FINITE: then the row's scores are not wanted.  Loss of 4096 rows x 20011 x 64,
+// a third of them such rows: 88 us, without any 63 (scored one by one in the join: 6100).
+constexpr int16_t OWN_SCALE = 1024, NOT_FINITE = 0x7fff;
+
+__device__ inline bool has_own_scale(int16_t code) { return code != 0 && code != NOT_FINITE; }
+
+__device__ inline Derived derived_from(float c)
+{
+    int e;
+    frexpf(c, &e);  // c = LOG2E 2^-k
+    return {c, 1 - e, 1.0f, -3.3e38f / fmaxf(c, 1.0f)};
+}
+
+__device__ inline Derived derive_row(const Derived &all, int16_t code)
+{
+    return has_own_scale(code) ? derived_from(ldexpf(LOG2E, OWN_SCALE - code)) : all;
+}
+
 __device__ inline float bias_units(float b, const Derived &d)
 {
     return fabsf(b) < INFINITY ? fminf(fmaxf(ldexpf(b, d.k), d.low), -d.low) : b;
@@ -129,11 +148,11 @@ __device__ inline int64_t target_of(const lfm_softmax_args &a, int64_t n)
 
 // -------------------------------------------------------------- operands ---
 
-// Largest finite magnitudes: `parts` blocks for x (rows with a target, and behind the others' the rows without one; their outlier
-// flags are cleared on the way), as many for w (float32 operands alone), as many for g.  Threads take four columns of a row each,
+// Largest finite magnitudes: `parts` blocks for x (rows with a target, and behind the others' the rows without one; all rows'
+// codes are cleared on the way), as many for w (float32 operands alone), as many for g.  Threads take four columns of a row each,
 // LOAD (4, 2, 1) of them at once.
 template <typename T, int LOAD>
-__global__ __launch_bounds__(256) void largest_kernel(lfm_softmax_args a, int parts, float *largest, int tensors, uint8_t *outlier)
+__global__ __launch_bounds__(256) void largest_kernel(lfm_softmax_args a, int parts, float *largest, int tensors, int16_t *codes)
 {
     const int which = blockIdx.x / parts, part = blockIdx.x % parts;
     float m = 0.0f, rest = 0.0f;  // rest: rows of x without a target
@@ -152,7 +171,7 @@ __global__ __launch_bounds__(256) void largest_kernel(lfm_softmax_args a, int pa
             for (int64_t r = (int64_t)part * per + tr; r < rows; r += step) {
                 bool counts = true;
                 if (!which) {
-                    if (c == 0) outlier[r] = 0;
+                    if (c == 0) codes[r] = 0;
                     counts = target_of(a, r) >= 0;
                 } else if (removed(a.bias, r))
                     continue;
@@ -201,9 +220,31 @@ struct PackArgs {
     const float *largest;  // parts values for x, w, g and x's rows without a target (or for g alone), or NULL: no scales are wanted
     int parts, tensors;
     Scales *scales;
-    void *x, *w;           // packed [rows + the outliers' flags], NULL: that operand is used where it is
-    uint8_t *outlier;      // [rows]: the row does not fit x's scale (only a row without a target, or one that is not finite)
+    void *x, *w;           // packed, NULL: that operand is used where it is
+    int16_t *codes;        // [rows], see OWN_SCALE
 };
+
+// The scale of a row without a target that is far larger than the rows with one: every thread of the row reads the whole row
+// (from the caches), so that such rows need no pass of their own and cost the others nothing.
+template <typename T, int LOAD>
+__device__ inline int16_t own_scale(const T *row, int d, int kx, int kw, int &k)
+{
+    float m = 0.0f;
+    bool finite = true;
+    for (int c = 0; c < d; c += LOAD) {
+        const Vec<T, LOAD> v = *(const Vec<T, LOAD> *)(row + c);
+#pragma unroll
+        for (int i = 0; i < LOAD; ++i) {
+            const float s = fabsf((float)v.v[i]);
+            finite &= s < INFINITY;
+            m = fmaxf(m, s);
+        }
+    }
+    const int kr = exponent_for(m);
+    if (!finite || !(m > 0.0f) || kr >= kx - 1) return 0;  // (up to twice x's largest still fits)
+    k = kr + kw > K_MOST ? K_MOST - kw : kr;
+    return (int16_t)(OWN_SCALE + k + kw);
+}
 
 // Rows of x and w to the padded, split form, zeros behind d: per row and chunk of `width` columns [hi: width | lo: width]
 // (width = dp up to 256 columns, 256 beyond).  A thread makes 8 elements and reads LOAD (4, 2, 1) of them at once.
@@ -212,6 +253,7 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs p, int dp, int width
 {
     __shared__ float ms[4];
     int kx = 0, kw = 0;
+    bool large = false;  // a row without a target does not fit x's scale
     if (p.largest) {
         const int which = threadIdx.x >> 6, lane = threadIdx.x & 63;
         float m = 0.0f;
@@ -223,6 +265,7 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs p, int dp, int width
         // the rows with a target set x's scale; where none holds anything, the others do
         kx = exponent_for(ms[0] > 0.0f ? ms[0] : ms[3]);
         kw = exponent_for(ms[1]);
+        large = !(ldexpf(ms[3], kx) < 65504.0f);
         if (blockIdx.x == 0 && threadIdx.x == 0) {
             Scales s = {kx, kw, ms[2] > 0.0f ? 14 - exponent_for(ms[2]) : 0, 0};
             *p.scales = s;
@@ -252,7 +295,11 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs p, int dp, int width
 #pragma unroll
             for (int j = 0; j < 8; ++j) hi[j] = (E)v[j];
         } else {
-            const int k = is_x ? kx : kw;
+            int k = is_x ? kx : kw;
+            if (large && is_x && target_of(p.a, r) < 0) {
+                const int16_t code = own_scale<T, LOAD>(src, p.a.d, kx, kw, k);
+                if (code && c == 0) p.codes[r] = code;
+            }
             bool fits = true;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -261,7 +308,7 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs p, int dp, int width
                 hi[j] = (E)f;
                 lo[j] = (E)(f - (float)hi[j]);
             }
-            if (is_x && !fits) p.outlier[r] = 1;
+            if (is_x && !fits) p.codes[r] = NOT_FINITE;
             *(x8 *)(dst + width) = lo;
         }
         *(x8 *)dst = hi;
@@ -477,6 +524,7 @@ struct SweepArgs {
     int64_t rows, vocab;
     const float *bias;
     const Scales *scales;
+    const int16_t *codes;   // rows_kernel, NS == 2: see OWN_SCALE
     const void *targets;    // rows_kernel: [rows], id_bytes wide
     int id_bytes;
     Pieces pieces;
@@ -544,9 +592,10 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, GRAD)) void rows_
     static_assert(!WIDE || St::BLOCKS == 1, "a chunk per tile");
     __shared__ __attribute__((aligned(16))) E tile[2][Tl::SIZE];
     __shared__ __attribute__((aligned(16))) float sb[2][Tl::BV];
+    __shared__ __attribute__((aligned(16))) float raw[2][NS == 2 ? Tl::BV : 4];  // the biases themselves
     __shared__ uint64_t gone[2];  // removed items of a tile
     __shared__ __attribute__((aligned(16))) Strip strips[GRAD ? 4 : 1];
-    const Derived dv = derive(NS == 2 ? a.scales : nullptr);
+    const Derived all = derive(NS == 2 ? a.scales : nullptr);
     const St sm(a.chunks);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
     uint64_t unit = a.pieces.begin(blockIdx.x);
@@ -557,6 +606,8 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, GRAD)) void rows_
         const int nt = (int)(a.pieces.tiles - t0 < left ? a.pieces.tiles - t0 : left);
         unit += nt;
         const int64_t n = (int64_t)owner * 128 + wave * 32 + (lane & 31);
+        const Derived dv = NS == 2 ? derive_row(all, n < a.rows ? a.codes[n] : (int16_t)0) : all;
+        const bool other_units = NS == 2 && __any(dv.c != all.c);
         typename Half<E>::x8 own[NS][DP / 16];
         if (!WIDE) load_owned<E, NS, DP>(own, (const E *)a.x, a.ldx, n, a.rows, dv.owned);
         const int64_t at = n >= a.rows ? -1 : a.id_bytes == 8 ? ((const int64_t *)a.targets)[n] : (int64_t)((const int32_t *)a.targets)[n];
@@ -568,13 +619,14 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, GRAD)) void rows_
             for (int b = 0; b < DP / 32; ++b) out[b] = (f32x16)(0.0f);
 
         Tl t;
-        float next_bias = 0.0f;
+        float next_bias = 0.0f, next_raw = 0.0f;
         bool next_gone = false;
         auto fetch = [&](int i, int j) {
             const int64_t r = (int64_t)(t0 + i) * Tl::BV, v = r + threadIdx.x;
             t.fetch((const E *)a.w + sm.offset(j), a.ldw, r, a.vocab);
             if (j == 0 && threadIdx.x < Tl::BV) {
-                next_bias = v >= a.vocab ? -INFINITY : a.bias ? bias_units(a.bias[v], dv) : 0.0f;
+                next_raw = v >= a.vocab ? -INFINITY : a.bias ? a.bias[v] : 0.0f;
+                next_bias = bias_units(next_raw, all);
                 next_gone = v < a.vocab && next_bias == -INFINITY;
             }
         };
@@ -582,6 +634,7 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, GRAD)) void rows_
             t.store(tile[buf]);
             if (j == 0 && threadIdx.x < Tl::BV) {
                 sb[i & 1][threadIdx.x] = next_bias;
+                if (NS == 2) raw[i & 1][threadIdx.x] = next_raw;
                 const uint64_t mask = __ballot(next_gone);
                 if (threadIdx.x == 0) gone[i & 1] = mask;
             }
@@ -616,6 +669,13 @@ __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, GRAD)) void rows_
                     s[4 * g + 1] = b.y;
                     s[4 * g + 2] = b.z;
                     s[4 * g + 3] = b.w;
+                }
+                if (other_units) {  // a wave in some; what it needs is made here, not kept in registers
+                    float c = dv.c;
+                    asm volatile("" : "+v"(c));
+                    const Derived units = derived_from(c);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) s[j] = bias_units(raw[i & 1][blk * 32 + 8 * (j / 4) + 4 * h + j % 4], units);
                 }
                 if (WIDE) {
                     for (int j = 0; j < sm.chunks; ++j) {
@@ -1035,7 +1095,7 @@ __global__ __launch_bounds__(256) void few_rows_kernel(SweepArgs a, const float 
 struct JoinArgs {
     lfm_softmax_args a;
     const Scales *scales;
-    const uint8_t *outlier;
+    const int16_t *codes;
     Pieces pieces;
     int parts, dp, ns, grad, shifted;
     int few;                // few_rows_kernel: every row has `parts` parts
@@ -1044,14 +1104,6 @@ struct JoinArgs {
     float *row_max, *row_rate, *row_weight;
     int32_t *row_target;
 };
-
-template <typename T>
-__device__ inline float dot_lane(const T *x, const T *w, int d)
-{
-    float s = 0.0f;
-    for (int c = 0; c < d; ++c) s = __builtin_fmaf((float)x[c], (float)w[c], s);
-    return s;
-}
 
 // Sums and maxima over the lanes that share a row: 16 neighbouring ones, or the block's 256
 template <int LANES>
@@ -1088,7 +1140,8 @@ __global__ __launch_bounds__(256) void join_rows_kernel(JoinArgs j)
     const int64_t n = (int64_t)blockIdx.x * (256 / LANES) + (LANES == 256 ? 0 : threadIdx.x / LANES);
     const int lane = threadIdx.x % LANES;
     if (n >= a.rows) return;  // (with 256 lanes: nobody; with 16: all of a row's)
-    const Derived dv = derive(j.ns == 2 ? j.scales : nullptr);
+    const int16_t code = j.ns == 2 ? j.codes[n] : (int16_t)0;
+    const Derived dv = derive_row(derive(j.ns == 2 ? j.scales : nullptr), code);
     const uint32_t owner = (uint32_t)(n / 128);
     const int splits = j.few ? j.parts : (int)(j.pieces.last_block(owner) - j.pieces.first_block(owner)) + 1;
     const int64_t t = target_of(a, n);
@@ -1125,25 +1178,8 @@ __global__ __launch_bounds__(256) void join_rows_kernel(JoinArgs j)
     // (m says nothing about a row of NaN, which no maximum takes in: its sum does)
     float lse = sum != sum ? sum : sum == 0.0f ? -INFINITY : m <= dv.low * 0.999f ? -3.402823466e38f : ldexpf(m, -dv.k) + (logf(sum) - P_SHIFT * LN2);
     const float other = sum == 0.0f ? 1.0f : l / sum;  // 1 - p[target]
-    const bool odd = j.ns == 2 && j.outlier[n];
-    if (odd) {  // a row beyond x's scale: not finite, or without a target and far larger than the others
-        float finite = 0.0f;
-        for (int c = lane; c < a.d; c += LANES) finite = fmaxf(finite, fabsf((float)x[c]) < INFINITY ? 0.0f : 1.0f);
-        lse = NAN;
-        if (row_max<LANES>(finite, shared) == 0.0f) {
-            float top = -INFINITY, mass = 0.0f;
-            for (int64_t v = lane; v < a.vocab; v += LANES) {
-                if (removed(a.bias, v)) continue;
-                const float s = dot_lane(x, (const T *)a.table + v * a.table_stride, a.d) + (a.bias ? a.bias[v] : 0.0f);
-                const float up = fmaxf(top, s);
-                if (up > -INFINITY) mass = mass * expf(top - up) + expf(s - up);
-                top = up;
-            }
-            const float up = row_max<LANES>(top, shared);
-            mass = row_sum<LANES>(top > -INFINITY ? mass * expf(top - up) : 0.0f, shared);
-            lse = up + logf(mass);
-        }
-    }
+    const bool odd = code == NOT_FINITE;
+    if (odd) lse = NAN;
     if (odd && t >= 0) loss = NAN;
     loss = t < 0 ? 0.0f : g * loss;
     if (lane == 0 && blockIdx.y == 0) {
@@ -1326,7 +1362,7 @@ Plan plan_for(int64_t rows, int64_t vocab, int d, int dtype, bool grad)
 struct Space {
     Scales *scales;
     float *largest;
-    uint8_t *outlier;
+    int16_t *codes;
     void *x, *w;
     float *pm, *pl, *po, *pw, *pb;
     float *row_max, *row_rate, *row_weight;
@@ -1347,7 +1383,7 @@ Space space_for(const Plan &p, int64_t rows, int64_t vocab, bool grad, void *ws)
     }
     s.scales = c.take<Scales>(1);
     s.largest = c.take<float>(4 * MAX_PARTS);
-    s.outlier = c.take<uint8_t>(rows);
+    s.codes = c.take<int16_t>(rows);
     s.x = c.take<uint16_t>(rows * p.ns * p.dp);
     s.w = c.take<uint16_t>(vocab * p.ns * p.dp);
     const int64_t parts = rows * p.rows.most(), shared = (int64_t)p.table.blocks * 2 * 128;
@@ -1474,14 +1510,14 @@ hipError_t run(const lfm_softmax_args &a, bool grad, void *ws, hipStream_t st)
     pk.scales = s.scales;
     pk.x = x_there ? nullptr : s.x;
     pk.w = w_there ? nullptr : s.w;
-    pk.outlier = s.outlier;
+    pk.codes = s.codes;
     const int64_t most = NS == 2 ? (a.rows > a.vocab ? a.rows : a.vocab) * a.d : a.rows;
     pk.parts = (int)(ceil_div(most, 4096) < MAX_PARTS ? ceil_div(most, 4096) : MAX_PARTS);
     if (scales) {
         const dim3 grid((unsigned)(pk.tensors * pk.parts));
-        if (wide) largest_kernel<T, 4><<<grid, 256, 0, st>>>(a, pk.parts, s.largest, pk.tensors, s.outlier);
-        else if (two) largest_kernel<T, 2><<<grid, 256, 0, st>>>(a, pk.parts, s.largest, pk.tensors, s.outlier);
-        else largest_kernel<T, 1><<<grid, 256, 0, st>>>(a, pk.parts, s.largest, pk.tensors, s.outlier);
+        if (wide) largest_kernel<T, 4><<<grid, 256, 0, st>>>(a, pk.parts, s.largest, pk.tensors, s.codes);
+        else if (two) largest_kernel<T, 2><<<grid, 256, 0, st>>>(a, pk.parts, s.largest, pk.tensors, s.codes);
+        else largest_kernel<T, 1><<<grid, 256, 0, st>>>(a, pk.parts, s.largest, pk.tensors, s.codes);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     if (scales || pk.x || pk.w) {
@@ -1499,6 +1535,7 @@ hipError_t run(const lfm_softmax_args &a, bool grad, void *ws, hipStream_t st)
     w.w = w_there ? a.table : s.w;
     w.ldw = w_there ? a.table_stride : NS * p.dp;
     w.scales = s.scales;
+    w.codes = s.codes;
     w.pieces = p.rows;
     w.parts = (int)p.rows.most();
     w.dp = p.dp;
@@ -1518,7 +1555,7 @@ hipError_t run(const lfm_softmax_args &a, bool grad, void *ws, hipStream_t st)
     BY_WIDTH(p.dp, ROWS)
     if (e != hipSuccess) return e;
     j.scales = s.scales;
-    j.outlier = s.outlier;
+    j.codes = s.codes;
     j.pieces = p.rows;
     j.parts = w.parts;
     j.dp = p.dp;

@@ -103,6 +103,60 @@ def lse_bound(torch, x, w, b):
     return torch.cat(values), torch.cat(bounds)
 
 
+@pytest.mark.parametrize("base, size", [(1.0, 20.0), (1.0, 1e4), (1.0, 1e30), (1e-18, 1e18), (1e-18, 1e12)])
+@pytest.mark.parametrize("rows, vocab, d", [(40, 2003, 64), (90, 333, 50), (40, 500, 300), (2500, 700, 64)])
+def test_large_rows_without_target(env, rows, vocab, d, base, size):
+    """Finite rows without a target, far larger than the rows with one: their lse is right, the others keep their bits."""
+    torch, ops = env
+    x, w, t, b, k = make(torch, rows, vocab, d, "f32", seed=34, ignored=False)
+    x *= base
+    b[vocab // 2] = -math.inf
+    t[t == vocab // 2] = 1
+    out = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    out[::3] = True
+    out[rows - 1] = True
+    t[out] = -1
+    clean = both(ops, torch.where(out[:, None], torch.zeros_like(x), x), w, t, b, k)
+    x = torch.where(out[:, None], x * size, x)
+    x[3] = x[3] * 0 + 2.0 ** -100
+    x[6] = 0.0
+    x[9, d - 1] = float("nan")
+    lost = torch.isnan(x).any(1)
+    value, bound = lse_bound(torch, torch.where(lost[:, None], torch.zeros_like(x), x), w, b)
+    for got, want in zip(both(ops, x, w, t, b, k), clean):
+        for i in range(len(got)):
+            if i != 1:
+                assert torch.equal(got[i], want[i]), i
+        assert torch.equal(got[1][~out], want[1][~out])
+        assert torch.isnan(got[1][lost]).all()
+        near(torch, got[1][~lost], value[~lost], bound[~lost], "lse")
+
+
+@pytest.mark.parametrize("d", [64, 300])
+def test_large_rows_without_target_cost_no_more_than_others(env, d):
+    """A padded batch whose padding holds large values takes the time of one whose padding is zero (a third of the rows here;
+    scored apart from the sweep they cost tens of times the batch)."""
+    torch, ops = env
+    x, w, t, b, k = make(torch, 4096, 20011, d, "f32", seed=35, ignored=False)
+    out = torch.arange(4096, device="cuda") % 3 == 0
+    t[out] = -1
+    zero, large = torch.where(out[:, None], torch.zeros_like(x), x), torch.where(out[:, None], x * 1e3, x)
+
+    def best(x):
+        ops.softmax_loss(x, w, t, bias=b, weights=k)
+        times = []
+        for _ in range(5):
+            one, two = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            one.record()
+            ops.softmax_loss(x, w, t, bias=b, weights=k)
+            two.record()
+            torch.cuda.synchronize()
+            times.append(one.elapsed_time(two))
+        return min(times)
+
+    assert best(large) <= 2.0 * best(zero)
+
+
 @pytest.mark.parametrize("rows, vocab, d", [(3, 333, 40), (7, 900, 50), (90, 333, 64), (2500, 400, 40), (60, 300, 300)])
 def test_batches_without_any_target(env, rows, vocab, d):
     """Tiny rows against a large table with nothing to train on: lse keeps its precision."""
