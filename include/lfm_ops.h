@@ -46,9 +46,10 @@ const char *lfm_ops_last_error(void);
  * A bias may be a large negative number instead, as masks are: scores below -2^67 (float32 operands; -2^127 in half precision) may
  * be cut there, where their probability is 0 beside any other.  The loss of a target so masked is the uncut score's; in a row
  * where nothing else is left, cut scores count as equal and lse is float32's lowest value.
- * float32 operands keep 22 bits and a floor of 2^-39 of the largest magnitude of hidden (rows with a target; all
- * rows where none has one) or table (items not removed); the terms q of d_table keep 22 bits and an absolute error of 2^-38 of the largest weight.  At most 2^27 rows and
- * 2^30 items. */
+ * float32 operands keep 22 bits and a floor of 2^-39 of the largest magnitude of hidden (rows with a target; all rows where none
+ * has one) or table (items not removed); the terms q of d_table keep 22 bits and an absolute error of 2^-38 of the largest weight,
+ * the terms of d_hidden 22 bits and 2^-32 of the row's largest.  In half precision the terms of both are rounded to the operands'
+ * type before they are summed (in float32).  At most 2^27 rows and 2^30 items. */
 typedef struct lfm_softmax_args {
     const void *hidden, *table; /* [rows, d], [vocab, d] of `dtype` */
     const void *targets;        /* [rows] int32 or int64 */

@@ -19,10 +19,13 @@
 // float32 operands: x = 2^-k (hi + lo) with hi, lo in float16 and k from the largest magnitude, a product is hi hi + hi lo +
 // lo hi on the float16 matrix pipe.  An operand keeps 22 bits (and a floor of 2^-39 of the largest magnitude), the product
 // left out is 2^-22 of the term: the size of float32's own rounding over a sum, at a third of the float16 rate instead of the
-// float32 pipe's 1/16.  The probabilities that enter the second product are split the same way: those of dw, scaled so that the
-// largest weight is 2^14, are off by 2^-38 of it at most, so a probability below 2^-17 or so has fewer bits than float32's.  Half-precision operands
-// are multiplied as they are; their probabilities are rounded once to the operands' type (to nearest: at most 2^-8 / 2^-11
-// relative, as much as the result's own rounding).  All sums, maxima and statistics are float32.
+// float32 pipe's 1/16.  The probabilities that enter the second product are split the same way.  Those of dw, scaled so that the
+// largest weight is 2^14, are off by 2^-38 of it at most, so a probability below 2^-17 or so has fewer bits than float32's; those
+// of dx, scaled so that the largest of a row is 2^7 or more, by 2^-32 of that.
+// Half-precision operands are multiplied as they are; their probabilities are rounded once to the operands' type, to nearest: at
+// most 2^-8 (bfloat16) or 2^-11 (float16) relative, as much as the result's own rounding -- where one term rules a sum the two
+// add up.  Of float16's, those below 2^-21 of a row's largest (dx) or 2^-27 of the largest weight (dw) are subnormal: off by
+// 2^-32 and 2^-38 of these.  All sums, maxima and statistics are float32.
 #include "ops_common.hpp"
 
 #include <math.h>

@@ -169,3 +169,67 @@ def test_batches_without_any_target(env, rows, vocab, d):
         assert (got[0] == 0).all()
         near(torch, got[1], value, bound, "lse")
         assert all((g == 0).all() for g in got[2:])
+
+
+# ------------------------------------------------------------------- precision ---
+
+@pytest.mark.parametrize("vocab", [20011, 200003])
+def test_float32_terms_keep_their_bits_in_a_large_vocabulary(env, vocab):
+    """All items but 40 have a bias of -40: their terms, below 2^-45 of the row's largest, vanish in the split halves, so that
+    however large the table is a sum has 40 terms and its bound is as small.  (m a multiple of ln 2 apart: at most 40
+    rescalings.)  d_hidden: a probability is off by its score, twice (own and lse's), its own split 2^-21, the 40 + 40
+    roundings of sum and rescalings.  The tail itself is vocab exp(-40) exp(2 max |s|) of the sum.  Probabilities rounded to one float16 half
+    are outside the bound: asserted as well."""
+    torch, ops = env
+    rows, d = 40, 64
+    x, w, t, b, k = make(torch, rows, vocab, d, "f32", seed=37, ignored=False)
+    x, w = (torch.round(a * 64) / 64 for a in (x, w))  # products and their sums are exact: multiples of 2^-12 below 2^11
+    live = torch.randperm(vocab, generator=torch.Generator().manual_seed(2))[:40].cuda()
+    b[:] = -40.0
+    b[live] = 0.25
+    t = live[torch.arange(rows, device="cuda") % 40]
+    xx, ww, g = x.double(), w.double(), k.double()[:, None]
+    s = xx @ ww[live].t() + 0.25
+    rest = torch.logsumexp(xx @ ww.t() + b.double(), 1)
+    lse = torch.logsumexp(s, 1)
+    tail = float((rest - lse).max()) + 2.0 ** -40
+    assert tail < 2.0 ** -26
+    top = float(s.abs().max())
+    p = torch.exp(s - rest[:, None])
+    hot = (t[:, None] == live[None, :]).double()
+    rel = 2 * 4 * U32 * top + (40 + 64) * U32 + 8 * U32 * (1 + top) + 16 * U32 + tail
+    half, sums = 2.0 ** -21, (40 + 40 + 16) * U32
+    q = g * (p - hot)
+    got = ops.softmax_loss_grad(x, w, t, bias=b, weights=k)
+    bx = (rel + half + sums + tail) * g * ((p + hot) @ ww[live].abs())
+    near(torch, got[2], q @ ww[live], bx + 2 * U32 * (q @ ww[live]).abs() + 2.0 ** -30, "d_hidden")
+    bw = ((rel + half) * g * p + (rel + half + sums) * q.abs() + 2.0 ** -38 * g.max()).t() @ xx.abs()
+    near(torch, got[3][live], q.t() @ xx, bw + 2 * U32 * (q.t() @ xx).abs(), "d_table")
+    # 2^7 p and 2^14 q / 2^e in one half
+    e = math.ceil(math.log2(float(k.max())))
+    single = g * ((p * 128).half().double() / 128 - hot) @ ww[live]
+    assert ((single - q @ ww[live]).abs() > bx).any()
+    single = ((q * 2.0 ** (14 - e)).half().double() * 2.0 ** (e - 14)).t() @ xx
+    assert ((single - q.t() @ xx).abs() > bw).any()
+
+
+@pytest.mark.parametrize("rows", [40, 300])
+def test_float32_gradients_of_unlikely_items(env, rows):
+    """Items of probabilities about 2^-24 to 2^-37: the terms of d_table keep 22 bits and an absolute error of 2^-38 of the largest
+    weight, as lfm_ops.h says."""
+    torch, ops = env
+    x, w, t, b, k = make(torch, rows, 700, 48, "f32", seed=38, ignored=False)
+    rare = torch.arange(200, 600, device="cuda")
+    b[rare] = -math.log(2.0) * (12.0 + 13.0 * torch.rand(400, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)))
+    t[(t >= 200) & (t < 600)] = 11
+    (_, _, _, dw, _), _ = reference(torch, x, w, t, b, k)
+    xx, ww = x.double(), w.double()
+    s = xx @ ww.t() + b.double()
+    q = k.double()[:, None] * torch.exp(s - torch.logsumexp(s, 1)[:, None])
+    ds = (48 * U32 + 2.0 ** -20) * (xx.abs() @ ww.abs().t()) + 8 * U32 * s.abs()
+    rel = ds + ds.max(1).values[:, None] + (700 + 64 + 40) * U32 + 2.0 ** -21 + 2.0 ** -20 + rows * U32
+    bound = (rel * q).t() @ xx.abs() + 2.0 ** -38 * float(k.max()) * xx.abs().sum(0) + 2 * U32 * dw.abs()
+    got = ops.softmax_loss_grad(x, w, t, bias=b, weights=k)[3]
+    near(torch, got[rare], dw[rare], bound[rare], "d_table")
+    # (a floor of 2^-26 of the largest weight would show)
+    assert (q[:, rare].t() @ xx.abs() > 4 * bound[rare]).any(1).float().mean() > 0.9
