@@ -106,9 +106,10 @@ def lib():
         if "torch" not in sys.modules:
             # A torch that is imported later brings its own HIP runtime and looks for "libhsa-runtime64.so" below it; two of
             # THOSE in a process cannot both open the GPU ("No HIP GPUs are available").  Known under that name, too, the one
-            # that this library has loaded serves both.
+            # that this library has loaded serves both.  RTLD_NOLOAD: where the name leads to another installation, nothing is
+            # loaded.
             try:
-                C.CDLL("libhsa-runtime64.so")
+                C.CDLL("libhsa-runtime64.so", mode=os.RTLD_LAZY | os.RTLD_NOLOAD)
             except OSError:
                 pass
         l.lfm_last_error.restype = C.c_char_p
