@@ -8,6 +8,7 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -58,6 +59,11 @@ const at::Tensor &tensor(PyObject *o, const char *name)
 {
     if (!THPVariable_Check(o)) refuse(PyExc_TypeError, "%s must be a torch tensor", name);
     const at::Tensor &t = THPVariable_Unpack(o);
+    // the caller's backward pass would end here without a word
+    if (t.requires_grad() && c10::GradMode::is_enabled() &&
+        PyErr_WarnFormat(PyExc_UserWarning, 2, "%s requires a gradient, which this operator does not record: call the gradient functions, "
+                                               "and this one under torch.no_grad() or with %s.detach()", name, name) < 0)
+        throw Refused();
     if (t.is_neg()) refuse(PyExc_ValueError, "%s is a lazily negated view: call resolve_neg() first", name);
     return t;
 }

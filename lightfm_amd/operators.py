@@ -15,7 +15,8 @@ float32, bfloat16 and float16 tensors; ids are int32 or int64, and an id outside
 loss, gives a zero row and gets no gradient.  Rows may be strided (`t[:, :64]`), the elements of a row are contiguous.
 Everything is enqueued on torch's current stream and nothing is waited for: the calls can be captured into HIP graphs.
 Results and scratch memory come from torch's allocator.  The functions compute on the values alone: they do not record
-autograd history (a training loop calls the gradient functions, or wraps them in its own `autograd.Function`).
+autograd history (a training loop calls the gradient functions, or wraps them in its own `autograd.Function`), and warn
+where a tensor requires a gradient and gradients are being recorded.
 
 Wrong arguments raise ValueError / TypeError like the rest of the package.  There is no CPU fallback.
 """

@@ -181,3 +181,26 @@ def test_python_layer_refuses_wrong_tensors(ops):
         ops.clip_global_norm([x], -1.0)
     with pytest.raises(ValueError, match="no tensors"):
         ops.global_norm([])
+
+
+def test_python_layer_warns_where_autograd_would_be_lost(ops):
+    """A tensor that requires a gradient, while gradients are recorded: the results carry none.  (The calls end at the place
+    of the tensors.)"""
+    import warnings
+
+    import torch
+    x, w = torch.zeros(3, 8), torch.zeros(5, 8, requires_grad=True)
+    t = torch.zeros(3, dtype=torch.int64)
+    calls = [lambda w: ops.softmax_loss(x, w, t), lambda w: ops.softmax_loss_grad(x, w, t), lambda w: ops.embedding_lookup(w, t),
+             lambda w: ops.global_norm([w]), lambda w: ops.clip_global_norm([w], 1.0)]
+    for call in calls:
+        with pytest.warns(UserWarning, match="does not record"), pytest.raises(ValueError, match="no CPU fallback"):
+            call(w)
+        with warnings.catch_warnings():
+            warnings.simplefilter("error")
+            with pytest.raises(UserWarning):
+                call(w)
+            with torch.no_grad(), pytest.raises(ValueError, match="no CPU fallback"):
+                call(w)
+            with pytest.raises(ValueError, match="no CPU fallback"):
+                call(w.detach())
