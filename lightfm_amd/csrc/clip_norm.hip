@@ -133,6 +133,20 @@ __device__ inline void piece_scale(const T *x, T *y, int64_t n, float f)
     for (int64_t i = done + threadIdx.x; i < n; i += 256) y[i] = (T)((float)x[i] * f);
 }
 
+// A factor below float32's normal numbers (values of 1e30 clipped to 1e-10) would have too few bits as one
+template <typename T>
+__device__ inline void piece_scale_far(const T *x, T *y, int64_t n, double f)
+{
+    for (int64_t i = threadIdx.x; i < n; i += 256) y[i] = (T)(float)((double)(float)x[i] * f);
+}
+
+template <typename T>
+__device__ inline void piece_scale(const T *x, T *y, int64_t n, double f)
+{
+    if (f < 1.17549435e-38) piece_scale_far(x, y, n, f);
+    else piece_scale(x, y, n, (float)f);
+}
+
 // Every block adds the partial sums itself (a fixed order) and scales its pieces; block 0 of the first group writes the
 // norm.  in_place with a factor of 1: the values stay as they are, there is nothing to write.
 __global__ __launch_bounds__(256) void scale_kernel(Table t, const double *partial, int partials, double max_norm,
@@ -146,7 +160,7 @@ __global__ __launch_bounds__(256) void scale_kernel(Table t, const double *parti
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
     if (!scale) return;
     // a norm that is not finite (an element was not) scales nothing
-    const float f = norm > max_norm && norm < HUGE_VAL ? (float)(max_norm / norm) : 1.0f;
+    const double f = norm > max_norm && norm < HUGE_VAL ? max_norm / norm : 1.0;
     const int pieces = t.first_piece[t.tensors];
     // From the last piece to the first: what the norm read last is still in the 256 MB cache, and the results, stored past it
     // (piece_scale), do not push the first ones out before the next call: 320 M elements of two types 209 + 396 us before, 177 + 408
@@ -154,7 +168,7 @@ __global__ __launch_bounds__(256) void scale_kernel(Table t, const double *parti
     for (int back = blockIdx.x; back < pieces; back += gridDim.x) {
         const int p = pieces - 1 - back;
         const int i = tensor_of(t, p);
-        if (f == 1.0f && t.x[i] == t.out[i]) continue;
+        if (f == 1.0 && t.x[i] == t.out[i]) continue;
         const int64_t lo = (int64_t)(p - t.first_piece[i]) * PIECE;
         const int64_t n = t.count[i] - lo < PIECE ? t.count[i] - lo : PIECE;
         if (t.dtype[i] == LFM_F32) piece_scale((const float *)t.x[i] + lo, (float *)t.out[i] + lo, n, f);

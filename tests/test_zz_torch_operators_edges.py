@@ -233,3 +233,22 @@ def test_float32_gradients_of_unlikely_items(env, rows):
     near(torch, got[rare], dw[rare], bound[rare], "d_table")
     # (a floor of 2^-26 of the largest weight would show)
     assert (q[:, rare].t() @ xx.abs() > 4 * bound[rare]).any(1).float().mean() > 0.9
+
+
+# ------------------------------------------------------------------------ clip ---
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_clip_by_a_factor_below_the_normal_numbers(env, dtype):
+    """max_norm / norm < 2^-126: the factor has its bits all the same.  Off by a rounding to float32, one to the result's type
+    and the factor's own."""
+    torch, ops = env
+    x = (torch.randn(70001, device="cuda") * 1e30).to(getattr(torch, dtype))
+    norm = math.sqrt(float(x.double().square().sum()))
+    for top in (1e-7, 3e-9):
+        out = [torch.empty_like(x), torch.empty_like(x[1:])]
+        got = ops.clip_global_norm([x, x[1:]], top, out=out)
+        both = math.sqrt(norm ** 2 + float(x[1:].double().square().sum()))
+        assert abs(float(got) - both) <= 2 * U32 * both
+        for o, t in zip(out, (x, x[1:])):
+            want = t.double() * (top / both)
+            near(torch, o, want, (torch.finfo(x.dtype).eps / 2 + 4 * U32) * want.abs() + 2.0 ** -149, "clipped")
