@@ -92,7 +92,9 @@ int lfm_ops_embedding_lookup_grad(const lfm_lookup_args *args, void *workspace, 
 
 /* norm = sqrt(sum of squares over all tensors), summed in float64; out[i] = x[i] * min(1, max_norm / norm).
  * `x`, `out`, `counts`, `dtypes` are HOST arrays of n_tensors entries; out[i] may be x[i] and overlaps nothing else (a
- * tensor that is listed twice cannot be scaled: LFM_EINVAL); out NULL computes the norm alone.  A norm that is not finite is reported in `norm` and leaves the values unscaled. */
+ * tensor that is listed twice cannot be scaled: LFM_EINVAL); out NULL computes the norm alone.  Where an element is not
+ * finite the norm is not either and the values are left unscaled; a finite norm beyond float32 is reported as infinite, and
+ * the values are scaled by it. */
 int lfm_ops_clip_workspace(int64_t n_tensors, const int64_t *counts, int64_t *bytes);
 int lfm_ops_clip_global_norm(int64_t n_tensors, const void *const *x, void *const *out, const int64_t *counts,
                              const int32_t *dtypes, double max_norm, float *norm, void *workspace,

@@ -118,8 +118,9 @@ def global_norm(tensors):
 
 def clip_global_norm(tensors, max_norm, out=None):
     """Scales all tensors (a list or tuple) by min(1, max_norm / norm), norm = global_norm(tensors), in place or into the
-    tensors of `out`, and returns the norm.  A norm that is not finite leaves the values unscaled: look at the returned
-    norm.  A tensor that is written overlaps no other one (ValueError)."""
+    tensors of `out`, and returns the norm.  Where an element is not finite the norm is not either and the values are left
+    unscaled: look at the returned norm (a finite norm beyond float32 is returned as infinite, and scales the values).  A
+    tensor that is written overlaps no other one (ValueError)."""
     if not max_norm >= 0.0:
         raise ValueError("max_norm must not be negative")
     return _ops.clip(tensors, max_norm, tensors if out is None else out)

@@ -252,3 +252,11 @@ def test_clip_by_a_factor_below_the_normal_numbers(env, dtype):
         for o, t in zip(out, (x, x[1:])):
             want = t.double() * (top / both)
             near(torch, o, want, (torch.finfo(x.dtype).eps / 2 + 4 * U32) * want.abs() + 2.0 ** -149, "clipped")
+
+
+def test_clip_of_a_norm_beyond_float32(env):
+    """1e39 from finite values: reported as infinite, the values are scaled by it."""
+    torch, ops = env
+    x = torch.full((100,), 1e38, device="cuda")
+    assert float(ops.clip_global_norm([x], 2.0)) == math.inf
+    near(torch, x, torch.full((100,), 0.2, dtype=torch.float64, device="cuda"), torch.tensor(0.2 * 4 * U32, device="cuda").double(), "clipped")
