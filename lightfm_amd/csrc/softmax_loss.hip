@@ -1328,9 +1328,16 @@ int width_for(int d)
 // As many blocks as run at once, with two exceptions.  A block of a single tile is mostly prologue and parts to join: up to
 // twice as many tiles as the card has compute units are dealt two to a block (gradients of 5276 rows x 712 items x 16 float32: 69 ->
 // 55 us, 3660 x 806 x 188 float16: 115 -> 100).  And where there are nearly as many owners as blocks would be, each has a block
-// to itself and nothing is joined (1003 x 50021 x 100 float16, 391 owners for 512 blocks: 120 -> 106 us; with 301 owners,
-// 2228 x 38507 x 19 float32, the idle slots cost more than the join: 125 -> 145).
-Pieces pieces_for(int64_t owned, int64_t streamed, int bv, int64_t slots)
+// to itself and nothing is joined, if what the other slots then leave undone, tiles (slots - owners) / slots, is less than the
+// join costs, `idle` tiles.  Calls with the gradients, blocks dealt and owners to themselves (us; 512 slots, 256 for 128 columns of float32):
+//   table's sweep   1003 rows (16 tiles) x 391 owners x 100 float16 124 and 109; 2000 (32) x 391 x 32 float16 103 and 101; 2228 (35) x
+//                   420 x 19 float32 159 and 162; 1003 (32) x 210 x 128 float32 163 and 162; 4096 (64) x 450 x 64 float32 420 and
+//                   422; 8192 (128) x 64 bfloat16, 391 owners 342 and 379, 480 411 and 416, 511 435 and 429: even from 4 to 12
+//   rows' sweep     (its join remains, with less to add) 500 items (8 tiles) x 368 owners x 64 bfloat16 109 and 110; 1682 (27) x 409 x 64
+//                   float32 230 and 231; its loss alone x 450 84 and 85; 8000 (125) x 486 260 and 262: even from 2 to 5
+constexpr int IDLE_TABLE = 7, IDLE_ROWS = 3;
+
+Pieces pieces_for(int64_t owned, int64_t streamed, int bv, int64_t slots, int idle)
 {
     Pieces p;
     p.owners = (uint32_t)ceil_div(owned < 1 ? 1 : owned, 128);
@@ -1339,7 +1346,7 @@ Pieces pieces_for(int64_t owned, int64_t streamed, int bv, int64_t slots)
     uint64_t blocks = units / 2 > p.owners ? units / 2 : p.owners;
     if (blocks < 256) blocks = units < 256 ? units : 256;
     if (blocks > (uint64_t)slots) blocks = slots;
-    if (p.owners <= blocks && (uint64_t)p.owners * 100 >= blocks * 70) blocks = p.owners;
+    if (p.owners <= blocks && (uint64_t)p.owners * 100 >= blocks * 70 && p.tiles * (blocks - p.owners) <= idle * blocks) blocks = p.owners;
     p.blocks = (uint32_t)blocks;
     return p;
 }
@@ -1352,13 +1359,13 @@ Plan plan_for(int64_t rows, int64_t vocab, int d, int dtype, bool grad)
     p.chunks = p.dp > 256 ? p.dp / 256 : 1;
     const int w = p.dp > 256 ? 256 : p.dp, bv = p.ns * w <= 128 ? 64 : 32;
     // slots: blocks that run at once on the card's 256 compute units
-    p.rows = pieces_for(rows, vocab, bv, 256 * (p.chunks > 1 ? 1 : waves_for(p.ns, w, grad)));
+    p.rows = pieces_for(rows, vocab, bv, 256 * (p.chunks > 1 ? 1 : waves_for(p.ns, w, grad)), IDLE_ROWS);
     p.few = 0;
     if (takes_few(rows, vocab, d, dtype, grad)) {
         const int64_t want = ceil_div(vocab, 16);  // (a block's lane groups have a few table rows each)
         p.few = (int)(want < 1024 ? want : 1024);
     }
-    p.table = pieces_for(vocab, rows, bv, 256 * (p.chunks > 1 ? 1 : waves_for(p.ns, w, true)));
+    p.table = pieces_for(vocab, rows, bv, 256 * (p.chunks > 1 ? 1 : waves_for(p.ns, w, true)), IDLE_TABLE);
     return p;
 }
 

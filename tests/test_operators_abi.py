@@ -110,6 +110,20 @@ def test_workspace_sizes_hold_at_the_limits(ops):
     assert l.lfm_ops_embedding_grad_workspace(C.c_int64(1), C.c_int64(0), C.c_int64(1), 64, 0, C.byref(need)) == -1
 
 
+def test_long_sweeps_use_the_whole_card(ops):
+    """The parts that a call joins are as many as it has blocks, and their space shows: a step of 8192 rows has as many for 391 * 128
+    items as for 301 * 128, so that the larger table needs no less space (with 128 tiles to an owner, owners with a block to
+    themselves would leave a quarter of the card idle)."""
+    need = C.c_int64()
+
+    def space(rows, vocab):
+        assert ops.lib().lfm_ops_softmax_workspace(C.c_int64(rows), C.c_int64(vocab), 64, 1, 1, C.byref(need)) == 0
+        return need.value
+
+    assert space(8192, 391 * 128) > space(8192, 301 * 128)
+    assert space(391 * 128, 26744) > space(301 * 128, 26744)
+
+
 def _lookup_args(ops, **kw):
     fake = 1 << 20
     values = dict(table=fake, ids=fake, indptr=None, values=None, out=fake, d_out=fake, rows=4, vocab=8, nnz=4,
