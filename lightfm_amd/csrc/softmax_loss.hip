@@ -557,8 +557,17 @@ struct Stream {
     __device__ inline int offset(int j) const { return WIDE ? ((first + j) % chunks) * (NS * DP) : 0; }  // of the j-th chunk
 };
 
-// registers: two waves per SIMD while the operands leave room for it, one beyond
-constexpr int waves_for(int ns, int dp, bool sums) { return ns * dp > (sums ? 192 : 256) ? 1 : 2; }
+// Registers that a block's operands take: the owned rows and the scores' operand ns dp / 4 each, with the sums their operand as many
+// and the result dp / 2.
+constexpr int registers_for(int ns, int dp, bool sums) { return ns * dp / 2 + (sums ? ns * dp / 4 + dp / 2 : 0); }
+
+// Two waves per SIMD while that leaves room for them, one beyond.  With the sums 192 (float32 x 96) fits 256 registers, up to 9
+// of them spilled; at 240 (half precision x 192) the sweeps spilled 39 and 75 as two waves, and one is as fast where the sweeps
+// are long and faster where they are not (gradients, bfloat16, two waves and one, us: 8192 x 26744 x 192 740 and 747, 2048 x 26744 x
+// 192 239 and 226, 1003 x 50021 x 136 232 and 221, 512 x 200003 x 192 418 and 401, 300 x 3000 x 192 51 and 43).  Without the sums
+// more than two would fit at small widths.  float32 beyond 128 columns does not fit one wave either: the rows' sweep spills 16, 312
+// and 68 registers at 192, 256 and more columns.
+constexpr int waves_for(int ns, int dp, bool sums) { return registers_for(ns, dp, sums) > (sums ? 200 : 128) ? 1 : 2; }
 
 // A wave's 32 rows x 32 columns of a result on their way to memory: the products leave a lane 4 neighbouring columns of its row,
 // which written as they are make 16-byte pieces (2-byte ones where rows are not aligned); by way of LDS a row's 32 columns
