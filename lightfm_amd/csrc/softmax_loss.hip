@@ -547,7 +547,8 @@ struct SweepArgs {
 
 // WIDE: more than 256 columns, taken 256 at a time.  The scores add up over the chunks (the owned operand is read again for
 // each, from the caches); a block accumulates the second product of one chunk, blockIdx.y's, which it streams last.  The
-// scores' work is repeated for every chunk of the result: a width that is rare is not worth a second shape of block.
+// scores' work is repeated for every chunk of the result, and the owned operand read again for every tile: gradients of 8192 x 26744
+// x 512 take 11.8 ms in float32 and 6.0 in bfloat16, where 256 columns take 3.6 and 0.86.
 template <typename E, int NS, int DP, bool WIDE>
 struct Stream {
     typedef Tile<E, NS, DP> Tl;
@@ -593,9 +594,9 @@ struct Strip {
 
 // Bound by the matrix pipe and the exponentials together: a block of 32 x 32 scores costs 4 DP matrix cycles per product and
 // about as many for its 16 exponentials, maxima, sums and roundings at DP = 128, which overlap only across the two waves of a
-// SIMD (one wave: 1.5 times the time; three: the operands spill).  8192 x 200003 x 128 bfloat16: 0.90 - 0.94 ms with the
-// gradient, 890 - 930 TFLOP/s, where a product of 8192^3 by the library reaches 1137; 8192 x 26744 x 64 float32: 0.187 ms (300
-// TFLOP/s, each of them three float16 products; the float32 pipe reaches 150).
+// SIMD (one wave: 1.5 times the time; three: the operands spill).  8192 x 200003 x 128 bfloat16: 0.96 ms with the gradient,
+// 880 TFLOP/s, where a product of 8192^3 by the library reaches 1137; 8192 x 26744 x 64 float32: 0.20 ms (280 TFLOP/s, each of
+// them three float16 products; the float32 pipe reaches 150).
 template <typename E, int NS, int DP, bool GRAD, bool WIDE>
 __global__ __launch_bounds__(256, WIDE ? 1 : waves_for(NS, DP, GRAD)) void rows_kernel(SweepArgs a)
 {
@@ -780,7 +781,7 @@ struct RowFacts {
 };
 
 // Bound like rows_kernel, with more to do per score: maximum, rate and target of a score's row come from LDS.  8192 x 200003 x
-// 128 bfloat16: 1.13 ms, 740 TFLOP/s; 8192 x 26744 x 64 float32: 0.220 ms.
+// 128 bfloat16: 1.13 ms, 740 TFLOP/s; 8192 x 26744 x 64 float32: 0.23 ms.
 // ONE: all rows are one tile, which stays in LDS over the owners: few rows, and what counts is how the table is read and dw written
 // (whole calls in us, the general form and this one: 2 x 178913 x 98 bfloat16 110 and 78, 24 x 211856 x 65 float16 100 and 76, 1 x
 // 24380 x 169 float32 77 and 68).  With more tiles the detour by LDS costs registers in the sweep and gains nothing.
