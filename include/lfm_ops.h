@@ -43,9 +43,9 @@ const char *lfm_ops_last_error(void);
  * its loss is infinite and the gradients are the formula's with a probability of 0: -weights[n] table[v] in d_hidden[n]
  * (elements of that row that are not finite count as 0), -weights[n] hidden[n] in d_table[v], -weights[n] in d_bias[v].
  * Rows of hidden and table are contiguous, `*_stride` elements apart; the gradients are dense.
- * A bias may be a large negative number instead, as masks are: scores below -2^67 (float32 operands; -2^127 in half precision) may
- * be cut there, where their probability is 0 beside any other.  The loss of a target so masked is the uncut score's; in a row
- * where nothing else is left, cut scores count as equal and lse is float32's lowest value.
+ * A bias may be a large negative number instead, as masks are.  Biases beyond +-2^67 (float32 operands; +-2^127 in half
+ * precision) may be cut there: below, the probability is 0 beside any other score, and the loss of a target so masked is the
+ * uncut score's; in a row where nothing else is left, cut scores count as equal and lse is float32's lowest value.
  * float32 operands keep 22 bits and a floor of 2^-39 of the largest magnitude of hidden (rows with a target; all rows where none
  * has one) or table (items not removed); the terms q of d_table keep 22 bits and an absolute error of 2^-38 of the largest weight,
  * the terms of d_hidden 22 bits and 2^-32 of the row's largest.  In half precision the terms of both are rounded to the operands'
